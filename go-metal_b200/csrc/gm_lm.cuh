@@ -1,0 +1,160 @@
+// gm_lm.cuh -- what the language-model operators share: element types, eight-element
+// vectors, the counter-based generator of dropout, and argument checks.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "gm_internal.h"
+
+namespace gm {
+
+// ---- element types: arithmetic is in binary32, one rounding at the store ----
+template <typename T> __device__ __forceinline__ float to_f32(T x);
+template <> __device__ __forceinline__ float to_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Two neighbours of a 16-bit type in one 32-bit word (low half first).
+template <typename T> __device__ __forceinline__ unsigned pack2(float lo, float hi);
+template <> __device__ __forceinline__ unsigned pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+template <> __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&h);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(unsigned w);
+template <> __device__ __forceinline__ float2 unpack2<__half>(unsigned w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(unsigned w) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w)); }
+
+// Eight elements as they lie in memory: one 16-byte word of a 16-bit type, two of fp32.
+template <typename T> struct Raw8 { uint4 a; };
+template <> struct Raw8<float> { uint4 a, b; };
+
+// CACHED: the line may be wanted again soon (table rows of frequent tokens, partial sums);
+// otherwise it is streamed.
+template <typename T, bool CACHED> __device__ __forceinline__ Raw8<T> load8(const T* p) {
+    Raw8<T> r;
+    const uint4* q = reinterpret_cast<const uint4*>(p);
+    r.a = CACHED ? *q : __ldcs(q);
+    if constexpr (sizeof(T) == 4) r.b = CACHED ? q[1] : __ldcs(q + 1);
+    return r;
+}
+
+template <typename T> __device__ __forceinline__ void widen8(const Raw8<T>& r, float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const unsigned w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(w[k]);
+    } else {
+        const unsigned w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 f = unpack2<T>(w[k]);
+            x[2 * k] = f.x;
+            x[2 * k + 1] = f.y;
+        }
+    }
+}
+
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+    uint4* q = reinterpret_cast<uint4*>(p);
+    if constexpr (sizeof(T) == 4) {
+        __stcs(q, make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])));
+        __stcs(q + 1, make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7])));
+    } else {
+        __stcs(q, make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7])));
+    }
+}
+
+// ---- dropout's generator ----
+// Philox-4x32 with ten rounds (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy
+// as 1, 2, 3", SC 2011): counter {element / 8 (64 bits), offset (64 bits)}, key = seed.  The
+// 128 bits of one answer serve eight elements, 16 bits each, so the generator costs a quarter
+// of a multiply-pair per element and round; an element stays when its 16 bits, as a number,
+// reach `cut` = round(p * 65536).  What stays is multiplied by 65536 / (65536 - cut), which
+// makes the expectation exact for the probability that is really used, cut / 65536.
+struct Drop {
+    unsigned k0, k1;                     // seed
+    unsigned o0, o1;                     // offset
+    const unsigned long long* more;      // null, or a device word that is added to the offset
+    unsigned cut;                        // 0: everything stays, no generator
+    float up;
+};
+
+__device__ __forceinline__ void drop_begin(Drop& d) {
+    if (d.cut != 0u && d.more != nullptr) {
+        const unsigned long long o = (((unsigned long long)d.o1 << 32) | d.o0) + *d.more;
+        d.o0 = (unsigned)o;
+        d.o1 = (unsigned)(o >> 32);
+    }
+}
+
+// Bit k: element 8 * block + k stays.
+__device__ __forceinline__ unsigned drop_block(const Drop& d, const unsigned long long block) {
+    unsigned c0 = (unsigned)block, c1 = (unsigned)(block >> 32), c2 = d.o0, c3 = d.o1;
+    unsigned k0 = d.k0, k1 = d.k1;
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const unsigned h0 = __umulhi(0xD2511F53u, c0), l0 = 0xD2511F53u * c0;
+        const unsigned h1 = __umulhi(0xCD9E8D57u, c2), l1 = 0xCD9E8D57u * c2;
+        c0 = h1 ^ c1 ^ k0;
+        c1 = l1;
+        c2 = h0 ^ c3 ^ k1;
+        c3 = l0;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    const unsigned w[4] = {c0, c1, c2, c3};
+    unsigned keep = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        keep |= ((w[k] & 0xffffu) >= d.cut ? 1u : 0u) << (2 * k);
+        keep |= ((w[k] >> 16) >= d.cut ? 1u : 0u) << (2 * k + 1);
+    }
+    return keep;
+}
+
+// Bit k: element first + k stays, for eight elements that may begin inside a block.
+__device__ __forceinline__ unsigned drop_mask8(const Drop& d, const unsigned long long first) {
+    if (d.cut == 0u) return 0xffu;
+    unsigned keep = drop_block(d, first >> 3);
+    const unsigned skip = (unsigned)first & 7u;
+    if (skip != 0u) keep = (keep | (drop_block(d, (first >> 3) + 1) << 8)) >> skip;
+    return keep & 0xffu;
+}
+
+__device__ __forceinline__ bool drop_keeps(const Drop& d, const unsigned long long e) {
+    return d.cut == 0u || ((drop_block(d, e >> 3) >> ((unsigned)e & 7u)) & 1u);
+}
+
+// ---- host side ----
+inline int dtype_bytes(int dtype) { return dtype == GM_F32 ? 4 : dtype == GM_F16 || dtype == GM_BF16 ? 2 : 0; }
+
+// Fills the kernel's form of a dropout argument (null: none).  Returns GM_OK or a code.
+int make_drop(const gm_dropout_t* in, Drop* out);
+
+// A buffer of at least `need` bytes on this device, aligned to `align`; need 0 checks the rest.
+int check_buffer(const Device* d, uintptr_t p, int64_t need, int64_t align, const char* what);
+
+// Rows and columns in [1, 2^31), a row stride that covers the columns, and a size whose byte
+// offsets fit 64 bits with room to spare.
+int check_matrix(int64_t rows, int64_t cols, int64_t ld, const char* what);
+
+// Bytes from a matrix's first element to behind its last one.
+inline int64_t matrix_bytes(int64_t rows, int64_t cols, int64_t ld, int eb) { return rows > 0 ? ((rows - 1) * ld + cols) * eb : 0; }
+
+#define GM_TRY(expr)                      \
+    do {                                  \
+        const int rc__ = (expr);          \
+        if (rc__ != GM_OK) return rc__;   \
+    } while (0)
+
+}  // namespace gm

@@ -37,6 +37,19 @@ class LossScale(C.Structure):
                 ("skipped", C.c_int32), ("last_overflow", C.c_int32)]
 
 
+# element types of the language-model operators
+F32, F16, BF16 = 0, 2, 4
+
+
+class Dropout(C.Structure):
+    _fields_ = [("p", f), ("seed", C.c_uint64), ("offset", C.c_uint64), ("offset_device", u)]
+
+
+class Embedding(C.Structure):
+    _fields_ = [("dtype", i), ("tokens", i64), ("dim", i64), ("vocab", i64), ("ld_table", i64), ("ld_out", i64),
+                ("padding_token", i64), ("scale", f)]
+
+
 RULE_SGD, RULE_ADAM, RULE_RMSPROP, RULE_ADAGRAD, RULE_ADADELTA, RULE_NADAM = range(6)
 
 _SIGS = {
@@ -121,6 +134,10 @@ _SIGS = {
     "gm_lbfgs_set_mode": (i, [u, i]),
     "gm_dot_canonical": (i, [u, u, u, i64, C.POINTER(f)]),
     "gm_dot_canonical_static": (i, [u, u, i64, u, u]),
+    "gm_dropout_async": (i, [u, i, i64, i64, u, i64, u, i64, u, i64, C.POINTER(Dropout)]),
+    "gm_embedding_forward_async": (i, [u, C.POINTER(Embedding), u, u, u, C.POINTER(Dropout)]),
+    "gm_embedding_workspace_bytes": (i64, [C.POINTER(Embedding)]),
+    "gm_embedding_backward_async": (i, [u, C.POINTER(Embedding), u, u, C.POINTER(Dropout), u, i, i, u, i64]),
     "gm_zero1_unique_id": (i, [vp]),
     "gm_zero1_create": (u, [u, vp, i, i]),
     "gm_zero1_destroy": (None, [u]),
@@ -180,6 +197,10 @@ def uarray(values) -> "C.Array":
 def iarray(values) -> "C.Array":
     values = list(values)
     return (C.c_int * len(values))(*values)
+
+
+def dropout(p: float, seed: int, offset: int = 0, offset_device: int = 0) -> Dropout:
+    return Dropout(p=p, seed=seed, offset=offset, offset_device=offset_device)
 
 
 class Device:

@@ -327,6 +327,59 @@ int gm_dot_canonical(uintptr_t device_ptr, uintptr_t a, uintptr_t b, int64_t n, 
 #define GM_DOT_STATIC_MAX_ELEMENTS 67108864LL
 int gm_dot_canonical_static(uintptr_t a, uintptr_t b, int64_t n, uintptr_t out_device, uintptr_t stream);
 
+/* ---- operators at the two ends of a language model ----
+ * No counterpart in the reference.  They make the gradients that the steps above take:
+ * the token embedding and the vocabulary loss (whose gradients are a model's largest
+ * tensors, and one tensor in a tied model), and the dropout between.  All run on the
+ * device's stream, return without waiting, allocate nothing and keep nothing: a call may be
+ * captured into a graph (on gm_device_stream).  Workspaces are the caller's, 256-byte aligned,
+ * and hold nothing between calls; two calls or captured graphs that can run at the same
+ * time need workspaces of their own.  Matrices are row-major with a row stride (ld, in
+ * elements) of at least their columns.  Buffers are read and written only inside the
+ * rows and columns named. */
+
+/* Element types: the codes of memory/tensor.go:12-17, and one more for bfloat16. */
+enum { GM_F32 = 0, GM_F16 = 2, GM_BF16 = 4 };
+
+/* Dropout from a counter-based generator; the mask is never stored.  Element e (row * cols +
+ * col, whatever the strides) is set to zero when 16 bits of Philox-4x32-10 with key `seed`
+ * and counter {e / 8, offset} lie below cut = round(p * 65536), otherwise multiplied by
+ * 65536 / (65536 - cut).  A use of its own (layer, step) takes an offset of its own.
+ * offset_device: 0, or the device address of a uint64_t that is added to `offset` when the
+ * kernel runs, so that a replayed graph can go on. */
+typedef struct {
+    float p;                                     /* 0 <= p <= 1 */
+    uint64_t seed, offset;
+    uintptr_t offset_device;
+} gm_dropout_t;
+
+/* y = residual + dropout(x); residual may be 0 (y = dropout(x)).  The backward pass is the
+ * same call on the gradient with residual 0.  y may be x or residual with the same stride. */
+int gm_dropout_async(uintptr_t device_ptr, int dtype, int64_t rows, int64_t cols, uintptr_t x, int64_t ld_x,
+                     uintptr_t residual, int64_t ld_residual, uintptr_t y, int64_t ld_y,
+                     const gm_dropout_t* dropout);
+
+/* Embedding: out[t, :] = dropout(scale * table[token_t, :]), tokens are int32.  A token
+ * outside [0, vocab) gives a row of zeros and no gradient. */
+typedef struct {
+    int dtype;                                   /* of table, out and dout */
+    int64_t tokens, dim, vocab;
+    int64_t ld_table, ld_out;                    /* strides of table and dtable, of out and dout */
+    int64_t padding_token;                       /* its row takes no gradient; -1: none */
+    float scale;
+} gm_embedding_t;
+int gm_embedding_forward_async(uintptr_t device_ptr, const gm_embedding_t* e, uintptr_t table, uintptr_t tokens,
+                               uintptr_t out, const gm_dropout_t* dropout /* NULL: none */);
+/* dtable[v, :] = scale * sum over t with token_t = v of dropout(dout[t, :]), summed in binary32
+ * in ascending t after a sort of the tokens, no float atomics: the same call gives the same
+ * bits.  grad_dtype is GM_F32 or e->dtype.  accumulate 0 writes every row of the table's
+ * gradient (zeros where no token points); accumulate 1 adds to the rows that tokens point at and
+ * leaves the others untouched.  Sums run in runs of 64 sorted tokens whose sums are then added. */
+int64_t gm_embedding_workspace_bytes(const gm_embedding_t* e);   /* of the backward pass; -1: bad argument */
+int gm_embedding_backward_async(uintptr_t device_ptr, const gm_embedding_t* e, uintptr_t tokens, uintptr_t dout,
+                                const gm_dropout_t* dropout /* NULL: none */, uintptr_t dtable, int grad_dtype,
+                                int accumulate, uintptr_t workspace, int64_t workspace_bytes);
+
 /* ---- ZeRO-1: sharded state + all-gather of updated parameters ---- */
 #define GM_NCCL_UNIQUE_ID_BYTES 128
 int gm_zero1_unique_id(void* out_id /* 128 bytes */);
