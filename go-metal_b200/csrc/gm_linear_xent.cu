@@ -1,0 +1,712 @@
+// gm_linear_xent.cu -- softmax cross entropy over a large vocabulary, straight from hidden
+// states X [N, D] and table W [V, D], without the logits in memory, and both gradients.
+//
+//   l = X W^T,  lse_n = log sum_v exp l_nv,  loss_n = lse_n - l_{n, t_n}
+//   S = softmax(l) - onehot(t),  dX = c S W,  dW = c S^T X,  c = grad_scale * scale / count
+//
+// Forward: one matrix product whose epilogue leaves, per row and tile of 256 vocabulary
+// entries, the maximum and the sum of exponentials (8 bytes for 256 logits), then a small
+// kernel joins them.  Backward: for one piece of the vocabulary after the other the logits
+// are formed again, S goes to the workspace in 16 bits, and two products take it from there;
+// dX is carried from piece to piece in binary32.  8 N D V operations for a training step: 2
+// forward, 2 again for the logits, 4 for the gradients.  Bound by the tensor cores, for a few
+// rows by the read of W.
+//
+// Rows whose target lies outside the vocabulary are left out before all this: an index of the
+// others is built on the device, their hidden states are gathered into the workspace, and the
+// products see only those.  They cost nothing, and what they hold (padding, NaN) goes nowhere.
+//
+// Roundings: S is rounded once to the inputs' type, as the operand of a tensor-core product
+// has to be.  In fp16 it is first multiplied by 2^15 (|S| <= 1), which keeps probabilities
+// down to 2^-29 normal; the factor is taken out in binary32 in the epilogue.
+#include <mutex>
+
+#include "gm_tile_gemm.cuh"
+
+namespace gm {
+
+constexpr int kXentStatusWord = 48;      // of the device's scalars: 1 when a wait of a product ran out
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <typename T> struct Half16;
+template <> struct Half16<__half> { static constexpr bool kBf16 = false; static constexpr float kUp = 32768.0f; };
+template <> struct Half16<__nv_bfloat16> { static constexpr bool kBf16 = true; static constexpr float kUp = 1.0f; };
+
+// Scalars at the workspace's begin.
+struct XentScalars {
+    int count;                // rows with a target
+    unsigned ticket;
+};
+
+__device__ __forceinline__ int up_to(int x, int m) { return (x + m - 1) / m * m; }
+
+// ---------------------------------------------------------------- index and gather
+// rows[i] = the i-th row with a target, target[i] = that target.  One CTA: eight rows per
+// thread and turn, a prefix sum over the CTA.
+constexpr int kIndexThreads = 1024;
+__global__ void __launch_bounds__(kIndexThreads)
+xent_index_kernel(const int* __restrict__ targets, const int n, const int vocab, int* __restrict__ rows, int* __restrict__ target,
+                  XentScalars* __restrict__ sc) {
+    __shared__ int warp_sum[32];
+    __shared__ int carry;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) carry = 0;
+    __syncthreads();
+    for (long long base = 0; base < n; base += kIndexThreads * 8) {
+        int t[8];
+        int mine = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const long long i = base + tid * 8 + k;
+            t[k] = i < n ? __ldg(targets + i) : -1;
+            if (t[k] >= vocab) t[k] = -1;
+            mine += t[k] >= 0;
+        }
+        int scan = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += x;
+        }
+        if (lane == 31) warp_sum[warp] = scan;
+        __syncthreads();
+        if (warp == 0) {
+            int s = warp_sum[lane];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += x;
+            }
+            warp_sum[lane] = s;
+        }
+        __syncthreads();
+        int at = carry + scan - mine + (warp > 0 ? warp_sum[warp - 1] : 0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (t[k] >= 0) {
+                rows[at] = (int)(base + tid * 8 + k);
+                target[at] = t[k];
+                ++at;
+            }
+        __syncthreads();
+        if (tid == 0) carry += warp_sum[31];
+        __syncthreads();
+    }
+    if (tid == 0) { sc->count = carry; sc->ticket = 0u; }
+}
+
+// Gathers the hidden states of the rows with a target, zeroes the rows behind them up to a
+// whole tile, and clears the outputs of rows without a target.  One CTA per row.
+template <typename T>
+__global__ void __launch_bounds__(128)
+xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n, const int dim, const int vocab, const int* __restrict__ targets,
+                   const int* __restrict__ rows, const XentScalars* __restrict__ sc, T* __restrict__ packed, const long long ld_packed,
+                   float* __restrict__ losses, float* __restrict__ lse, T* __restrict__ dhidden, const bool vec, const bool vec_out) {
+    const int r = blockIdx.x, tid = threadIdx.x;
+    const int count = sc->count;
+    const int groups = dim >> 3;
+    const T zero = from_f32<T>(0.0f);
+    if (r < n) {
+        const int t = __ldg(targets + r);
+        if (t < 0 || t >= vocab) {
+            if (losses && tid == 0) { losses[r] = 0.0f; lse[r] = 0.0f; }
+            if (dhidden) {
+                T* to = dhidden + (long long)r * ld;
+                const int from = vec_out ? groups * 8 : 0;
+                if (vec_out)
+                    for (int g = tid; g < groups; g += 128) *reinterpret_cast<uint4*>(to + g * 8) = make_uint4(0u, 0u, 0u, 0u);
+                for (int c = from + tid; c < dim; c += 128) to[c] = zero;
+            }
+        }
+    }
+    if (r >= up_to(count, kTileM)) return;
+    T* to = packed + (long long)r * ld_packed;
+    if (r >= count) {
+        for (int c = tid; c < dim; c += 128) to[c] = zero;
+        return;
+    }
+    const T* from = hidden + (long long)__ldg(rows + r) * ld;
+    if (vec) {
+        for (int g = tid; g < groups; g += 128) *reinterpret_cast<uint4*>(to + g * 8) = __ldcs(reinterpret_cast<const uint4*>(from + g * 8));
+        for (int c = groups * 8 + tid; c < dim; c += 128) to[c] = from[c];
+    } else {
+        for (int c = tid; c < dim; c += 128) to[c] = from[c];
+    }
+}
+
+// ---------------------------------------------------------------- epilogues
+constexpr int kGroupM = 8;      // m-tiles walked together: 2,048 rows, so W is read once per 2,048 rows
+
+// Row maximum, sum of exponentials and the target's logit of one tile of logits.
+template <typename T>
+struct StatsOps {
+    static constexpr bool kBf16 = Half16<T>::kBf16;
+    const XentScalars* sc;
+    const int* target;
+    float2* stats;               // [vocabulary tile][row]
+    float* target_logit;
+    int rows_cap, dim, vocab, a0, b0;
+    __device__ __forceinline__ TilePlan plan() const {
+        return {(sc->count + kTileM - 1) / kTileM, (vocab + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, kGroupM};
+    }
+    __device__ __forceinline__ void epilogue(int row, int n, unsigned addr, bool) const {
+        const bool live = row < sc->count;
+        const int c0 = n * kTileN;
+        const int width = vocab - c0 < kTileN ? vocab - c0 : kTileN;
+        const int at = live ? __ldg(target + row) - c0 : -1;
+        float m = -INFINITY, s = 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < width; c += 32) {
+            float v[32];
+            tmem_load32(addr + c, v);
+            if (width - c < 32) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (c + j >= width) v[j] = -INFINITY;
+            }
+            if ((unsigned)(at - c) < 32u) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (at - c == j) target_logit[row] = v[j];
+            }
+            float top = v[0];
+#pragma unroll
+            for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
+            const float next = fmaxf(m, top);
+            const float ref = next == -INFINITY ? 0.0f : next * kLog2e;       // nothing but -inf so far: exponentials are zero
+            float a0_ = 0.0f, a1_ = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                a0_ += exp2f(fmaf(v[j], kLog2e, -ref));
+                a1_ += exp2f(fmaf(v[j + 1], kLog2e, -ref));
+            }
+            s = fmaf(s, exp2f(fmaf(m, kLog2e, -ref)), a0_ + a1_);
+            m = next;
+        }
+        if (live) stats[(long long)n * rows_cap + row] = make_float2(m, s);
+    }
+};
+
+// S of one tile, rounded to 16 bits, into the workspace; zeros behind the last row and column.
+template <typename T>
+struct SoftmaxGradOps {
+    static constexpr bool kBf16 = Half16<T>::kBf16;
+    const XentScalars* sc;
+    const int* target;
+    const int* rows;
+    const float* lse;            // by row of the caller
+    T* ds;
+    long long ld_ds;
+    int dim, v0, v1, a0, b0;
+    __device__ __forceinline__ TilePlan plan() const {
+        return {(sc->count + kTileM - 1) / kTileM, (v1 - v0 + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, kGroupM};
+    }
+    __device__ __forceinline__ void epilogue(int row, int n, unsigned addr, bool) const {
+        const bool live = row < sc->count;
+        const int c0 = v0 + n * kTileN;
+        const int width = live ? (v1 - c0 < kTileN ? v1 - c0 : kTileN) : 0;
+        const int at = live ? __ldg(target + row) - c0 : -1;
+        const float ref = live ? lse[__ldg(rows + row)] * kLog2e : 0.0f;
+        T* to = ds + (long long)row * ld_ds + n * kTileN;
+#pragma unroll 1
+        for (int c = 0; c < kTileN; c += 32) {
+            float v[32];
+            tmem_load32(addr + c, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                v[j] = exp2f(fmaf(v[j], kLog2e, -ref));
+                v[j] = c + j < width ? v[j] * Half16<T>::kUp : 0.0f;
+            }
+            if ((unsigned)(at - c) < 32u) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (at - c == j) v[j] -= Half16<T>::kUp;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+                *reinterpret_cast<uint4*>(to + c + j) =
+                    make_uint4(pack2<T>(v[j], v[j + 1]), pack2<T>(v[j + 2], v[j + 3]), pack2<T>(v[j + 4], v[j + 5]), pack2<T>(v[j + 6], v[j + 7]));
+        }
+    }
+};
+
+// What both gradient products multiply by.
+struct GradScale {
+    const float* scale;          // device scalar (the loss scale), or null
+    float grad_scale;
+    int mean;
+    float down;                  // takes out the factor S carries
+    __device__ __forceinline__ float value(int count) const {
+        float c = scale ? __fmul_rn(grad_scale, *scale) : grad_scale;
+        if (mean) c = __fdiv_rn(c, (float)(count > 0 ? count : 1));
+        return c * down;
+    }
+};
+
+// 32 columns of a row to memory in the output's type; cols of them exist.
+template <typename T>
+__device__ __forceinline__ void emit32(T* to, const float (&v)[32], int cols, bool vec, bool add) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+        if (vec && j + 8 <= cols) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = v[j + k];
+            if (add) {
+                float old[8];
+                widen8<T>(load8<T, false>(to + j), old);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = __fadd_rn(old[k], x[k]);
+            }
+            store8<T>(to + j, x);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (j + k < cols) to[j + k] = from_f32<T>(add ? __fadd_rn(to_f32<T>(to[j + k]), v[j + k]) : v[j + k]);
+        }
+    }
+}
+
+// dX: S [rows, piece] times W [piece, D]; carried in binary32 over the pieces, scattered to the
+// caller's rows by the last one.
+template <typename T>
+struct HiddenGradOps {
+    static constexpr bool kBf16 = Half16<T>::kBf16;
+    const XentScalars* sc;
+    const int* rows;
+    float* carried;
+    long long ld_carried;
+    T* out;
+    long long ld_out;
+    GradScale scale;
+    int dim, v0, v1, a0, b0;
+    bool first, last, vec;
+    __device__ __forceinline__ TilePlan plan() const {
+        return {(sc->count + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (v1 - v0 + kTileK - 1) / kTileK, kGroupM};
+    }
+    __device__ __forceinline__ void epilogue(int row, int n, unsigned addr, bool) const {
+        const int count = sc->count;
+        const bool live = row < count;
+        const float c_all = scale.value(count);
+        T* to = live && last ? out + (long long)__ldg(rows + row) * ld_out + n * kTileN : nullptr;
+        float* acc = carried + (long long)row * ld_carried + n * kTileN;
+        const int width = dim - n * kTileN < kTileN ? dim - n * kTileN : kTileN;
+#pragma unroll 1
+        for (int c = 0; c < width; c += 32) {
+            float v[32];
+            tmem_load32(addr + c, v);
+            if (!live) continue;
+            const int cols = width - c < 32 ? width - c : 32;
+            if (!first) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    if (j < cols) {
+                        const float4 x = *reinterpret_cast<const float4*>(acc + c + j);
+                        v[j] = __fadd_rn(x.x, v[j]); v[j + 1] = __fadd_rn(x.y, v[j + 1]);
+                        v[j + 2] = __fadd_rn(x.z, v[j + 2]); v[j + 3] = __fadd_rn(x.w, v[j + 3]);
+                    }
+            }
+            if (last) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = __fmul_rn(v[j], c_all);
+                emit32<T>(to + c, v, cols, vec, false);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    if (j < cols) *reinterpret_cast<float4*>(acc + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            }
+        }
+    }
+};
+
+// dW of a piece: S^T [piece, rows] times X [rows, D].
+template <typename T>
+struct WeightGradOps {
+    static constexpr bool kBf16 = Half16<T>::kBf16;
+    const XentScalars* sc;
+    T* out;
+    long long ld_out;
+    GradScale scale;
+    int dim, v0, v1, a0, b0;
+    bool add, vec;
+    __device__ __forceinline__ TilePlan plan() const {
+        return {(v1 - v0 + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (sc->count + kTileK - 1) / kTileK, kGroupM};
+    }
+    __device__ __forceinline__ void epilogue(int row, int n, unsigned addr, bool empty) const {
+        const bool live = row < v1 - v0;
+        const float c_all = scale.value(sc->count);
+        T* to = out + (long long)(v0 + row) * ld_out + n * kTileN;
+        const int width = dim - n * kTileN < kTileN ? dim - n * kTileN : kTileN;
+#pragma unroll 1
+        for (int c = 0; c < width; c += 32) {
+            float v[32];
+            tmem_load32(addr + c, v);
+            if (!live) continue;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = empty ? 0.0f : __fmul_rn(v[j], c_all);
+            emit32<T>(to + c, v, width - c < 32 ? width - c : 32, vec, add);
+        }
+    }
+};
+
+// ---------------------------------------------------------------- joining the row statistics
+// 32 rows by 8 lanes over the vocabulary tiles; the CTA that finishes last adds up the loss.
+__global__ void __launch_bounds__(256)
+xent_join_kernel(XentScalars* sc, const float2* __restrict__ stats, const int rows_cap, const int tiles, const float* __restrict__ target_logit,
+                 const int* __restrict__ rows, float* __restrict__ losses, float* __restrict__ lse, float* partial, float* __restrict__ total,
+                 const int mean, const int* status) {
+    __shared__ float sm[8][32], ss[8][32];
+    __shared__ int is_last;
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int row = blockIdx.x * 32 + x;
+    const int count = sc->count;
+    float m = -INFINITY, s = 0.0f;
+    if (row < count) {
+        for (int t = y; t < tiles; t += 8) {
+            const float2 p = __ldcs(stats + (long long)t * rows_cap + row);
+            const float next = fmaxf(m, p.x);
+            const float ref = next == -INFINITY ? 0.0f : next * kLog2e;
+            s = fmaf(s, exp2f(fmaf(m, kLog2e, -ref)), p.y * exp2f(fmaf(p.x, kLog2e, -ref)));
+            m = next;
+        }
+    }
+    sm[y][x] = m;
+    ss[y][x] = s;
+    __syncthreads();
+    if (y == 0) {
+        for (int k = 1; k < 8; ++k) {
+            const float next = fmaxf(m, sm[k][x]);
+            const float ref = next == -INFINITY ? 0.0f : next * kLog2e;
+            s = fmaf(s, exp2f(fmaf(m, kLog2e, -ref)), ss[k][x] * exp2f(fmaf(sm[k][x], kLog2e, -ref)));
+            m = next;
+        }
+        float loss = 0.0f;
+        if (row < count) {
+            const float l = m + logf(s);
+            loss = l - target_logit[row];
+            losses[rows[row]] = loss;
+            lse[rows[row]] = l;
+        }
+        for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+        if (x == 0) {
+            partial[blockIdx.x] = loss;
+            __threadfence();
+            is_last = atomicAdd(&sc->ticket, 1u) == gridDim.x - 1;
+        }
+    }
+    __syncthreads();
+    if (!is_last || y != 0) return;
+    __threadfence();
+    double sum = 0.0;
+    for (int b = x; b < (int)gridDim.x; b += 32) sum += (double)((volatile float*)partial)[b];
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (x == 0) {
+        if (*status) sum = NAN;                                   // a wait of the product ran out: say so in the result
+        total[0] = (float)(mean && count > 0 ? sum / count : sum);
+        total[1] = (float)count;
+        sc->ticket = 0u;
+    }
+}
+
+// ---------------------------------------------------------------- host side
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled() {
+    static EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            p = nullptr;
+        }
+        return (EncodeTiled)p;
+    }();
+    return fn;
+}
+
+// A row-major 16-bit matrix in boxes of 64 columns by box_rows, 128-byte swizzle; reads outside give zeros.
+static int make_map(CUtensorMap* map, int dtype, uintptr_t base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+    EncodeTiled fn = encode_tiled();
+    if (!fn) { set_error("the driver does not offer cuTensorMapEncodeTiled"); return GM_ERR_UNSUPPORTED; }
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)kTileK, (cuuint32_t)box_rows};
+    const cuuint32_t one[2] = {1, 1};
+    const CUresult r = fn(map, dtype == GM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void*)base, dims, strides,
+                          box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { set_error("cuTensorMapEncodeTiled failed with %d", (int)r); return GM_ERR_CUDA; }
+    return GM_OK;
+}
+
+// Launches one product with as many CTA pairs as fit at once, at most one per tile.
+template <bool MN_A, bool MN_B, typename Ops>
+static int launch_tiles(Device* d, const CUtensorMap& a, const CUtensorMap& b, const Ops& ops, int64_t max_tiles) {
+    auto kernel = tile_gemm_kernel<MN_A, MN_B, Ops>;
+    static std::mutex mu;
+    static int pairs_of[64] = {0};                   // per device ordinal
+    int pairs;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        int& known = pairs_of[d->ordinal & 63];
+        if (known == 0) {
+            GM_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem));
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)(d->sm_count / 2 * 2));
+            cfg.blockDim = dim3(kGemmThreads);
+            cfg.dynamicSmemBytes = kGemmSmem;
+            cudaLaunchAttribute attr = {};
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            GM_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+            if (n < 1) { set_error("no CTA pair of the matrix product fits the device"); return GM_ERR_UNSUPPORTED; }
+            known = n;
+        }
+        pairs = known;
+    }
+    if (max_tiles < pairs) pairs = (int)max_tiles;
+    kernel<<<(unsigned)pairs * 2, kGemmThreads, kGemmSmem, d->stream>>>(a, b, ops, reinterpret_cast<int*>(d->scalars + kXentStatusWord), d->barrier_budget_cycles);
+    d->launches++;
+    GM_CUDA_CHECK(cudaGetLastError());
+    return GM_OK;
+}
+
+static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+
+constexpr int64_t kPieceTarget = 512LL << 20;        // bytes of S the recommended workspace holds
+
+struct XentSpace {
+    int64_t cap, ld_packed;                          // rows up to a whole tile, stride of the gathered hidden states
+    int64_t scalars, rows, target, packed;           // both passes
+    int64_t stats, target_logit, partial;            // forward
+    int64_t carried, ld_carried, ds, width;          // backward
+    int64_t total;
+};
+
+static XentSpace common_space(const gm_linear_xent_t* h) {
+    XentSpace s = {};
+    s.cap = up256(h->tokens);
+    s.ld_packed = (h->dim + 7) / 8 * 8;
+    s.rows = 256;
+    s.target = s.rows + up256(s.cap * 4);
+    s.packed = s.target + up256(s.cap * 4);
+    s.total = s.packed + up256(s.cap * s.ld_packed * 2);
+    return s;
+}
+
+static XentSpace forward_space(const gm_linear_xent_t* h) {
+    XentSpace s = common_space(h);
+    s.stats = s.total;
+    s.target_logit = s.stats + up256((h->vocab + kTileN - 1) / kTileN * s.cap * 8);
+    s.partial = s.target_logit + up256(s.cap * 4);
+    s.total = s.partial + up256(s.cap / 32 * 4);
+    return s;
+}
+
+// The widest piece of the vocabulary whose S fits `bytes`; width 0 when not even 256 entries do.
+static XentSpace backward_space(const gm_linear_xent_t* h, int64_t bytes) {
+    XentSpace s = common_space(h);
+    const int64_t all = up256(h->vocab);
+    s.ld_carried = s.ld_packed;
+    if (s.total + up256(s.cap * all * 2) <= bytes) {              // one piece: nothing is carried
+        s.width = all;
+        s.carried = s.ds = s.total;
+    } else {
+        s.carried = s.total;
+        s.ds = s.carried + up256(s.cap * s.ld_carried * 4);
+        const int64_t room = bytes - s.ds;
+        s.width = room > 0 ? room / (s.cap * 2) / 256 * 256 : 0;
+        if (s.width > all) s.width = all;
+        // pieces of even size: the last one is not a sliver
+        if (s.width > 0) {
+            const int64_t pieces = (all + s.width - 1) / s.width;
+            s.width = up256((all + pieces - 1) / pieces);
+        }
+    }
+    s.total = s.ds + up256(s.cap * s.width * 2);
+    return s;
+}
+
+static int64_t backward_bytes(const gm_linear_xent_t* h, bool smallest) {
+    const XentSpace s = common_space(h);
+    const int64_t all = up256(h->vocab);
+    int64_t width = smallest ? 256 : kPieceTarget / (s.cap * 2) / 256 * 256;
+    if (width < 256) width = 256;
+    const int64_t whole = s.total + up256(s.cap * all * 2);       // one piece: nothing is carried
+    if (width >= all) return whole;
+    const int64_t pieces = (all + width - 1) / width;
+    width = up256((all + pieces - 1) / pieces);
+    const int64_t pieced = s.total + up256(s.cap * s.ld_packed * 4) + up256(s.cap * width * 2);
+    return pieced < whole ? pieced : whole;
+}
+
+static int check_xent(const gm_linear_xent_t* h) {
+    if (!h) { set_error("loss argument is nil"); return GM_ERR_BAD_ARG; }
+    if (h->dtype != GM_F16 && h->dtype != GM_BF16) { set_error("element type %d is not Float16 or BFloat16", h->dtype); return GM_ERR_BAD_ARG; }
+    GM_TRY(check_matrix(h->tokens, h->dim, h->ld_hidden, "hidden states"));
+    GM_TRY(check_matrix(h->vocab, h->dim, h->ld_weight, "vocabulary table"));
+    if (h->tokens > (1LL << 28) || h->vocab > (1LL << 28) || h->dim > (1LL << 24)) { set_error("%lld tokens, %lld columns or %lld vocabulary entries are too many", (long long)h->tokens, (long long)h->dim, (long long)h->vocab); return GM_ERR_BAD_SIZE; }
+    if (up256(h->tokens) / 256 * (up256(h->vocab) / 256) > 0x3fffffffLL) { set_error("%lld tokens by %lld vocabulary entries are too many", (long long)h->tokens, (long long)h->vocab); return GM_ERR_BAD_SIZE; }
+    if (h->ld_weight % 8) { set_error("the table's row stride %lld is not a multiple of 8 elements", (long long)h->ld_weight); return GM_ERR_BAD_ARG; }
+    return GM_OK;
+}
+
+struct XentCall {
+    Device* d;
+    const gm_linear_xent_t* h;
+    uintptr_t ws;
+    XentSpace s;
+    XentScalars* sc() const { return (XentScalars*)(ws + s.scalars); }
+    int* rows() const { return (int*)(ws + s.rows); }
+    int* target() const { return (int*)(ws + s.target); }
+};
+
+template <typename T>
+static int index_and_gather(const XentCall& c, uintptr_t hidden, uintptr_t targets, float* losses, float* lse, T* dhidden) {
+    const gm_linear_xent_t* h = c.h;
+    xent_index_kernel<<<1, kIndexThreads, 0, c.d->stream>>>((const int*)targets, (int)h->tokens, (int)h->vocab, c.rows(), c.target(), c.sc());
+    c.d->launches++;
+    GM_CUDA_CHECK(cudaGetLastError());
+    const bool vec = hidden % 16 == 0 && h->ld_hidden % 8 == 0;
+    const bool vec_out = (uintptr_t)dhidden % 16 == 0 && h->ld_hidden % 8 == 0;
+    xent_gather_kernel<T><<<(unsigned)c.s.cap, 128, 0, c.d->stream>>>((const T*)hidden, h->ld_hidden, (int)h->tokens, (int)h->dim, (int)h->vocab,
+                                                                     (const int*)targets, c.rows(), c.sc(), (T*)(c.ws + c.s.packed), c.s.ld_packed,
+                                                                     losses, lse, dhidden, vec, vec_out);
+    c.d->launches++;
+    GM_CUDA_CHECK(cudaGetLastError());
+    return GM_OK;
+}
+
+template <typename T>
+static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, uintptr_t targets, float* losses, float* lse, float* total) {
+    const gm_linear_xent_t* h = c.h;
+    const XentSpace& s = c.s;
+    CUtensorMap map_x, map_w;
+    GM_TRY(make_map(&map_x, h->dtype, c.ws + s.packed, s.cap, h->dim, s.ld_packed, kHalf));
+    GM_TRY(make_map(&map_w, h->dtype, weight, h->vocab, h->dim, h->ld_weight, kHalf));
+    GM_TRY(index_and_gather<T>(c, hidden, targets, losses, lse, (T*)nullptr));
+    const int tiles = (int)((h->vocab + kTileN - 1) / kTileN);
+    float2* stats = (float2*)(c.ws + s.stats);
+    float* target_logit = (float*)(c.ws + s.target_logit);
+    const StatsOps<T> ops{c.sc(), c.target(), stats, target_logit, (int)s.cap, (int)h->dim, (int)h->vocab, 0, 0};
+    GM_TRY((launch_tiles<false, false>(c.d, map_x, map_w, ops, s.cap / kTileM * tiles)));
+    xent_join_kernel<<<(unsigned)(s.cap / 32), 256, 0, c.d->stream>>>(c.sc(), stats, (int)s.cap, tiles, target_logit, c.rows(), losses, lse,
+                                                                     (float*)(c.ws + s.partial), total, h->mean, reinterpret_cast<const int*>(c.d->scalars + kXentStatusWord));
+    c.d->launches++;
+    GM_CUDA_CHECK(cudaGetLastError());
+    return GM_OK;
+}
+
+template <typename T>
+static int run_backward(const XentCall& c, uintptr_t hidden, uintptr_t weight, uintptr_t targets, const float* lse, const float* scale_device,
+                        float grad_scale, uintptr_t dhidden, uintptr_t dweight, bool accumulate) {
+    const gm_linear_xent_t* h = c.h;
+    const XentSpace& s = c.s;
+    const uintptr_t packed = c.ws + s.packed, ds = c.ws + s.ds;
+    CUtensorMap x_k, x_mn, w_k, w_mn, ds_k, ds_mn;       // K-major for the logits and dX's S, MN-major for the rest
+    GM_TRY(make_map(&x_k, h->dtype, packed, s.cap, h->dim, s.ld_packed, kHalf));
+    GM_TRY(make_map(&x_mn, h->dtype, packed, s.cap, h->dim, s.ld_packed, kTileK));
+    GM_TRY(make_map(&w_k, h->dtype, weight, h->vocab, h->dim, h->ld_weight, kHalf));
+    GM_TRY(make_map(&w_mn, h->dtype, weight, h->vocab, h->dim, h->ld_weight, kTileK));
+    GM_TRY(make_map(&ds_k, h->dtype, ds, s.cap, s.width, s.width, kHalf));
+    GM_TRY(make_map(&ds_mn, h->dtype, ds, s.cap, s.width, s.width, kTileK));
+    GM_TRY(index_and_gather<T>(c, hidden, targets, nullptr, nullptr, (T*)dhidden));
+    const GradScale scale{scale_device, grad_scale, h->mean, 1.0f / Half16<T>::kUp};
+    const int dim = (int)h->dim, vocab = (int)h->vocab;
+    const int64_t m_tiles = s.cap / kTileM, d_tiles = (h->dim + kTileN - 1) / kTileN;
+    for (int64_t v = 0; v < vocab; v += s.width) {
+        const int v0 = (int)v, v1 = (int)(v + s.width < vocab ? v + s.width : vocab);
+        const int64_t v_tiles = (v1 - v0 + kTileN - 1) / kTileN;
+        const SoftmaxGradOps<T> grad{c.sc(), c.target(), c.rows(), lse, (T*)ds, s.width, dim, v0, v1, 0, v0};
+        GM_TRY((launch_tiles<false, false>(c.d, x_k, w_k, grad, m_tiles * v_tiles)));
+        if (dhidden) {
+            const bool vec = dhidden % 16 == 0 && h->ld_hidden % 8 == 0;
+            const HiddenGradOps<T> ops{c.sc(), c.rows(), (float*)(c.ws + s.carried), s.ld_carried, (T*)dhidden, h->ld_hidden, scale,
+                                       dim, v0, v1, 0, v0, v0 == 0, v1 == vocab, vec};
+            GM_TRY((launch_tiles<false, true>(c.d, ds_k, w_mn, ops, m_tiles * d_tiles)));
+        }
+        if (dweight) {
+            const bool vec = dweight % 16 == 0;
+            const WeightGradOps<T> ops{c.sc(), (T*)dweight, h->ld_weight, scale, dim, v0, v1, 0, 0, accumulate, vec};
+            GM_TRY((launch_tiles<true, true>(c.d, ds_mn, x_mn, ops, v_tiles * d_tiles)));
+        }
+    }
+    return GM_OK;
+}
+
+}  // namespace gm
+
+using namespace gm;
+
+extern "C" {
+
+int64_t gm_linear_xent_workspace_bytes(const gm_linear_xent_t* h, int pass) {
+    if (check_xent(h) != GM_OK) return -1;
+    if (pass < 0 || pass > 2) { set_error("pass %d is not 0, 1 or 2", pass); return -1; }
+    if (pass == 0) return forward_space(h).total;
+    if (pass == 2) return backward_bytes(h, true);
+    const int64_t f = forward_space(h).total, b = backward_bytes(h, false);
+    return f > b ? f : b;
+}
+
+int gm_linear_xent_forward_async(uintptr_t device_ptr, const gm_linear_xent_t* h, uintptr_t hidden, uintptr_t weight, uintptr_t targets,
+                                 uintptr_t losses, uintptr_t lse, uintptr_t total, uintptr_t workspace, int64_t workspace_bytes) {
+    Device* d = as_device(device_ptr);
+    if (!d) return GM_ERR_NIL_DEVICE;
+    GM_TRY(check_xent(h));
+    GM_TRY(check_buffer(d, hidden, matrix_bytes(h->tokens, h->dim, h->ld_hidden, 2), 2, "hidden states"));
+    GM_TRY(check_buffer(d, weight, matrix_bytes(h->vocab, h->dim, h->ld_weight, 2), 16, "vocabulary table"));
+    GM_TRY(check_buffer(d, targets, h->tokens * 4, 4, "targets"));
+    GM_TRY(check_buffer(d, losses, h->tokens * 4, 4, "losses"));
+    GM_TRY(check_buffer(d, lse, h->tokens * 4, 4, "log-sum-exp"));
+    GM_TRY(check_buffer(d, total, 8, 4, "total"));
+    const XentCall c{d, h, workspace, forward_space(h)};
+    if (workspace_bytes < c.s.total) { set_error("workspace of %lld bytes, the call needs %lld", (long long)workspace_bytes, (long long)c.s.total); return GM_ERR_BAD_SIZE; }
+    GM_TRY(check_buffer(d, workspace, c.s.total, 256, "workspace"));
+    DeviceGuard g(d);
+    if (h->dtype == GM_F16) return run_forward<__half>(c, hidden, weight, targets, (float*)losses, (float*)lse, (float*)total);
+    return run_forward<__nv_bfloat16>(c, hidden, weight, targets, (float*)losses, (float*)lse, (float*)total);
+}
+
+int gm_linear_xent_backward_async(uintptr_t device_ptr, const gm_linear_xent_t* h, uintptr_t hidden, uintptr_t weight, uintptr_t targets,
+                                  uintptr_t lse, uintptr_t scale_device, float grad_scale, uintptr_t dhidden, uintptr_t dweight,
+                                  int accumulate, uintptr_t workspace, int64_t workspace_bytes) {
+    Device* d = as_device(device_ptr);
+    if (!d) return GM_ERR_NIL_DEVICE;
+    GM_TRY(check_xent(h));
+    GM_TRY(check_buffer(d, hidden, matrix_bytes(h->tokens, h->dim, h->ld_hidden, 2), 2, "hidden states"));
+    GM_TRY(check_buffer(d, weight, matrix_bytes(h->vocab, h->dim, h->ld_weight, 2), 16, "vocabulary table"));
+    GM_TRY(check_buffer(d, targets, h->tokens * 4, 4, "targets"));
+    GM_TRY(check_buffer(d, lse, h->tokens * 4, 4, "log-sum-exp"));
+    if (scale_device) GM_TRY(check_buffer(d, scale_device, 4, 4, "loss scale"));
+    if (!dhidden && !dweight) { set_error("neither gradient is asked for"); return GM_ERR_NIL_BUFFER; }
+    if (dhidden) GM_TRY(check_buffer(d, dhidden, matrix_bytes(h->tokens, h->dim, h->ld_hidden, 2), 2, "hidden states' gradient"));
+    if (dweight) GM_TRY(check_buffer(d, dweight, matrix_bytes(h->vocab, h->dim, h->ld_weight, 2), 2, "table's gradient"));
+    const int64_t need = backward_bytes(h, true);
+    if (workspace_bytes < need) { set_error("workspace of %lld bytes, the call needs %lld", (long long)workspace_bytes, (long long)need); return GM_ERR_BAD_SIZE; }
+    const XentCall c{d, h, workspace, backward_space(h, workspace_bytes)};
+    GM_TRY(check_buffer(d, workspace, c.s.total, 256, "workspace"));
+    DeviceGuard g(d);
+    if (h->dtype == GM_F16)
+        return run_backward<__half>(c, hidden, weight, targets, (const float*)lse, (const float*)scale_device, grad_scale, dhidden, dweight, accumulate != 0);
+    return run_backward<__nv_bfloat16>(c, hidden, weight, targets, (const float*)lse, (const float*)scale_device, grad_scale, dhidden, dweight, accumulate != 0);
+}
+
+int gm_linear_xent_status(uintptr_t device_ptr) {
+    Device* d = as_device(device_ptr);
+    if (!d) return GM_ERR_NIL_DEVICE;
+    DeviceGuard g(d);
+    int status = 0;
+    GM_CUDA_CHECK(cudaStreamSynchronize(d->stream));
+    GM_CUDA_CHECK(cudaMemcpy(&status, d->scalars + kXentStatusWord, sizeof(int), cudaMemcpyDeviceToHost));
+    if (!status) return GM_OK;
+    GM_CUDA_CHECK(cudaMemset(d->scalars + kXentStatusWord, 0, sizeof(int)));
+    set_error("a wait of the vocabulary loss's matrix products ran out; the outputs of that call are not complete");
+    return GM_ERR_TIMEOUT;
+}
+
+}  // extern "C"

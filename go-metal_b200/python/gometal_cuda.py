@@ -50,6 +50,10 @@ class Embedding(C.Structure):
                 ("padding_token", i64), ("scale", f)]
 
 
+class LinearXent(C.Structure):
+    _fields_ = [("dtype", i), ("tokens", i64), ("dim", i64), ("vocab", i64), ("ld_hidden", i64), ("ld_weight", i64), ("mean", i)]
+
+
 RULE_SGD, RULE_ADAM, RULE_RMSPROP, RULE_ADAGRAD, RULE_ADADELTA, RULE_NADAM = range(6)
 
 _SIGS = {
@@ -138,6 +142,10 @@ _SIGS = {
     "gm_embedding_forward_async": (i, [u, C.POINTER(Embedding), u, u, u, C.POINTER(Dropout)]),
     "gm_embedding_workspace_bytes": (i64, [C.POINTER(Embedding)]),
     "gm_embedding_backward_async": (i, [u, C.POINTER(Embedding), u, u, C.POINTER(Dropout), u, i, i, u, i64]),
+    "gm_linear_xent_workspace_bytes": (i64, [C.POINTER(LinearXent), i]),
+    "gm_linear_xent_forward_async": (i, [u, C.POINTER(LinearXent), u, u, u, u, u, u, u, i64]),
+    "gm_linear_xent_backward_async": (i, [u, C.POINTER(LinearXent), u, u, u, u, u, f, u, u, i, u, i64]),
+    "gm_linear_xent_status": (i, [u]),
     "gm_zero1_unique_id": (i, [vp]),
     "gm_zero1_create": (u, [u, vp, i, i]),
     "gm_zero1_destroy": (None, [u]),

@@ -380,6 +380,42 @@ int gm_embedding_backward_async(uintptr_t device_ptr, const gm_embedding_t* e, u
                                 const gm_dropout_t* dropout /* NULL: none */, uintptr_t dtable, int grad_dtype,
                                 int accumulate, uintptr_t workspace, int64_t workspace_bytes);
 
+/* Softmax cross entropy over a vocabulary, from hidden states X [tokens, dim] and the table W
+ * [vocab, dim], both fp16 or both bf16, without the logits in memory:
+ *     l = X W^T,  lse = log sum exp l,  loss = lse - l[target]
+ *     dX = c (softmax(l) - onehot) W,  dW (+)= c (softmax(l) - onehot)^T X
+ * with c = grad_scale * (*scale_device, or 1 where that is 0) / (mean ? rows with a target : 1).
+ * scale_device takes the address of a mixed-precision state (gm_mixed_state_device_ptr, whose
+ * first member is the loss scale), so that dW is the fp16 gradient gm_mixed_step_async wants.
+ * targets are int32; a row whose target lies outside [0, vocab) takes no part: its loss, lse and
+ * gradient are 0 and it may hold anything.  losses, lse: one float per row; total: {sum or mean
+ * of the losses, rows with a target} (a mean over no rows is 0).  dX or dW may be 0.
+ * The logits and both gradients are tensor-core products with binary32 sums; softmax - onehot is
+ * rounded to the inputs' type in between.  The same call gives the same bits.
+ * The table's rows begin on 16-byte boundaries (its address, and ld_weight a multiple of 8). */
+typedef struct {
+    int dtype;                                   /* GM_F16 or GM_BF16: X, W, dX, dW */
+    int64_t tokens, dim, vocab;
+    int64_t ld_hidden, ld_weight;                /* strides of X and dX, of W and dW */
+    int mean;                                    /* 1: loss and gradients over the rows with a target; 0: sum */
+} gm_linear_xent_t;
+/* pass 0: the forward pass needs this; 1: enough for both passes, with large pieces of the
+ * vocabulary in the backward pass; 2: the least the backward pass takes (pieces of 256).  The
+ * backward pass uses the largest pieces the given workspace holds; their size changes the order
+ * in which dX is summed.  -1: bad argument. */
+int64_t gm_linear_xent_workspace_bytes(const gm_linear_xent_t* h, int pass);
+int gm_linear_xent_forward_async(uintptr_t device_ptr, const gm_linear_xent_t* h, uintptr_t hidden, uintptr_t weight,
+                                 uintptr_t targets, uintptr_t losses, uintptr_t lse, uintptr_t total,
+                                 uintptr_t workspace, int64_t workspace_bytes);
+int gm_linear_xent_backward_async(uintptr_t device_ptr, const gm_linear_xent_t* h, uintptr_t hidden, uintptr_t weight,
+                                  uintptr_t targets, uintptr_t lse /* of the forward pass */, uintptr_t scale_device,
+                                  float grad_scale, uintptr_t dhidden, uintptr_t dweight, int accumulate_dweight,
+                                  uintptr_t workspace, int64_t workspace_bytes);
+/* Waits for the device's stream; GM_ERR_TIMEOUT when a bounded wait inside one of these
+ * products ran out since the last query (that call's outputs are not complete; a forward
+ * pass reports NaN as its total until the query). */
+int gm_linear_xent_status(uintptr_t device_ptr);
+
 /* ---- ZeRO-1: sharded state + all-gather of updated parameters ---- */
 #define GM_NCCL_UNIQUE_ID_BYTES 128
 int gm_zero1_unique_id(void* out_id /* 128 bytes */);
