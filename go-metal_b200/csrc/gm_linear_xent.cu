@@ -5,8 +5,11 @@
 //   S = softmax(l) - onehot(t),  dX = c S W,  dW = c S^T X,  c = grad_scale * scale / count
 //
 // Forward: one matrix product whose epilogue leaves, per row and tile of 256 vocabulary
-// entries, the maximum and the sum of exponentials (8 bytes for 256 logits), then a small
-// kernel joins them.  Backward: for one piece of the vocabulary after the other the logits
+// entries, the maximum and the sum of exponentials (8 bytes for 256 logits) of all entries but
+// the target's, then a small kernel joins them with the target's logit, which comes from a dot
+// product of its own.  loss = log(1 + sum of the others / the target's) then loses nothing when the
+// model is sure of the target, and the target's logit is as good as binary32 makes it (the
+// tensor cores cut where they add).  Backward: for one piece of the vocabulary after the other the logits
 // are formed again, S goes to the workspace in 16 bits, and two products take it from there;
 // dX is carried from piece to piece in binary32.  8 N D V operations for a training step: 2
 // forward, 2 again for the logits, 4 for the gradients.  Bound by the tensor cores, for a few
@@ -96,12 +99,16 @@ xent_index_kernel(const int* __restrict__ targets, const int n, const int vocab,
 }
 
 // Gathers the hidden states of the rows with a target, zeroes the rows behind them up to a
-// whole tile, and clears the outputs of rows without a target.  One CTA per row.
+// whole tile, and clears the outputs of rows without a target.  One CTA per row.  With
+// target_logit (forward) it also takes the dot product of the row with its target's row of W.
+constexpr int kGatherThreads = 128;
 template <typename T>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kGatherThreads)
 xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n, const int dim, const int vocab, const int* __restrict__ targets,
-                   const int* __restrict__ rows, const XentScalars* __restrict__ sc, T* __restrict__ packed, const long long ld_packed,
+                   const int* __restrict__ rows, const int* __restrict__ target, const XentScalars* __restrict__ sc, T* __restrict__ packed,
+                   const long long ld_packed, const T* __restrict__ weight, const long long ld_weight, float* __restrict__ target_logit,
                    float* __restrict__ losses, float* __restrict__ lse, T* __restrict__ dhidden, const bool vec, const bool vec_out) {
+    __shared__ float warp_sum[kGatherThreads / 32];
     const int r = blockIdx.x, tid = threadIdx.x;
     const int count = sc->count;
     const int groups = dim >> 3;
@@ -114,37 +121,60 @@ xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n
                 T* to = dhidden + (long long)r * ld;
                 const int from = vec_out ? groups * 8 : 0;
                 if (vec_out)
-                    for (int g = tid; g < groups; g += 128) *reinterpret_cast<uint4*>(to + g * 8) = make_uint4(0u, 0u, 0u, 0u);
-                for (int c = from + tid; c < dim; c += 128) to[c] = zero;
+                    for (int g = tid; g < groups; g += kGatherThreads) *reinterpret_cast<uint4*>(to + g * 8) = make_uint4(0u, 0u, 0u, 0u);
+                for (int c = from + tid; c < dim; c += kGatherThreads) to[c] = zero;
             }
         }
     }
     if (r >= up_to(count, kTileM)) return;
     T* to = packed + (long long)r * ld_packed;
     if (r >= count) {
-        for (int c = tid; c < dim; c += 128) to[c] = zero;
+        for (int c = tid; c < dim; c += kGatherThreads) to[c] = zero;
         return;
     }
     const T* from = hidden + (long long)__ldg(rows + r) * ld;
+    const T* w = target_logit ? weight + (long long)__ldg(target + r) * ld_weight : nullptr;
+    float dot = 0.0f;
+    int c0 = 0;
     if (vec) {
-        for (int g = tid; g < groups; g += 128) *reinterpret_cast<uint4*>(to + g * 8) = __ldcs(reinterpret_cast<const uint4*>(from + g * 8));
-        for (int c = groups * 8 + tid; c < dim; c += 128) to[c] = from[c];
-    } else {
-        for (int c = tid; c < dim; c += 128) to[c] = from[c];
+        c0 = groups * 8;
+        for (int g = tid; g < groups; g += kGatherThreads) {
+            const Raw8<T> x = load8<T, false>(from + g * 8);
+            *reinterpret_cast<uint4*>(to + g * 8) = x.a;
+            if (w) {
+                float a[8], b[8];
+                widen8<T>(x, a);
+                widen8<T>(load8<T, true>(w + g * 8), b);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) dot = fmaf(a[k], b[k], dot);
+            }
+        }
+    }
+    for (int c = c0 + tid; c < dim; c += kGatherThreads) {
+        to[c] = from[c];
+        if (w) dot = fmaf(to_f32<T>(from[c]), to_f32<T>(w[c]), dot);
+    }
+    if (!w) return;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if ((tid & 31) == 0) warp_sum[tid >> 5] = dot;
+    __syncthreads();
+    if (tid == 0) {
+        for (int k = 1; k < kGatherThreads / 32; ++k) dot += warp_sum[k];
+        target_logit[r] = dot;
     }
 }
 
 // ---------------------------------------------------------------- epilogues
 constexpr int kGroupM = 8;      // m-tiles walked together: 2,048 rows, so W is read once per 2,048 rows
 
-// Row maximum, sum of exponentials and the target's logit of one tile of logits.
+// Row maximum and sum of exponentials of one tile of logits, the target's left out.
 template <typename T>
 struct StatsOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
     const XentScalars* sc;
     const int* target;
     float2* stats;               // [vocabulary tile][row]
-    float* target_logit;
     int rows_cap, dim, vocab, a0, b0;
     __device__ __forceinline__ TilePlan plan() const {
         return {(sc->count + kTileM - 1) / kTileM, (vocab + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, kGroupM};
@@ -167,7 +197,7 @@ struct StatsOps {
             if ((unsigned)(at - c) < 32u) {
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
-                    if (at - c == j) target_logit[row] = v[j];
+                    if (at - c == j) v[j] = -INFINITY;
             }
             float top = v[0];
 #pragma unroll
@@ -382,11 +412,12 @@ xent_join_kernel(XentScalars* sc, const float2* __restrict__ stats, const int ro
         }
         float loss = 0.0f;
         if (row < count) {
-            const float l = m + logf(s);
-            loss = l - target_logit[row];
+            const float z = target_logit[row];
+            loss = z >= m ? log1pf(s * expf(m - z)) : (m - z) + logf(s + expf(z - m));
             losses[rows[row]] = loss;
-            lse[rows[row]] = l;
+            lse[rows[row]] = z + loss;
         }
+#pragma unroll
         for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
         if (x == 0) {
             partial[blockIdx.x] = loss;
@@ -566,16 +597,17 @@ struct XentCall {
 };
 
 template <typename T>
-static int index_and_gather(const XentCall& c, uintptr_t hidden, uintptr_t targets, float* losses, float* lse, T* dhidden) {
+static int index_and_gather(const XentCall& c, uintptr_t hidden, uintptr_t targets, uintptr_t weight, float* target_logit, float* losses, float* lse,
+                            T* dhidden) {
     const gm_linear_xent_t* h = c.h;
     xent_index_kernel<<<1, kIndexThreads, 0, c.d->stream>>>((const int*)targets, (int)h->tokens, (int)h->vocab, c.rows(), c.target(), c.sc());
     c.d->launches++;
     GM_CUDA_CHECK(cudaGetLastError());
     const bool vec = hidden % 16 == 0 && h->ld_hidden % 8 == 0;
     const bool vec_out = (uintptr_t)dhidden % 16 == 0 && h->ld_hidden % 8 == 0;
-    xent_gather_kernel<T><<<(unsigned)c.s.cap, 128, 0, c.d->stream>>>((const T*)hidden, h->ld_hidden, (int)h->tokens, (int)h->dim, (int)h->vocab,
-                                                                     (const int*)targets, c.rows(), c.sc(), (T*)(c.ws + c.s.packed), c.s.ld_packed,
-                                                                     losses, lse, dhidden, vec, vec_out);
+    xent_gather_kernel<T><<<(unsigned)c.s.cap, kGatherThreads, 0, c.d->stream>>>(
+        (const T*)hidden, h->ld_hidden, (int)h->tokens, (int)h->dim, (int)h->vocab, (const int*)targets, c.rows(), c.target(), c.sc(),
+        (T*)(c.ws + c.s.packed), c.s.ld_packed, (const T*)weight, h->ld_weight, target_logit, losses, lse, dhidden, vec, vec_out);
     c.d->launches++;
     GM_CUDA_CHECK(cudaGetLastError());
     return GM_OK;
@@ -588,11 +620,11 @@ static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
     CUtensorMap map_x, map_w;
     GM_TRY(make_map(&map_x, h->dtype, c.ws + s.packed, s.cap, h->dim, s.ld_packed, kHalf));
     GM_TRY(make_map(&map_w, h->dtype, weight, h->vocab, h->dim, h->ld_weight, kHalf));
-    GM_TRY(index_and_gather<T>(c, hidden, targets, losses, lse, (T*)nullptr));
+    float* target_logit = (float*)(c.ws + s.target_logit);
+    GM_TRY(index_and_gather<T>(c, hidden, targets, weight, target_logit, losses, lse, (T*)nullptr));
     const int tiles = (int)((h->vocab + kTileN - 1) / kTileN);
     float2* stats = (float2*)(c.ws + s.stats);
-    float* target_logit = (float*)(c.ws + s.target_logit);
-    const StatsOps<T> ops{c.sc(), c.target(), stats, target_logit, (int)s.cap, (int)h->dim, (int)h->vocab, 0, 0};
+    const StatsOps<T> ops{c.sc(), c.target(), stats, (int)s.cap, (int)h->dim, (int)h->vocab, 0, 0};
     GM_TRY((launch_tiles<false, false>(c.d, map_x, map_w, ops, s.cap / kTileM * tiles)));
     xent_join_kernel<<<(unsigned)(s.cap / 32), 256, 0, c.d->stream>>>(c.sc(), stats, (int)s.cap, tiles, target_logit, c.rows(), losses, lse,
                                                                      (float*)(c.ws + s.partial), total, h->mean, reinterpret_cast<const int*>(c.d->scalars + kXentStatusWord));
@@ -614,7 +646,7 @@ static int run_backward(const XentCall& c, uintptr_t hidden, uintptr_t weight, u
     GM_TRY(make_map(&w_mn, h->dtype, weight, h->vocab, h->dim, h->ld_weight, kTileK));
     GM_TRY(make_map(&ds_k, h->dtype, ds, s.cap, s.width, s.width, kHalf));
     GM_TRY(make_map(&ds_mn, h->dtype, ds, s.cap, s.width, s.width, kTileK));
-    GM_TRY(index_and_gather<T>(c, hidden, targets, nullptr, nullptr, (T*)dhidden));
+    GM_TRY(index_and_gather<T>(c, hidden, targets, 0, nullptr, nullptr, nullptr, (T*)dhidden));
     const GradScale scale{scale_device, grad_scale, h->mean, 1.0f / Half16<T>::kUp};
     const int dim = (int)h->dim, vocab = (int)h->vocab;
     const int64_t m_tiles = s.cap / kTileM, d_tiles = (h->dim + kTileN - 1) / kTileN;
