@@ -70,21 +70,23 @@ dropout_vec_kernel(const T* x, const T* res, T* y, const long long n, const int 
     for (int i = 0; i < kDropVec; ++i) {
         const long long g = g0 + (long long)i * kDropThreads;
         if (FLAT && g == groups) {
+            const unsigned keep = drop_mask8(d, (unsigned long long)groups * 8);
             for (long long e = groups * 8; e < n; ++e) {
-                float v = drop_keeps(d, (unsigned long long)e) ? __fmul_rn(to_f32<T>(x[e]), d.up) : 0.0f;
+                float v = (keep >> (e & 7)) & 1u ? __fmul_rn(to_f32<T>(x[e]), d.up) : 0.0f;
                 if (RES) v = __fadd_rn(to_f32<T>(res[e]), v);
                 y[e] = from_f32<T>(v);
             }
         }
         if (g >= groups) break;
-        const unsigned keep = d.cut == 0u ? 0xffu : drop_block(d, (unsigned long long)g);
         float v[8], r[8];
         widen8<T>(xv[i], v);
         if (RES) widen8<T>(rv[i], r);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            v[k] = (keep >> k) & 1u ? __fmul_rn(v[k], d.up) : 0.0f;      // a dropped NaN is dropped
-            if (RES) v[k] = __fadd_rn(r[k], v[k]);
+        for (int k = 0; k < 8; ++k) v[k] = __fmul_rn(v[k], d.up);
+        drop_block(d, (unsigned long long)g, v);                       // a dropped NaN is dropped
+        if (RES) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = __fadd_rn(r[k], v[k]);
         }
         store8<T>(y + row[i] * ld_y + col[i], v);
     }
@@ -98,7 +100,7 @@ dropout_any_kernel(const T* x, const T* res, T* y, const long long n, const long
     drop_begin(d);
     const long long g = (long long)blockIdx.x * kDropThreads + threadIdx.x;
     if (g * 8 >= n) return;
-    const unsigned keep = d.cut == 0u ? 0xffu : drop_block(d, (unsigned long long)g);
+    const unsigned keep = drop_mask8(d, (unsigned long long)g * 8);
     long long row = g * 8 / cols, col = g * 8 - row * cols;
     for (int k = 0; k < 8 && g * 8 + k < n; ++k) {
         float v = (keep >> k) & 1u ? __fmul_rn(to_f32<T>(x[row * ld_x + col]), d.up) : 0.0f;

@@ -1,6 +1,6 @@
 // gm_embedding.cu -- token embedding with scaling and dropout, and its gradient.
 //
-//   forward   out[t] = drop(scale * table[token_t])
+//   forward   out[t] = drop(scale * table[token_t])      one multiplication, by scale times dropout's factor
 //   backward  dtable[v] (+)= scale * sum over t with token_t = v, ascending, of drop(dout[t])
 //
 // Both are bound by HBM: the forward pass reads and writes one row per token; the backward
@@ -14,19 +14,21 @@ namespace gm {
 
 constexpr int kEmbThreads = 256;
 constexpr int kSortTile = 1024;          // words one CTA sorts in registers and shared memory
-constexpr int kMergeWays = 32;           // sorted runs that one merge pass joins
-constexpr int kPiece = 64;               // sorted tokens whose sum is one piece of a long row
+constexpr int kMergeWays = 64;           // sorted runs that one merge pass joins
+constexpr int kPiece = 32;               // sorted words whose sum is one piece of a long row
 
 // ---------------------------------------------------------------- forward
 // A CTA is tx lanes over groups of eight columns times ty tokens; each thread takes ROWS
 // tokens and issues all its loads first.  VEC: rows begin on 16-byte boundaries; the last
-// dim % 8 columns, and everything without VEC, go element by element.
-template <typename T, bool VEC, int ROWS>
-__global__ void __launch_bounds__(kEmbThreads)
+// dim % 8 columns, and everything without VEC, go element by element.  WHOLE: dim is a multiple
+// of eight, so a group is a block of dropout's generator.
+template <typename T, bool VEC, bool WHOLE, int ROWS>
+__global__ void __launch_bounds__(kEmbThreads, 4)
 embedding_forward_kernel(const T* __restrict__ table, const int* __restrict__ tokens, T* __restrict__ out,
                          const long long n, const long long dim, const long long vocab, const long long ld_table,
                          const long long ld_out, const float scale, Drop d) {
     drop_begin(d);
+    const float up = __fmul_rn(scale, d.up);
     const long long groups = (dim + 7) >> 3;
     const long long t0 = ((long long)blockIdx.x * blockDim.y + threadIdx.y) * ROWS;
     long long tok[ROWS];
@@ -49,9 +51,9 @@ embedding_forward_kernel(const T* __restrict__ table, const int* __restrict__ to
                 float x[8];
                 if (tok[r] >= 0) {
                     widen8<T>(raw[r], x);
-                    const unsigned keep = drop_mask8(d, (unsigned long long)(t * dim + c));
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) x[k] = (keep >> k) & 1u ? __fmul_rn(__fmul_rn(x[k], scale), d.up) : 0.0f;
+                    for (int k = 0; k < 8; ++k) x[k] = __fmul_rn(x[k], up);
+                    drop8<WHOLE>(d, (unsigned long long)(t * dim + c), x);
                 } else {
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[k] = 0.0f;
@@ -65,7 +67,7 @@ embedding_forward_kernel(const T* __restrict__ table, const int* __restrict__ to
                 const unsigned keep = tok[r] >= 0 ? drop_mask8(d, (unsigned long long)(t * dim + c)) : 0u;
                 for (int k = 0; k < 8 && c + k < dim; ++k) {
                     float x = 0.0f;
-                    if ((keep >> k) & 1u) x = __fmul_rn(__fmul_rn(to_f32<T>(table[tok[r] * ld_table + c + k]), scale), d.up);
+                    if ((keep >> k) & 1u) x = __fmul_rn(to_f32<T>(table[tok[r] * ld_table + c + k]), up);
                     out[t * ld_out + c + k] = from_f32<T>(x);
                 }
             }
@@ -119,22 +121,29 @@ __device__ __forceinline__ long long lower_bound(const unsigned long long* __res
     return lo;
 }
 
-// Joins kMergeWays sorted runs of `run` words: a word's place is the number of smaller words
-// in every run of its group, found by bisection, so one pass has no serial part.
-__global__ void __launch_bounds__(256)
-token_merge_kernel(const unsigned long long* __restrict__ in, unsigned long long* __restrict__ out, const long long n, const long long run) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+// Joins kMergeWays sorted runs of `run` words (a power of two): a word's place is the number of
+// smaller words in every run of its group, found by bisection, so one pass has no serial part.
+// Bisections are chains of dependent loads, so 32 of them go in step.
+__global__ void __launch_bounds__(128)
+token_merge_kernel(const unsigned long long* __restrict__ in, unsigned long long* __restrict__ out, const long long n, const int run) {
+    const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
     if (i >= n) return;
     const unsigned long long key = __ldg(in + i);
-    const long long base = i / (run * kMergeWays) * (run * kMergeWays);
-    const long long mine = base + (i - base) / run * run;
-    long long rank = i - mine;
-    for (int q = 0; q < kMergeWays; ++q) {
-        const long long a = base + q * run;
-        if (a >= n) break;
-        if (a == mine) continue;
-        const long long b = a + run < n ? a + run : n;
-        rank += lower_bound(in, a, b, key) - a;
+    const long long base = i / ((long long)run * kMergeWays) * ((long long)run * kMergeWays);
+    long long rank = 0;
+    for (int q = 0; q < kMergeWays && base + (long long)q * run < n; q += 32) {
+        int below[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) below[j] = 0;
+        for (int step = run; step > 0; step >>= 1) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const long long probe = base + (long long)(q + j) * run + below[j] + step - 1;
+                if (below[j] + step <= run && probe < n && __ldg(in + probe) < key) below[j] += step;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) rank += below[j];
     }
     out[base + rank] = key;
 }
@@ -148,11 +157,11 @@ token_first_kernel(const unsigned long long* __restrict__ words, const long long
 
 // ---------------------------------------------------------------- backward sums
 // Adds the rows of dout that words [a, b) name, in order, to acc: eight columns from c.
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool WHOLE>
 __device__ __forceinline__ void add_rows(const T* __restrict__ dout, const unsigned long long* __restrict__ words, long long a, const long long b,
                                          const long long c, const long long dim, const long long ld_out, const Drop& d, float (&acc)[8]) {
     if (VEC && c + 8 <= dim) {
-        constexpr int DEEP = 8;
+        constexpr int DEEP = sizeof(T) == 2 ? 8 : 4;                 // loads in flight per thread
         while (a < b) {
             Raw8<T> raw[DEEP];
             unsigned pos[DEEP];
@@ -168,9 +177,9 @@ __device__ __forceinline__ void add_rows(const T* __restrict__ dout, const unsig
                 if (j < m) {
                     float x[8];
                     widen8<T>(raw[j], x);
-                    const unsigned keep = drop_mask8(d, (unsigned long long)((long long)pos[j] * dim + c));
+                    drop8<WHOLE>(d, (unsigned long long)((long long)pos[j] * dim + c), x);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) acc[k] = __fadd_rn(acc[k], (keep >> k) & 1u ? x[k] : 0.0f);
+                    for (int k = 0; k < 8; ++k) acc[k] = __fadd_rn(acc[k], x[k]);
                 }
             a += m;
         }
@@ -184,35 +193,58 @@ __device__ __forceinline__ void add_rows(const T* __restrict__ dout, const unsig
     }
 }
 
-// A row whose sorted words lie in more than one chunk of kPiece words is summed in pieces, one
-// per chunk, so that a token that fills half the batch is still spread over the GPU.  Slot 2j
-// holds chunk j's part of a row that began before it, slot 2j + 1 that of a row that begins in
-// it and goes on.
-template <typename T, bool VEC>
+// The row of table that word i belongs to: its words are [a, b).
+__device__ __forceinline__ void row_of(const unsigned long long* __restrict__ words, const int* __restrict__ first, const long long n,
+                                       const unsigned key, long long* a, long long* b) {
+    if (first) {
+        *a = __ldg(first + key);
+        *b = __ldg(first + key + 1);
+    } else {
+        *a = lower_bound(words, 0, n, (unsigned long long)key << 32);
+        *b = lower_bound(words, *a, n, (unsigned long long)(key + 1u) << 32);
+    }
+}
+
+// A row of more than kPiece words is summed in pieces of kPiece, counted from its first word, so
+// that a token that fills half the batch is still spread over the GPU.  A piece that begins at
+// word s leaves its sum in slot 2 (s / kPiece), the row's first piece in the slot behind that:
+// among kPiece neighbouring words there begin at most one first piece and one other.
+template <typename T, bool VEC, bool WHOLE>
 __global__ void __launch_bounds__(128)
-embedding_pieces_kernel(const T* __restrict__ dout, const unsigned long long* __restrict__ words, float* __restrict__ pieces,
-                        const long long n, const long long dim, const long long vocab, const long long ld_out, Drop d) {
-    __shared__ unsigned tok[kPiece];
+embedding_pieces_kernel(const T* __restrict__ dout, const unsigned long long* __restrict__ words, const int* __restrict__ first,
+                        float* __restrict__ pieces, const long long n, const long long dim, const long long vocab, const long long ld_out, Drop d) {
+    __shared__ long long from[2], to[2];
     const int tid = threadIdx.x;
     const long long begin = (long long)blockIdx.x * kPiece;
-    const int len = n - begin < kPiece ? (int)(n - begin) : kPiece;
-    if (tid < len) tok[tid] = (unsigned)(__ldg(words + begin + tid) >> 32);
+    if (tid < 2) from[tid] = -1;
     __syncthreads();
-    const unsigned head = tok[0], tail = tok[len - 1];
-    const bool from_before = begin > 0 && head < vocab && (unsigned)(__ldg(words + begin - 1) >> 32) == head;
-    const bool goes_on = begin + len < n && tail < vocab && (unsigned)(__ldg(words + begin + len) >> 32) == tail;
-    if (!from_before && !goes_on) return;
-    const int n_head = __syncthreads_count(tid < len && tok[tid] == head);
-    const int n_tail = __syncthreads_count(tid < len && tok[tid] == tail);
+    if (tid < kPiece && begin + tid < n) {
+        const long long i = begin + tid;
+        const unsigned key = (unsigned)(__ldg(words + i) >> 32);
+        // a row of more than kPiece words has a word of its own kPiece places on or back
+        const bool maybe = key < vocab && ((i + kPiece < n && (unsigned)(__ldg(words + i + kPiece) >> 32) == key) ||
+                                           (i >= kPiece && (unsigned)(__ldg(words + i - kPiece) >> 32) == key));
+        if (maybe) {
+            long long a, b;
+            row_of(words, first, n, key, &a, &b);
+            if ((i - a) % kPiece == 0) {
+                const int side = i == a ? 1 : 0;
+                from[side] = i;
+                to[side] = i + kPiece < b ? i + kPiece : b;
+            }
+        }
+    }
+    __syncthreads();
+    if (from[0] < 0 && from[1] < 0) return;
     drop_begin(d);
     const long long groups = (dim + 7) >> 3;
     for (long long g = (long long)blockIdx.y * 128 + tid; g < groups; g += (long long)gridDim.y * 128) {
         const long long c = g << 3;
 #pragma unroll 1
         for (int side = 0; side < 2; ++side) {
-            if (side == 0 ? !from_before : !goes_on || (from_before && n_head == len)) continue;
+            if (from[side] < 0) continue;
             float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            add_rows<T, VEC>(dout, words, side == 0 ? begin : begin + len - n_tail, side == 0 ? begin + n_head : begin + len, c, dim, ld_out, d, acc);
+            add_rows<T, VEC, WHOLE>(dout, words, from[side], to[side], c, dim, ld_out, d, acc);
             float* p = pieces + (2 * (long long)blockIdx.x + side) * (groups * 8) + c;
             reinterpret_cast<float4*>(p)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
             reinterpret_cast<float4*>(p)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
@@ -220,66 +252,80 @@ embedding_pieces_kernel(const T* __restrict__ dout, const unsigned long long* __
     }
 }
 
-// HEADS false: one item per row of the table, every row is written.  HEADS true (accumulate):
-// one item per sorted word, those that begin a row add to it, the others leave.
-template <typename T, typename G, bool VEC, bool HEADS>
-__global__ void __launch_bounds__(kEmbThreads)
+// HEADS false: items are the table's rows, every one is written.  HEADS true (accumulate): items
+// are the sorted words; one that begins a row adds to it, the others are passed over.  A CTA is
+// tx lanes over groups of eight columns times ty items at a time, kRowTurns times.
+constexpr int kRowTurns = 8;
+template <typename T, typename G, bool VEC, bool WHOLE, bool HEADS>
+__global__ void __launch_bounds__(kEmbThreads, 3)
 embedding_rows_kernel(const T* __restrict__ dout, const unsigned long long* __restrict__ words, const int* __restrict__ first,
                       const float* __restrict__ pieces, G* dtable, const long long n, const long long dim, const long long vocab,
                       const long long ld_table, const long long ld_out, const float scale, Drop d) {
-    const long long item = (long long)blockIdx.x * blockDim.y + threadIdx.y;
-    long long v, a, b;
-    if (HEADS) {
-        if (item >= n) return;
-        const unsigned key = (unsigned)(__ldg(words + item) >> 32);
-        if (key >= vocab || (item > 0 && (unsigned)(__ldg(words + item - 1) >> 32) == key)) return;
-        v = key;
-        a = item;
-        b = lower_bound(words, item + 1, n, (unsigned long long)(key + 1u) << 32);
-    } else {
-        if (item >= vocab) return;
-        v = item;
-        a = __ldg(first + v);
-        b = __ldg(first + v + 1);
+    // where the CTA's rows begin and end (its words' tokens, and the one before), read at once
+    __shared__ int mark[kEmbThreads / 8 * kRowTurns + 1];
+    const int items = blockDim.y * kRowTurns;
+    const long long item0 = (long long)blockIdx.x * items;
+    for (int i = threadIdx.y * blockDim.x + threadIdx.x; i <= items; i += kEmbThreads) {
+        const long long at = HEADS ? item0 + i - 1 : item0 + i;
+        if (HEADS) mark[i] = at >= 0 && at < n ? (int)(__ldg(words + at) >> 32) : (int)vocab;
+        else mark[i] = at <= vocab ? __ldg(first + at) : 0;
     }
+    __syncthreads();
     drop_begin(d);
     const long long groups = (dim + 7) >> 3;
     const float up = __fmul_rn(scale, d.up);
-    const long long ca = a / kPiece, cb = b > a ? (b - 1) / kPiece : ca;
-    for (long long g = (long long)blockIdx.y * blockDim.x + threadIdx.x; g < groups; g += (long long)gridDim.y * blockDim.x) {
-        const long long c = g << 3;
-        float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (b > a) {
-            if (ca == cb) {
-                add_rows<T, VEC>(dout, words, a, b, c, dim, ld_out, d, acc);
-            } else {
-                // a row that begins on a chunk's first word left that chunk's part in the odd slot
+#pragma unroll 1
+    for (int turn = 0; turn < kRowTurns; ++turn) {
+        const int slot = turn * blockDim.y + threadIdx.y;
+        const long long item = item0 + slot;
+        long long v, a, b;
+        if (HEADS) {
+            if (item >= n) return;
+            v = mark[slot + 1];
+            if (v >= vocab || (item > 0 && mark[slot] == v)) continue;
+            a = item;
+            b = item + 1;
+            if (b < n && (long long)(__ldg(words + b) >> 32) == v) b = lower_bound(words, b, n, (unsigned long long)(v + 1) << 32);
+        } else {
+            if (item >= vocab) return;
+            v = item;
+            a = mark[slot];
+            b = mark[slot + 1];
+        }
+        for (long long g = (long long)blockIdx.y * blockDim.x + threadIdx.x; g < groups; g += (long long)gridDim.y * blockDim.x) {
+            const long long c = g << 3;
+            float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            if (b - a > kPiece) {
 #pragma unroll 4
-                for (long long j = ca; j <= cb; ++j) {
-                    const float4* p = reinterpret_cast<const float4*>(pieces + (2 * j + (j == ca ? 1 : 0)) * (groups * 8) + c);
+                for (long long s = a; s < b; s += kPiece) {
+                    const float4* p = reinterpret_cast<const float4*>(pieces + (2 * (s / kPiece) + (s == a ? 1 : 0)) * (groups * 8) + c);
                     const float4 x = p[0], y = p[1];
                     acc[0] = __fadd_rn(acc[0], x.x); acc[1] = __fadd_rn(acc[1], x.y);
                     acc[2] = __fadd_rn(acc[2], x.z); acc[3] = __fadd_rn(acc[3], x.w);
                     acc[4] = __fadd_rn(acc[4], y.x); acc[5] = __fadd_rn(acc[5], y.y);
                     acc[6] = __fadd_rn(acc[6], y.z); acc[7] = __fadd_rn(acc[7], y.w);
                 }
+            } else if (b > a) {
+                add_rows<T, VEC, WHOLE>(dout, words, a, b, c, dim, ld_out, d, acc);
             }
+            if (b > a) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) acc[k] = __fmul_rn(acc[k], up);
-        }
-        G* to = dtable + v * ld_table + c;
-        if (VEC && c + 8 <= dim) {
-            if (HEADS) {
-                float old[8];
-                widen8<G>(load8<G, false>(to), old);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) acc[k] = __fadd_rn(old[k], acc[k]);
+                for (int k = 0; k < 8; ++k) acc[k] = __fmul_rn(acc[k], up);
             }
-            store8<G>(to, acc);
-        } else {
+            G* to = dtable + v * ld_table + c;
+            if (VEC && c + 8 <= dim) {
+                if (HEADS) {
+                    float old[8];
+                    widen8<G>(load8<G, false>(to), old);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (c + k < dim) to[k] = from_f32<G>(HEADS ? __fadd_rn(to_f32<G>(to[k]), acc[k]) : acc[k]);
+                    for (int k = 0; k < 8; ++k) acc[k] = __fadd_rn(old[k], acc[k]);
+                }
+                store8<G>(to, acc);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (c + k < dim) to[k] = from_f32<G>(HEADS ? __fadd_rn(to_f32<G>(to[k]), acc[k]) : acc[k]);
+            }
         }
     }
 }
@@ -324,9 +370,17 @@ static int launch_embedding_forward(Device* d, const gm_embedding_t* e, uintptr_
     unsigned gy = 1;
     row_shape(e->dim, &block, &gy);
     const bool vec = table % 16 == 0 && out % 16 == 0 && e->ld_table * (int)sizeof(T) % 16 == 0 && e->ld_out * (int)sizeof(T) % 16 == 0;
-    const dim3 grid((unsigned)((e->tokens + block.y - 1) / block.y), gy);
-    if (vec) embedding_forward_kernel<T, true, 1><<<grid, block, 0, d->stream>>>((const T*)table, (const int*)tokens, (T*)out, e->tokens, e->dim, e->vocab, e->ld_table, e->ld_out, e->scale, drop);
-    else embedding_forward_kernel<T, false, 1><<<grid, block, 0, d->stream>>>((const T*)table, (const int*)tokens, (T*)out, e->tokens, e->dim, e->vocab, e->ld_table, e->ld_out, e->scale, drop);
+    // four tokens per thread keep more loads in flight; a call too small for that takes one
+    const bool many = e->tokens * gy >= (int64_t)d->sm_count * 8 * block.y;
+#define GM_FORWARD(VEC, WHOLE, ROWS)                                                                                                            \
+    embedding_forward_kernel<T, VEC, WHOLE, ROWS><<<dim3((unsigned)((e->tokens + block.y * ROWS - 1) / (block.y * ROWS)), gy), block, 0, d->stream>>>( \
+        (const T*)table, (const int*)tokens, (T*)out, e->tokens, e->dim, e->vocab, e->ld_table, e->ld_out, e->scale, drop)
+    const bool whole = e->dim % 8 == 0;
+    if (!vec) GM_FORWARD(false, false, 1);
+    else if (!whole) GM_FORWARD(true, false, 1);
+    else if (many) GM_FORWARD(true, true, 4);
+    else GM_FORWARD(true, true, 1);
+#undef GM_FORWARD
     d->launches++;
     GM_CUDA_CHECK(cudaGetLastError());
     return GM_OK;
@@ -344,7 +398,7 @@ static int launch_embedding_backward(Device* d, const gm_embedding_t* e, uintptr
     token_sort_tile_kernel<<<(unsigned)((n + kSortTile - 1) / kSortTile), kSortTile, 0, d->stream>>>((const int*)tokens, n, e->vocab, e->padding_token, words);
     d->launches++;
     for (int64_t run = kSortTile; run < n; run *= kMergeWays) {
-        token_merge_kernel<<<(unsigned)((n + 255) / 256), 256, 0, d->stream>>>(words, other, n, run);
+        token_merge_kernel<<<(unsigned)((n + 127) / 128), 128, 0, d->stream>>>(words, other, n, (int)run);
         d->launches++;
         unsigned long long* t = words; words = other; other = t;
     }
@@ -353,24 +407,34 @@ static int launch_embedding_backward(Device* d, const gm_embedding_t* e, uintptr
         d->launches++;
     }
     const bool vec = dout % 16 == 0 && e->ld_out * (int)sizeof(T) % 16 == 0 && dtable % 16 == 0 && e->ld_table * (int)sizeof(G) % 16 == 0;
+    const bool whole = e->dim % 8 == 0;
     const int64_t groups = (e->dim + 7) / 8;
     if (n > kPiece) {
         const int64_t y = (groups + 127) / 128;
         const dim3 grid((unsigned)((n + kPiece - 1) / kPiece), (unsigned)(y < 65535 ? y : 65535));
-        if (vec) embedding_pieces_kernel<T, true><<<grid, 128, 0, d->stream>>>((const T*)dout, words, pieces, n, e->dim, e->vocab, e->ld_out, drop);
-        else embedding_pieces_kernel<T, false><<<grid, 128, 0, d->stream>>>((const T*)dout, words, pieces, n, e->dim, e->vocab, e->ld_out, drop);
+        if (vec && whole) embedding_pieces_kernel<T, true, true><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, n, e->dim, e->vocab, e->ld_out, drop);
+        else if (vec) embedding_pieces_kernel<T, true, false><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, n, e->dim, e->vocab, e->ld_out, drop);
+        else embedding_pieces_kernel<T, false, false><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, n, e->dim, e->vocab, e->ld_out, drop);
         d->launches++;
     }
     dim3 block;
     unsigned gy = 1;
     row_shape(e->dim, &block, &gy);
     const int64_t items = accumulate ? n : e->vocab;
-    const dim3 grid((unsigned)((items + block.y - 1) / block.y), gy);
-#define GM_ROWS(VEC, HEADS)                                                                                                   \
-    embedding_rows_kernel<T, G, VEC, HEADS><<<grid, block, 0, d->stream>>>((const T*)dout, words, first, pieces, (G*)dtable, n, \
+    const int64_t per_cta = (int64_t)block.y * kRowTurns;
+    const dim3 grid((unsigned)((items + per_cta - 1) / per_cta), gy);
+#define GM_ROWS(VEC, WHOLE, HEADS)                                                                                                   \
+    embedding_rows_kernel<T, G, VEC, WHOLE, HEADS><<<grid, block, 0, d->stream>>>((const T*)dout, words, first, pieces, (G*)dtable, n, \
                                                                            e->dim, e->vocab, e->ld_table, e->ld_out, e->scale, drop)
-    if (accumulate) { if (vec) GM_ROWS(true, true); else GM_ROWS(false, true); }
-    else { if (vec) GM_ROWS(true, false); else GM_ROWS(false, false); }
+    if (accumulate) {
+        if (vec && whole) GM_ROWS(true, true, true);
+        else if (vec) GM_ROWS(true, false, true);
+        else GM_ROWS(false, false, true);
+    } else {
+        if (vec && whole) GM_ROWS(true, true, false);
+        else if (vec) GM_ROWS(true, false, false);
+        else GM_ROWS(false, false, false);
+    }
 #undef GM_ROWS
     d->launches++;
     GM_CUDA_CHECK(cudaGetLastError());

@@ -97,22 +97,46 @@ __device__ __forceinline__ void drop_begin(Drop& d) {
     }
 }
 
-// Bit k: element 8 * block + k stays.
-__device__ __forceinline__ unsigned drop_block(const Drop& d, const unsigned long long block) {
+// The 128 bits of one block, elements 2k and 2k + 1 in the low and high half of word k.
+__device__ __forceinline__ void drop_words(const Drop& d, const unsigned long long block, unsigned (&w)[4]) {
     unsigned c0 = (unsigned)block, c1 = (unsigned)(block >> 32), c2 = d.o0, c3 = d.o1;
     unsigned k0 = d.k0, k1 = d.k1;
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
-        const unsigned h0 = __umulhi(0xD2511F53u, c0), l0 = 0xD2511F53u * c0;
-        const unsigned h1 = __umulhi(0xCD9E8D57u, c2), l1 = 0xCD9E8D57u * c2;
-        c0 = h1 ^ c1 ^ k0;
-        c1 = l1;
-        c2 = h0 ^ c3 ^ k1;
-        c3 = l0;
+        const unsigned long long a = (unsigned long long)0xD2511F53u * c0, b = (unsigned long long)0xCD9E8D57u * c2;
+        c0 = (unsigned)(b >> 32) ^ c1 ^ k0;
+        c1 = (unsigned)b;
+        c2 = (unsigned)(a >> 32) ^ c3 ^ k1;
+        c3 = (unsigned)a;
         k0 += 0x9E3779B9u;
         k1 += 0xBB67AE85u;
     }
-    const unsigned w[4] = {c0, c1, c2, c3};
+    w[0] = c0; w[1] = c1; w[2] = c2; w[3] = c3;
+}
+
+// Zeroes the dropped ones of a whole block of eight elements.  A half reaches the cut when the
+// word that has it on top reaches the cut shifted up: two compares and one shift per word.
+__device__ __forceinline__ void drop_block(const Drop& d, const unsigned long long block, float (&x)[8]) {
+    if (d.cut == 0u) return;
+    if (d.cut > 0xffffu) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+        return;
+    }
+    unsigned w[4];
+    drop_words(d, block, w);
+    const unsigned top = d.cut << 16;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        x[2 * k] = (w[k] << 16) >= top ? x[2 * k] : 0.0f;
+        x[2 * k + 1] = w[k] >= top ? x[2 * k + 1] : 0.0f;
+    }
+}
+
+// Bit k: element 8 * block + k stays.
+__device__ __forceinline__ unsigned drop_bits(const Drop& d, const unsigned long long block) {
+    unsigned w[4];
+    drop_words(d, block, w);
     unsigned keep = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -125,14 +149,22 @@ __device__ __forceinline__ unsigned drop_block(const Drop& d, const unsigned lon
 // Bit k: element first + k stays, for eight elements that may begin inside a block.
 __device__ __forceinline__ unsigned drop_mask8(const Drop& d, const unsigned long long first) {
     if (d.cut == 0u) return 0xffu;
-    unsigned keep = drop_block(d, first >> 3);
+    unsigned keep = drop_bits(d, first >> 3);
     const unsigned skip = (unsigned)first & 7u;
-    if (skip != 0u) keep = (keep | (drop_block(d, (first >> 3) + 1) << 8)) >> skip;
+    if (skip != 0u) keep = (keep | (drop_bits(d, (first >> 3) + 1) << 8)) >> skip;
     return keep & 0xffu;
 }
 
-__device__ __forceinline__ bool drop_keeps(const Drop& d, const unsigned long long e) {
-    return d.cut == 0u || ((drop_block(d, e >> 3) >> ((unsigned)e & 7u)) & 1u);
+// Zeroes the dropped ones of eight elements from `first` on; WHOLE: they are a block.
+template <bool WHOLE>
+__device__ __forceinline__ void drop8(const Drop& d, const unsigned long long first, float (&x)[8]) {
+    if (WHOLE) {
+        drop_block(d, first >> 3, x);
+    } else {
+        const unsigned keep = drop_mask8(d, first);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = (keep >> k) & 1u ? x[k] : 0.0f;
+    }
 }
 
 // ---- host side ----

@@ -63,7 +63,7 @@ def test_forward(gm, dev, dtype, n, dim, vocab, p):
     tok[0] = vocab - 1
     keep, up = R.keep_mask(n * dim, p, 77, 1 << 40)
     rows = np.where((tok >= 0) & (tok < vocab), tok, 0)
-    want = (table[rows].astype(np.float32) * np.float32(SCALE)) * up
+    want = table[rows].astype(np.float32) * (np.float32(SCALE) * up)
     want = np.where(keep.reshape(n, dim) & ((tok >= 0) & (tok < vocab))[:, None], want, np.float32(0))
     want = R.rounded(want.astype(np.float32), dtype)
     d_tok = dev.to_device(tok)
