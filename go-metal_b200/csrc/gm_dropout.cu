@@ -8,12 +8,15 @@
 namespace gm {
 
 int make_drop(const gm_dropout_t* in, Drop* out) {
-    *out = Drop{0, 0, 0, 0, nullptr, 0, 1.0f};
+    *out = Drop{};
+    out->up = 1.0f;
     if (!in) return GM_OK;
     if (!(in->p >= 0.0f && in->p <= 1.0f)) { set_error("dropout probability %g is outside [0, 1]", (double)in->p); return GM_ERR_BAD_ARG; }
     if (in->offset_device % 8) { set_error("the device offset of dropout is not 8-byte aligned"); return GM_ERR_BAD_ARG; }
-    out->k0 = (unsigned)in->seed;
-    out->k1 = (unsigned)(in->seed >> 32);
+    for (int r = 0; r < 10; ++r) {
+        out->key[2 * r] = (unsigned)in->seed + (unsigned)r * 0x9E3779B9u;
+        out->key[2 * r + 1] = (unsigned)(in->seed >> 32) + (unsigned)r * 0xBB67AE85u;
+    }
     out->o0 = (unsigned)in->offset;
     out->o1 = (unsigned)(in->offset >> 32);
     out->more = (const unsigned long long*)in->offset_device;
@@ -35,8 +38,8 @@ int check_matrix(int64_t rows, int64_t cols, int64_t ld, const char* what) {
         set_error("%s: size %lld x %lld is outside [1, 2^31)", what, (long long)rows, (long long)cols);
         return GM_ERR_BAD_SIZE;
     }
+    if (ld > 0x7fffffffLL) { set_error("%s: row stride %lld is outside [1, 2^31)", what, (long long)ld); return GM_ERR_BAD_SIZE; }
     if (ld < cols) { set_error("%s: row stride %lld is smaller than its %lld columns", what, (long long)ld, (long long)cols); return GM_ERR_BAD_ARG; }
-    if (ld > (1LL << 46) / rows) { set_error("%s: %lld rows of stride %lld are more than 2^46 elements", what, (long long)rows, (long long)ld); return GM_ERR_BAD_SIZE; }
     return GM_OK;
 }
 
@@ -50,8 +53,8 @@ constexpr int kDropVec = 2;
 template <typename T, bool RES, bool FLAT>
 __global__ void __launch_bounds__(kDropThreads)
 dropout_vec_kernel(const T* x, const T* res, T* y, const long long n, const int row_groups,
-                   const long long ld_x, const long long ld_r, const long long ld_y, Drop d) {
-    drop_begin(d);
+                   const long long ld_x, const long long ld_r, const long long ld_y, const __grid_constant__ Drop d) {
+    const DropOffset o = drop_begin(d);
     const long long groups = n >> 3;
     const long long g0 = (long long)blockIdx.x * (kDropThreads * kDropVec) + threadIdx.x;
     Raw8<T> xv[kDropVec], rv[kDropVec];
@@ -70,7 +73,7 @@ dropout_vec_kernel(const T* x, const T* res, T* y, const long long n, const int 
     for (int i = 0; i < kDropVec; ++i) {
         const long long g = g0 + (long long)i * kDropThreads;
         if (FLAT && g == groups) {
-            const unsigned keep = drop_mask8(d, (unsigned long long)groups * 8);
+            const unsigned keep = drop_mask8(d, o, (unsigned long long)groups * 8);
             for (long long e = groups * 8; e < n; ++e) {
                 float v = (keep >> (e & 7)) & 1u ? __fmul_rn(to_f32<T>(x[e]), d.up) : 0.0f;
                 if (RES) v = __fadd_rn(to_f32<T>(res[e]), v);
@@ -83,7 +86,7 @@ dropout_vec_kernel(const T* x, const T* res, T* y, const long long n, const int 
         if (RES) widen8<T>(rv[i], r);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = __fmul_rn(v[k], d.up);
-        drop_block(d, (unsigned long long)g, v);                       // a dropped NaN is dropped
+        drop_block(d, o, (unsigned long long)g, v);                       // a dropped NaN is dropped
         if (RES) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = __fadd_rn(r[k], v[k]);
@@ -96,11 +99,11 @@ dropout_vec_kernel(const T* x, const T* res, T* y, const long long n, const int 
 template <typename T, bool RES>
 __global__ void __launch_bounds__(kDropThreads)
 dropout_any_kernel(const T* x, const T* res, T* y, const long long n, const long long cols,
-                   const long long ld_x, const long long ld_r, const long long ld_y, Drop d) {
-    drop_begin(d);
+                   const long long ld_x, const long long ld_r, const long long ld_y, const __grid_constant__ Drop d) {
+    const DropOffset o = drop_begin(d);
     const long long g = (long long)blockIdx.x * kDropThreads + threadIdx.x;
     if (g * 8 >= n) return;
-    const unsigned keep = drop_mask8(d, (unsigned long long)g * 8);
+    const unsigned keep = drop_mask8(d, o, (unsigned long long)g * 8);
     long long row = g * 8 / cols, col = g * 8 - row * cols;
     for (int k = 0; k < 8 && g * 8 + k < n; ++k) {
         float v = (keep >> k) & 1u ? __fmul_rn(to_f32<T>(x[row * ld_x + col]), d.up) : 0.0f;

@@ -14,7 +14,7 @@ namespace gm {
 
 constexpr int kEmbThreads = 256;
 constexpr int kSortTile = 1024;          // words one CTA sorts in registers and shared memory
-constexpr int kMergeWays = 64;           // sorted runs that one merge pass joins
+constexpr int kMergeWays = 8;            // sorted runs that one merge pass joins
 constexpr int kPiece = 32;               // sorted words whose sum is one piece of a long row
 
 // ---------------------------------------------------------------- forward
@@ -24,51 +24,45 @@ constexpr int kPiece = 32;               // sorted words whose sum is one piece 
 // of eight, so a group is a block of dropout's generator.
 template <typename T, bool VEC, bool WHOLE, int ROWS>
 __global__ void __launch_bounds__(kEmbThreads, 4)
-embedding_forward_kernel(const T* __restrict__ table, const int* __restrict__ tokens, T* __restrict__ out,
-                         const long long n, const long long dim, const long long vocab, const long long ld_table,
-                         const long long ld_out, const float scale, Drop d) {
-    drop_begin(d);
+embedding_forward_kernel(const T* __restrict__ table, const int* __restrict__ tokens, T* __restrict__ out, const int n, const int dim,
+                         const int vocab, const int ld_table, const int ld_out, const float scale, const __grid_constant__ Drop d) {
+    const DropOffset o = drop_begin(d);
     const float up = __fmul_rn(scale, d.up);
-    const long long groups = (dim + 7) >> 3;
+    const int groups = (int)(((unsigned)dim + 7u) >> 3);
     const long long t0 = ((long long)blockIdx.x * blockDim.y + threadIdx.y) * ROWS;
-    long long tok[ROWS];
+    int tok[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-        tok[r] = t0 + r < n ? (long long)__ldg(tokens + t0 + r) : -1;
+        tok[r] = t0 + r < n ? __ldg(tokens + t0 + r) : -1;
         if (tok[r] >= vocab) tok[r] = -1;
     }
-    for (long long g = (long long)blockIdx.y * blockDim.x + threadIdx.x; g < groups; g += (long long)gridDim.y * blockDim.x) {
-        const long long c = g << 3;
-        if (VEC && c + 8 <= dim) {
+    const int live = n - t0 < ROWS ? (int)(n - t0) : ROWS;           // tokens of this thread (may be none)
+    for (int g = blockIdx.y * blockDim.x + threadIdx.x; g < groups; g += gridDim.y * blockDim.x) {
+        const int c = g << 3;
+        if (VEC && (WHOLE || c + 8 <= dim)) {
             Raw8<T> raw[ROWS];
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
-                if (tok[r] >= 0) raw[r] = load8<T, true>(table + tok[r] * ld_table + c);
+                if (tok[r] >= 0) raw[r] = load8<T, true>(table + (long long)tok[r] * ld_table + c);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
-                const long long t = t0 + r;
-                if (t >= n) break;
-                float x[8];
+                if (r >= live) break;
+                float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
                 if (tok[r] >= 0) {
                     widen8<T>(raw[r], x);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[k] = __fmul_rn(x[k], up);
-                    drop8<WHOLE>(d, (unsigned long long)(t * dim + c), x);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+                    drop8<WHOLE>(d, o, (unsigned long long)((t0 + r) * dim + c), x);
                 }
-                store8<T>(out + t * ld_out + c, x);
+                store8<T>(out + (t0 + r) * ld_out + c, x);
             }
         } else {
-            for (int r = 0; r < ROWS; ++r) {
-                const long long t = t0 + r;
-                if (t >= n) break;
-                const unsigned keep = tok[r] >= 0 ? drop_mask8(d, (unsigned long long)(t * dim + c)) : 0u;
-                for (int k = 0; k < 8 && c + k < dim; ++k) {
+            for (int r = 0; r < live; ++r) {
+                const unsigned keep = tok[r] >= 0 ? drop_mask8(d, o, (unsigned long long)((t0 + r) * dim + c)) : 0u;
+                for (int k = 0; k < 8 && k < dim - c; ++k) {
                     float x = 0.0f;
-                    if ((keep >> k) & 1u) x = __fmul_rn(to_f32<T>(table[tok[r] * ld_table + c + k]), up);
-                    out[t * ld_out + c + k] = from_f32<T>(x);
+                    if ((keep >> k) & 1u) x = __fmul_rn(to_f32<T>(table[(long long)tok[r] * ld_table + c + k]), up);
+                    out[(t0 + r) * ld_out + c + k] = from_f32<T>(x);
                 }
             }
         }
@@ -112,96 +106,115 @@ token_sort_tile_kernel(const int* __restrict__ tokens, const long long n, const 
     if (i < n) out[i] = key;
 }
 
-__device__ __forceinline__ long long lower_bound(const unsigned long long* __restrict__ a, long long lo, long long hi, unsigned long long x) {
+// The token of a sorted word.
+__device__ __forceinline__ unsigned token_at(const unsigned long long* __restrict__ words, long long i) {
+    return __ldg(reinterpret_cast<const unsigned*>(words + i) + 1);
+}
+
+// First of the words [lo, hi) whose token is not below `key`.
+__device__ __forceinline__ long long first_at(const unsigned long long* __restrict__ words, long long lo, long long hi, unsigned key) {
     while (lo < hi) {
         const long long mid = (lo + hi) >> 1;
-        if (__ldg(a + mid) < x) lo = mid + 1;
+        if (token_at(words, mid) < key) lo = mid + 1;
         else hi = mid;
     }
     return lo;
 }
 
 // Joins kMergeWays sorted runs of `run` words (a power of two): a word's place is the number of
-// smaller words in every run of its group, found by bisection, so one pass has no serial part.
-// Bisections are chains of dependent loads, so 32 of them go in step.
+// words in front of it in every run of its group, found by bisection, so one pass has no serial
+// part.  Runs hold ascending positions, so an equal token of an earlier run comes first and one
+// of a later run behind: comparing tokens is enough.  The bisections, chains of dependent loads,
+// go in step.
 __global__ void __launch_bounds__(128)
 token_merge_kernel(const unsigned long long* __restrict__ in, unsigned long long* __restrict__ out, const long long n, const int run) {
     const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
     if (i >= n) return;
-    const unsigned long long key = __ldg(in + i);
+    const unsigned long long word = __ldg(in + i);
+    const unsigned token = (unsigned)(word >> 32);
     const long long base = i / ((long long)run * kMergeWays) * ((long long)run * kMergeWays);
-    long long rank = 0;
-    for (int q = 0; q < kMergeWays && base + (long long)q * run < n; q += 32) {
-        int below[32];
+    const int mine = (int)((i - base) / run);
+    int below[kMergeWays], len[kMergeWays];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) below[j] = 0;
-        for (int step = run; step > 0; step >>= 1) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                const long long probe = base + (long long)(q + j) * run + below[j] + step - 1;
-                if (below[j] + step <= run && probe < n && __ldg(in + probe) < key) below[j] += step;
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) rank += below[j];
+    for (int j = 0; j < kMergeWays; ++j) {
+        const long long left = n - (base + (long long)j * run);
+        below[j] = 0;
+        len[j] = left <= 0 ? 0 : left < run ? (int)left : run;
     }
-    out[base + rank] = key;
+    for (int step = run; step > 0; step >>= 1) {
+#pragma unroll
+        for (int j = 0; j < kMergeWays; ++j)
+            if (below[j] + step <= len[j] && token_at(in, base + (long long)j * run + below[j] + step - 1) < token + (j < mine ? 1u : 0u)) below[j] += step;
+    }
+    long long place = base + (i - base - (long long)mine * run);
+#pragma unroll
+    for (int j = 0; j < kMergeWays; ++j) place += j == mine ? 0 : below[j];
+    out[place] = word;
 }
 
 // first[v] = number of sorted words whose token is below v, for v in [0, vocab].
 __global__ void __launch_bounds__(256)
 token_first_kernel(const unsigned long long* __restrict__ words, const long long n, const long long vocab, int* __restrict__ first) {
     const long long v = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (v <= vocab) first[v] = (int)lower_bound(words, 0, n, (unsigned long long)v << 32);
+    if (v <= vocab) first[v] = (int)first_at(words, 0, n, (unsigned)v);
 }
 
 // ---------------------------------------------------------------- backward sums
-// Adds the rows of dout that words [a, b) name, in order, to acc: eight columns from c.
-template <typename T, bool VEC, bool WHOLE>
+// Adds the rows of dout that words [a, b) name, in order, to acc: COLS groups of eight columns,
+// `apart` groups from one to the next, the first one g.  COLS x DEEP loads are in flight.
+template <typename T, bool VEC, bool WHOLE, int COLS, int DEEP>
 __device__ __forceinline__ void add_rows(const T* __restrict__ dout, const unsigned long long* __restrict__ words, long long a, const long long b,
-                                         const long long c, const long long dim, const long long ld_out, const Drop& d, float (&acc)[8]) {
-    if (VEC && c + 8 <= dim) {
-        constexpr int DEEP = sizeof(T) == 2 ? 8 : 4;                 // loads in flight per thread
+                                         const int g, const int apart, const int dim, const int ld_out, const Drop& d, const DropOffset& o,
+                                         float (&acc)[COLS][8]) {
+    const int c0 = g << 3;
+    if (VEC && (WHOLE || c0 + 8 <= dim)) {                            // without WHOLE there is one group per thread
         while (a < b) {
-            Raw8<T> raw[DEEP];
+            Raw8<T> raw[DEEP][COLS];
             unsigned pos[DEEP];
             const int m = b - a < DEEP ? (int)(b - a) : DEEP;
 #pragma unroll
             for (int j = 0; j < DEEP; ++j)
                 if (j < m) {
-                    pos[j] = (unsigned)__ldg(words + a + j);
-                    raw[j] = load8<T, false>(dout + (long long)pos[j] * ld_out + c);
+                    pos[j] = __ldg(reinterpret_cast<const unsigned*>(words + a + j));
+                    const T* row = dout + (long long)pos[j] * ld_out + c0;
+#pragma unroll
+                    for (int q = 0; q < COLS; ++q)
+                        if (q == 0 || c0 + q * apart * 8 < dim) raw[j][q] = load8<T, false>(row + q * apart * 8);
                 }
 #pragma unroll
             for (int j = 0; j < DEEP; ++j)
                 if (j < m) {
-                    float x[8];
-                    widen8<T>(raw[j], x);
-                    drop8<WHOLE>(d, (unsigned long long)((long long)pos[j] * dim + c), x);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) acc[k] = __fadd_rn(acc[k], x[k]);
+                    for (int q = 0; q < COLS; ++q)
+                        if (q == 0 || c0 + q * apart * 8 < dim) {
+                            float x[8];
+                            widen8<T>(raw[j][q], x);
+                            drop8<WHOLE>(d, o, (unsigned long long)((long long)pos[j] * dim + c0 + q * apart * 8), x);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) acc[q][k] = __fadd_rn(acc[q][k], x[k]);
+                        }
                 }
             a += m;
         }
     } else {
         for (; a < b; ++a) {
-            const long long p = (long long)(unsigned)__ldg(words + a);
-            const unsigned keep = drop_mask8(d, (unsigned long long)(p * dim + c));
-            for (int k = 0; k < 8 && c + k < dim; ++k)
-                if ((keep >> k) & 1u) acc[k] = __fadd_rn(acc[k], to_f32<T>(dout[p * ld_out + c + k]));
+            const long long p = __ldg(reinterpret_cast<const unsigned*>(words + a));
+            const unsigned keep = drop_mask8(d, o, (unsigned long long)(p * dim + c0));
+            for (int k = 0; k < 8 && k < dim - c0; ++k)
+                if ((keep >> k) & 1u) acc[0][k] = __fadd_rn(acc[0][k], to_f32<T>(dout[p * ld_out + c0 + k]));
         }
     }
 }
 
-// The row of table that word i belongs to: its words are [a, b).
+// The row of table that a word with this token belongs to: its words are [a, b).
 __device__ __forceinline__ void row_of(const unsigned long long* __restrict__ words, const int* __restrict__ first, const long long n,
                                        const unsigned key, long long* a, long long* b) {
     if (first) {
         *a = __ldg(first + key);
         *b = __ldg(first + key + 1);
     } else {
-        *a = lower_bound(words, 0, n, (unsigned long long)key << 32);
-        *b = lower_bound(words, *a, n, (unsigned long long)(key + 1u) << 32);
+        *a = first_at(words, 0, n, key);
+        *b = first_at(words, *a, n, key + 1u);
     }
 }
 
@@ -212,7 +225,7 @@ __device__ __forceinline__ void row_of(const unsigned long long* __restrict__ wo
 template <typename T, bool VEC, bool WHOLE>
 __global__ void __launch_bounds__(128)
 embedding_pieces_kernel(const T* __restrict__ dout, const unsigned long long* __restrict__ words, const int* __restrict__ first,
-                        float* __restrict__ pieces, const long long n, const long long dim, const long long vocab, const long long ld_out, Drop d) {
+                        float* __restrict__ pieces, const int n, const int dim, const int vocab, const int ld_out, const __grid_constant__ Drop d) {
     __shared__ long long from[2], to[2];
     const int tid = threadIdx.x;
     const long long begin = (long long)blockIdx.x * kPiece;
@@ -220,10 +233,9 @@ embedding_pieces_kernel(const T* __restrict__ dout, const unsigned long long* __
     __syncthreads();
     if (tid < kPiece && begin + tid < n) {
         const long long i = begin + tid;
-        const unsigned key = (unsigned)(__ldg(words + i) >> 32);
+        const unsigned key = token_at(words, i);
         // a row of more than kPiece words has a word of its own kPiece places on or back
-        const bool maybe = key < vocab && ((i + kPiece < n && (unsigned)(__ldg(words + i + kPiece) >> 32) == key) ||
-                                           (i >= kPiece && (unsigned)(__ldg(words + i - kPiece) >> 32) == key));
+        const bool maybe = key < (unsigned)vocab && ((i + kPiece < n && token_at(words, i + kPiece) == key) || (i >= kPiece && token_at(words, i - kPiece) == key));
         if (maybe) {
             long long a, b;
             row_of(words, first, n, key, &a, &b);
@@ -236,95 +248,115 @@ embedding_pieces_kernel(const T* __restrict__ dout, const unsigned long long* __
     }
     __syncthreads();
     if (from[0] < 0 && from[1] < 0) return;
-    drop_begin(d);
-    const long long groups = (dim + 7) >> 3;
-    for (long long g = (long long)blockIdx.y * 128 + tid; g < groups; g += (long long)gridDim.y * 128) {
-        const long long c = g << 3;
+    const DropOffset o = drop_begin(d);
+    const int groups = (int)(((unsigned)dim + 7u) >> 3);
+    for (int g = blockIdx.y * 128 + tid; g < groups; g += gridDim.y * 128) {
 #pragma unroll 1
         for (int side = 0; side < 2; ++side) {
             if (from[side] < 0) continue;
-            float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            add_rows<T, VEC, WHOLE>(dout, words, from[side], to[side], c, dim, ld_out, d, acc);
-            float* p = pieces + (2 * (long long)blockIdx.x + side) * (groups * 8) + c;
-            reinterpret_cast<float4*>(p)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-            reinterpret_cast<float4*>(p)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+            float acc[1][8] = {};
+            add_rows<T, VEC, WHOLE, 1, 8>(dout, words, from[side], to[side], g, 0, dim, ld_out, d, o, acc);
+            float4* p = reinterpret_cast<float4*>(pieces + ((2 * (long long)blockIdx.x + side) * groups + g) * 8);
+            p[0] = make_float4(acc[0][0], acc[0][1], acc[0][2], acc[0][3]);
+            p[1] = make_float4(acc[0][4], acc[0][5], acc[0][6], acc[0][7]);
         }
     }
 }
 
 // HEADS false: items are the table's rows, every one is written.  HEADS true (accumulate): items
 // are the sorted words; one that begins a row adds to it, the others are passed over.  A CTA is
-// tx lanes over groups of eight columns times ty items at a time, kRowTurns times.
+// tx lanes, each with COLS groups of eight columns, times ty items at a time, kRowTurns times.
 constexpr int kRowTurns = 8;
-template <typename T, typename G, bool VEC, bool WHOLE, bool HEADS>
+constexpr int kRowLanesLeast = 8;
+template <typename T, typename G, bool VEC, bool WHOLE, bool HEADS, int COLS>
 __global__ void __launch_bounds__(kEmbThreads, 3)
 embedding_rows_kernel(const T* __restrict__ dout, const unsigned long long* __restrict__ words, const int* __restrict__ first,
-                      const float* __restrict__ pieces, G* dtable, const long long n, const long long dim, const long long vocab,
-                      const long long ld_table, const long long ld_out, const float scale, Drop d) {
+                      const float* __restrict__ pieces, G* dtable, const int n, const int dim, const int vocab, const int ld_table,
+                      const int ld_out, const float scale, const __grid_constant__ Drop d) {
     // where the CTA's rows begin and end (its words' tokens, and the one before), read at once
-    __shared__ int mark[kEmbThreads / 8 * kRowTurns + 1];
+    __shared__ int mark[kEmbThreads / kRowLanesLeast * kRowTurns + 1];
     const int items = blockDim.y * kRowTurns;
     const long long item0 = (long long)blockIdx.x * items;
     for (int i = threadIdx.y * blockDim.x + threadIdx.x; i <= items; i += kEmbThreads) {
         const long long at = HEADS ? item0 + i - 1 : item0 + i;
-        if (HEADS) mark[i] = at >= 0 && at < n ? (int)(__ldg(words + at) >> 32) : (int)vocab;
+        if (HEADS) mark[i] = at >= 0 && at < n ? (int)token_at(words, at) : vocab;
         else mark[i] = at <= vocab ? __ldg(first + at) : 0;
     }
     __syncthreads();
-    drop_begin(d);
-    const long long groups = (dim + 7) >> 3;
+    const DropOffset o = drop_begin(d);
+    const int groups = (int)(((unsigned)dim + 7u) >> 3), lanes = blockDim.x;
     const float up = __fmul_rn(scale, d.up);
 #pragma unroll 1
     for (int turn = 0; turn < kRowTurns; ++turn) {
         const int slot = turn * blockDim.y + threadIdx.y;
         const long long item = item0 + slot;
-        long long v, a, b;
+        int v;
+        long long a, b;
         if (HEADS) {
             if (item >= n) return;
             v = mark[slot + 1];
             if (v >= vocab || (item > 0 && mark[slot] == v)) continue;
             a = item;
             b = item + 1;
-            if (b < n && (long long)(__ldg(words + b) >> 32) == v) b = lower_bound(words, b, n, (unsigned long long)(v + 1) << 32);
+            if (b < n && token_at(words, b) == (unsigned)v) b = first_at(words, b, n, (unsigned)v + 1u);
         } else {
             if (item >= vocab) return;
-            v = item;
+            v = (int)item;
             a = mark[slot];
             b = mark[slot + 1];
         }
-        for (long long g = (long long)blockIdx.y * blockDim.x + threadIdx.x; g < groups; g += (long long)gridDim.y * blockDim.x) {
-            const long long c = g << 3;
-            float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        G* const row = dtable + (long long)v * ld_table;
+        for (int g = blockIdx.y * lanes * COLS + threadIdx.x; g < groups; g += gridDim.y * lanes * COLS) {
+            const int c = g << 3;
+            if (!HEADS && VEC && WHOLE && a == b) {                       // a row of zeros, most of them in a large table
+#pragma unroll
+                for (int q = 0; q < COLS; ++q)
+                    if (q == 0 || c + q * lanes * 8 < dim) {
+                        uint4* to = reinterpret_cast<uint4*>(row + c + q * lanes * 8);
+                        __stcs(to, make_uint4(0u, 0u, 0u, 0u));
+                        if (sizeof(G) == 4) __stcs(to + 1, make_uint4(0u, 0u, 0u, 0u));
+                    }
+                continue;
+            }
+            float acc[COLS][8] = {};
             if (b - a > kPiece) {
-#pragma unroll 4
+#pragma unroll 2
                 for (long long s = a; s < b; s += kPiece) {
-                    const float4* p = reinterpret_cast<const float4*>(pieces + (2 * (s / kPiece) + (s == a ? 1 : 0)) * (groups * 8) + c);
-                    const float4 x = p[0], y = p[1];
-                    acc[0] = __fadd_rn(acc[0], x.x); acc[1] = __fadd_rn(acc[1], x.y);
-                    acc[2] = __fadd_rn(acc[2], x.z); acc[3] = __fadd_rn(acc[3], x.w);
-                    acc[4] = __fadd_rn(acc[4], y.x); acc[5] = __fadd_rn(acc[5], y.y);
-                    acc[6] = __fadd_rn(acc[6], y.z); acc[7] = __fadd_rn(acc[7], y.w);
+                    const float* p = pieces + (2 * (s / kPiece) + (s == a ? 1 : 0)) * groups * 8 + c;
+#pragma unroll
+                    for (int q = 0; q < COLS; ++q)
+                        if (q == 0 || c + q * lanes * 8 < dim) {
+                            const float4* at = reinterpret_cast<const float4*>(p + q * lanes * 8);
+                            const float4 x = at[0], y = at[1];
+                            acc[q][0] = __fadd_rn(acc[q][0], x.x); acc[q][1] = __fadd_rn(acc[q][1], x.y);
+                            acc[q][2] = __fadd_rn(acc[q][2], x.z); acc[q][3] = __fadd_rn(acc[q][3], x.w);
+                            acc[q][4] = __fadd_rn(acc[q][4], y.x); acc[q][5] = __fadd_rn(acc[q][5], y.y);
+                            acc[q][6] = __fadd_rn(acc[q][6], y.z); acc[q][7] = __fadd_rn(acc[q][7], y.w);
+                        }
                 }
             } else if (b > a) {
-                add_rows<T, VEC, WHOLE>(dout, words, a, b, c, dim, ld_out, d, acc);
+                constexpr int DEEP = COLS == 1 ? (sizeof(T) == 2 ? 8 : 4) : (sizeof(T) == 2 ? 2 : 1);
+                add_rows<T, VEC, WHOLE, COLS, DEEP>(dout, words, a, b, g, lanes, dim, ld_out, d, o, acc);
             }
-            if (b > a) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) acc[k] = __fmul_rn(acc[k], up);
-            }
-            G* to = dtable + v * ld_table + c;
-            if (VEC && c + 8 <= dim) {
-                if (HEADS) {
-                    float old[8];
-                    widen8<G>(load8<G, false>(to), old);
+            for (int q = 0; q < COLS; ++q) {
+                if (q > 0 && c + q * lanes * 8 >= dim) break;
+                G* to = row + c + q * lanes * 8;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) acc[k] = __fadd_rn(old[k], acc[k]);
+                for (int k = 0; k < 8; ++k) acc[q][k] = __fmul_rn(acc[q][k], up);
+                if (VEC && (WHOLE || c + 8 <= dim)) {
+                    if (HEADS) {
+                        float old[8];
+                        widen8<G>(load8<G, false>(to), old);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) acc[q][k] = __fadd_rn(old[k], acc[q][k]);
+                    }
+                    store8<G>(to, acc[q]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (k < dim - c) to[k] = from_f32<G>(HEADS ? __fadd_rn(to_f32<G>(to[k]), acc[q][k]) : acc[q][k]);
                 }
-                store8<G>(to, acc);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (c + k < dim) to[k] = from_f32<G>(HEADS ? __fadd_rn(to_f32<G>(to[k]), acc[k]) : acc[k]);
             }
         }
     }
@@ -354,10 +386,10 @@ static int check_embedding(const gm_embedding_t* e) {
     return GM_OK;
 }
 
-// CTA of tx lanes over the column groups and ty rows, and the grid's second axis for wide rows.
-static void row_shape(int64_t dim, dim3* block, unsigned* grid_y) {
-    const int64_t groups = (dim + 7) / 8;
-    int tx = 8;
+// CTA of tx lanes, each with `cols` column groups, and ty rows; the grid's second axis for wide rows.
+static void row_shape(int64_t dim, int cols, dim3* block, unsigned* grid_y) {
+    const int64_t groups = ((dim + 7) / 8 + cols - 1) / cols;
+    int tx = kRowLanesLeast;
     while (tx < kEmbThreads && tx < groups) tx <<= 1;
     *block = dim3((unsigned)tx, (unsigned)(kEmbThreads / tx));
     const int64_t y = (groups + tx - 1) / tx;
@@ -368,13 +400,13 @@ template <typename T>
 static int launch_embedding_forward(Device* d, const gm_embedding_t* e, uintptr_t table, uintptr_t tokens, uintptr_t out, const Drop& drop) {
     dim3 block;
     unsigned gy = 1;
-    row_shape(e->dim, &block, &gy);
+    row_shape(e->dim, 1, &block, &gy);
     const bool vec = table % 16 == 0 && out % 16 == 0 && e->ld_table * (int)sizeof(T) % 16 == 0 && e->ld_out * (int)sizeof(T) % 16 == 0;
     // four tokens per thread keep more loads in flight; a call too small for that takes one
     const bool many = e->tokens * gy >= (int64_t)d->sm_count * 8 * block.y;
 #define GM_FORWARD(VEC, WHOLE, ROWS)                                                                                                            \
     embedding_forward_kernel<T, VEC, WHOLE, ROWS><<<dim3((unsigned)((e->tokens + block.y * ROWS - 1) / (block.y * ROWS)), gy), block, 0, d->stream>>>( \
-        (const T*)table, (const int*)tokens, (T*)out, e->tokens, e->dim, e->vocab, e->ld_table, e->ld_out, e->scale, drop)
+        (const T*)table, (const int*)tokens, (T*)out, (int)e->tokens, (int)e->dim, (int)e->vocab, (int)e->ld_table, (int)e->ld_out, e->scale, drop)
     const bool whole = e->dim % 8 == 0;
     if (!vec) GM_FORWARD(false, false, 1);
     else if (!whole) GM_FORWARD(true, false, 1);
@@ -412,28 +444,32 @@ static int launch_embedding_backward(Device* d, const gm_embedding_t* e, uintptr
     if (n > kPiece) {
         const int64_t y = (groups + 127) / 128;
         const dim3 grid((unsigned)((n + kPiece - 1) / kPiece), (unsigned)(y < 65535 ? y : 65535));
-        if (vec && whole) embedding_pieces_kernel<T, true, true><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, n, e->dim, e->vocab, e->ld_out, drop);
-        else if (vec) embedding_pieces_kernel<T, true, false><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, n, e->dim, e->vocab, e->ld_out, drop);
-        else embedding_pieces_kernel<T, false, false><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, n, e->dim, e->vocab, e->ld_out, drop);
+        if (vec && whole) embedding_pieces_kernel<T, true, true><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, (int)n, (int)e->dim, (int)e->vocab, (int)e->ld_out, drop);
+        else if (vec) embedding_pieces_kernel<T, true, false><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, (int)n, (int)e->dim, (int)e->vocab, (int)e->ld_out, drop);
+        else embedding_pieces_kernel<T, false, false><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, (int)n, (int)e->dim, (int)e->vocab, (int)e->ld_out, drop);
         d->launches++;
     }
+    // four groups per lane where that still fills a warp: the bookkeeping of a row is paid less often
+    const bool wide = vec && whole && groups >= 128;
     dim3 block;
     unsigned gy = 1;
-    row_shape(e->dim, &block, &gy);
+    row_shape(e->dim, wide ? 4 : 1, &block, &gy);
     const int64_t items = accumulate ? n : e->vocab;
     const int64_t per_cta = (int64_t)block.y * kRowTurns;
     const dim3 grid((unsigned)((items + per_cta - 1) / per_cta), gy);
-#define GM_ROWS(VEC, WHOLE, HEADS)                                                                                                   \
-    embedding_rows_kernel<T, G, VEC, WHOLE, HEADS><<<grid, block, 0, d->stream>>>((const T*)dout, words, first, pieces, (G*)dtable, n, \
-                                                                           e->dim, e->vocab, e->ld_table, e->ld_out, e->scale, drop)
+#define GM_ROWS(VEC, WHOLE, HEADS, COLS)                                                                                        \
+    embedding_rows_kernel<T, G, VEC, WHOLE, HEADS, COLS><<<grid, block, 0, d->stream>>>(                                         \
+        (const T*)dout, words, first, pieces, (G*)dtable, (int)n, (int)e->dim, (int)e->vocab, (int)e->ld_table, (int)e->ld_out, e->scale, drop)
     if (accumulate) {
-        if (vec && whole) GM_ROWS(true, true, true);
-        else if (vec) GM_ROWS(true, false, true);
-        else GM_ROWS(false, false, true);
+        if (wide) GM_ROWS(true, true, true, 4);
+        else if (vec && whole) GM_ROWS(true, true, true, 1);
+        else if (vec) GM_ROWS(true, false, true, 1);
+        else GM_ROWS(false, false, true, 1);
     } else {
-        if (vec && whole) GM_ROWS(true, true, false);
-        else if (vec) GM_ROWS(true, false, false);
-        else GM_ROWS(false, false, false);
+        if (wide) GM_ROWS(true, true, false, 4);
+        else if (vec && whole) GM_ROWS(true, true, false, 1);
+        else if (vec) GM_ROWS(true, false, false, 1);
+        else GM_ROWS(false, false, false, 1);
     }
 #undef GM_ROWS
     d->launches++;

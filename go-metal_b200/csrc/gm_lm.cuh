@@ -82,41 +82,38 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float (
 // reach `cut` = round(p * 65536).  What stays is multiplied by 65536 / (65536 - cut), which
 // makes the expectation exact for the probability that is really used, cut / 65536.
 struct Drop {
-    unsigned k0, k1;                     // seed
+    unsigned key[20];                    // the ten rounds' keys: the seed, and after each round the Weyl constants on top
     unsigned o0, o1;                     // offset
     const unsigned long long* more;      // null, or a device word that is added to the offset
     unsigned cut;                        // 0: everything stays, no generator
     float up;
 };
 
-__device__ __forceinline__ void drop_begin(Drop& d) {
-    if (d.cut != 0u && d.more != nullptr) {
-        const unsigned long long o = (((unsigned long long)d.o1 << 32) | d.o0) + *d.more;
-        d.o0 = (unsigned)o;
-        d.o1 = (unsigned)(o >> 32);
-    }
+// The offset this launch uses.
+struct DropOffset { unsigned o0, o1; };
+__device__ __forceinline__ DropOffset drop_begin(const Drop& d) {
+    if (d.cut == 0u || d.more == nullptr) return {d.o0, d.o1};
+    const unsigned long long o = (((unsigned long long)d.o1 << 32) | d.o0) + *d.more;
+    return {(unsigned)o, (unsigned)(o >> 32)};
 }
 
 // The 128 bits of one block, elements 2k and 2k + 1 in the low and high half of word k.
-__device__ __forceinline__ void drop_words(const Drop& d, const unsigned long long block, unsigned (&w)[4]) {
-    unsigned c0 = (unsigned)block, c1 = (unsigned)(block >> 32), c2 = d.o0, c3 = d.o1;
-    unsigned k0 = d.k0, k1 = d.k1;
+__device__ __forceinline__ void drop_words(const Drop& d, const DropOffset& o, const unsigned long long block, unsigned (&w)[4]) {
+    unsigned c0 = (unsigned)block, c1 = (unsigned)(block >> 32), c2 = o.o0, c3 = o.o1;
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
         const unsigned long long a = (unsigned long long)0xD2511F53u * c0, b = (unsigned long long)0xCD9E8D57u * c2;
-        c0 = (unsigned)(b >> 32) ^ c1 ^ k0;
+        c0 = (unsigned)(b >> 32) ^ c1 ^ d.key[2 * r];
         c1 = (unsigned)b;
-        c2 = (unsigned)(a >> 32) ^ c3 ^ k1;
+        c2 = (unsigned)(a >> 32) ^ c3 ^ d.key[2 * r + 1];
         c3 = (unsigned)a;
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
     }
     w[0] = c0; w[1] = c1; w[2] = c2; w[3] = c3;
 }
 
 // Zeroes the dropped ones of a whole block of eight elements.  A half reaches the cut when the
 // word that has it on top reaches the cut shifted up: two compares and one shift per word.
-__device__ __forceinline__ void drop_block(const Drop& d, const unsigned long long block, float (&x)[8]) {
+__device__ __forceinline__ void drop_block(const Drop& d, const DropOffset& o, const unsigned long long block, float (&x)[8]) {
     if (d.cut == 0u) return;
     if (d.cut > 0xffffu) {
 #pragma unroll
@@ -124,7 +121,7 @@ __device__ __forceinline__ void drop_block(const Drop& d, const unsigned long lo
         return;
     }
     unsigned w[4];
-    drop_words(d, block, w);
+    drop_words(d, o, block, w);
     const unsigned top = d.cut << 16;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -134,9 +131,9 @@ __device__ __forceinline__ void drop_block(const Drop& d, const unsigned long lo
 }
 
 // Bit k: element 8 * block + k stays.
-__device__ __forceinline__ unsigned drop_bits(const Drop& d, const unsigned long long block) {
+__device__ __forceinline__ unsigned drop_bits(const Drop& d, const DropOffset& o, const unsigned long long block) {
     unsigned w[4];
-    drop_words(d, block, w);
+    drop_words(d, o, block, w);
     unsigned keep = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -147,21 +144,21 @@ __device__ __forceinline__ unsigned drop_bits(const Drop& d, const unsigned long
 }
 
 // Bit k: element first + k stays, for eight elements that may begin inside a block.
-__device__ __forceinline__ unsigned drop_mask8(const Drop& d, const unsigned long long first) {
+__device__ __forceinline__ unsigned drop_mask8(const Drop& d, const DropOffset& o, const unsigned long long first) {
     if (d.cut == 0u) return 0xffu;
-    unsigned keep = drop_bits(d, first >> 3);
+    unsigned keep = drop_bits(d, o, first >> 3);
     const unsigned skip = (unsigned)first & 7u;
-    if (skip != 0u) keep = (keep | (drop_bits(d, (first >> 3) + 1) << 8)) >> skip;
+    if (skip != 0u) keep = (keep | (drop_bits(d, o, (first >> 3) + 1) << 8)) >> skip;
     return keep & 0xffu;
 }
 
 // Zeroes the dropped ones of eight elements from `first` on; WHOLE: they are a block.
 template <bool WHOLE>
-__device__ __forceinline__ void drop8(const Drop& d, const unsigned long long first, float (&x)[8]) {
+__device__ __forceinline__ void drop8(const Drop& d, const DropOffset& o, const unsigned long long first, float (&x)[8]) {
     if (WHOLE) {
-        drop_block(d, first >> 3, x);
+        drop_block(d, o, first >> 3, x);
     } else {
-        const unsigned keep = drop_mask8(d, first);
+        const unsigned keep = drop_mask8(d, o, first);
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] = (keep >> k) & 1u ? x[k] : 0.0f;
     }
@@ -176,8 +173,7 @@ int make_drop(const gm_dropout_t* in, Drop* out);
 // A buffer of at least `need` bytes on this device, aligned to `align`; need 0 checks the rest.
 int check_buffer(const Device* d, uintptr_t p, int64_t need, int64_t align, const char* what);
 
-// Rows and columns in [1, 2^31), a row stride that covers the columns, and a size whose byte
-// offsets fit 64 bits with room to spare.
+// Rows, columns and the row stride in [1, 2^31), and a stride that covers the columns.
 int check_matrix(int64_t rows, int64_t cols, int64_t ld, const char* what);
 
 // Bytes from a matrix's first element to behind its last one.
