@@ -15,7 +15,6 @@ namespace gm {
 constexpr int kEmbThreads = 256;
 constexpr int kSortTile = 1024;          // words one CTA sorts in registers and shared memory
 constexpr int kMergeWays = 8;            // sorted runs that one merge pass joins
-constexpr int kPiece = 32;               // sorted words whose sum is one piece of a long row
 
 // ---------------------------------------------------------------- forward
 // A CTA is tx lanes over groups of eight columns times ty tokens; each thread takes ROWS
@@ -78,14 +77,19 @@ __device__ __forceinline__ unsigned long long sort_word(const int* tokens, long 
 }
 
 // Bitonic sort of 1,024 words, one per thread: strides below a warp by shuffle, the others
-// through shared memory.
+// through shared memory.  The same launch clears `used`, one byte per row of the table (a
+// multiple of 16 of them), and the number of rows split over chunks; the launch after it, or this one where a tile is all there is, marks
+// the rows that tokens point at.
 __global__ void __launch_bounds__(kSortTile)
 token_sort_tile_kernel(const int* __restrict__ tokens, const long long n, const long long vocab, const long long padding,
-                       unsigned long long* __restrict__ out) {
+                       unsigned long long* __restrict__ out, unsigned char* used, int* split) {
     __shared__ unsigned long long buf[kSortTile];
     const int tid = threadIdx.x;
     const long long i = (long long)blockIdx.x * kSortTile + tid;
     unsigned long long key = i < n ? sort_word(tokens, i, vocab, padding) : ~0ull;
+    if (i == 0) *split = 0;
+    if (used)
+        for (long long c = i * 16; c < vocab; c += (long long)gridDim.x * kSortTile * 16) *reinterpret_cast<uint4*>(used + c) = make_uint4(0u, 0u, 0u, 0u);
     for (int size = 2; size <= kSortTile; size <<= 1) {
         const bool up = (tid & size) == 0;
         for (int stride = size >> 1; stride > 0; stride >>= 1) {
@@ -104,6 +108,10 @@ token_sort_tile_kernel(const int* __restrict__ tokens, const long long n, const 
         }
     }
     if (i < n) out[i] = key;
+    if (used && gridDim.x == 1) {
+        __syncthreads();
+        if (i < n && (key >> 32) < (unsigned long long)vocab) used[key >> 32] = 1;
+    }
 }
 
 // The token of a sorted word.
@@ -127,11 +135,13 @@ __device__ __forceinline__ long long first_at(const unsigned long long* __restri
 // of a later run behind: comparing tokens is enough.  The bisections, chains of dependent loads,
 // go in step.
 __global__ void __launch_bounds__(128)
-token_merge_kernel(const unsigned long long* __restrict__ in, unsigned long long* __restrict__ out, const long long n, const int run) {
+token_merge_kernel(const unsigned long long* __restrict__ in, unsigned long long* __restrict__ out, const long long n, const int run,
+                   unsigned char* used, const unsigned vocab) {
     const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
     if (i >= n) return;
     const unsigned long long word = __ldg(in + i);
     const unsigned token = (unsigned)(word >> 32);
+    if (used && token < vocab) used[token] = 1;
     const long long base = i / ((long long)run * kMergeWays) * ((long long)run * kMergeWays);
     const int mine = (int)((i - base) / run);
     int below[kMergeWays], len[kMergeWays];
@@ -152,218 +162,193 @@ token_merge_kernel(const unsigned long long* __restrict__ in, unsigned long long
     out[place] = word;
 }
 
-// first[v] = number of sorted words whose token is below v, for v in [0, vocab].
-__global__ void __launch_bounds__(256)
-token_first_kernel(const unsigned long long* __restrict__ words, const long long n, const long long vocab, int* __restrict__ first) {
-    const long long v = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (v <= vocab) first[v] = (int)first_at(words, 0, n, (unsigned)v);
-}
-
 // ---------------------------------------------------------------- backward sums
-// Adds the rows of dout that words [a, b) name, in order, to acc: COLS groups of eight columns,
-// `apart` groups from one to the next, the first one g.  COLS x DEEP loads are in flight.
-template <typename T, bool VEC, bool WHOLE, int COLS, int DEEP>
-__device__ __forceinline__ void add_rows(const T* __restrict__ dout, const unsigned long long* __restrict__ words, long long a, const long long b,
-                                         const int g, const int apart, const int dim, const int ld_out, const Drop& d, const DropOffset& o,
-                                         float (&acc)[COLS][8]) {
-    const int c0 = g << 3;
-    if (VEC && (WHOLE || c0 + 8 <= dim)) {                            // without WHOLE there is one group per thread
-        while (a < b) {
-            Raw8<T> raw[DEEP][COLS];
-            unsigned pos[DEEP];
-            const int m = b - a < DEEP ? (int)(b - a) : DEEP;
+// The sorted words are cut into chunks of `piece` (at most kPieceMost).  A CTA walks one chunk for
+// 1,024 columns, eight loads per thread in flight whatever rows they belong to, and writes a
+// row's sum when its last word has been added.  So every CTA has the same work, and a token that
+// fills half the batch is spread over the GPU.  A row whose words lie in several chunks leaves a
+// partial sum per chunk (slot 2j: chunk j's part of a row that began before it; slot 2j + 1: that
+// of a row that begins in it and goes on) and its first chunk in a list, and embedding_join_kernel
+// adds them up.  The list's order is chance, the sums are not.
+//
+// The same launch holds, without ADD, the CTAs that zero the rows no token points at: they have no
+// loads to wait for and fill the time of those that do, alternating with them in proportion.
+constexpr int kSumThreads = 128;
+constexpr int kSumDeep = 8;
+constexpr int kPieceMost = 32;
+constexpr int kZeroRows = 32;
+
+// What becomes of a finished row: times `up`, added to what is there (ADD) or not.
+template <typename G, bool VEC, bool WHOLE, bool ADD>
+__device__ __forceinline__ void put_row(G* to, float (&x)[8], const float up, const int cols) {
 #pragma unroll
-            for (int j = 0; j < DEEP; ++j)
-                if (j < m) {
-                    pos[j] = __ldg(reinterpret_cast<const unsigned*>(words + a + j));
-                    const T* row = dout + (long long)pos[j] * ld_out + c0;
+    for (int k = 0; k < 8; ++k) x[k] = __fmul_rn(x[k], up);
+    if (VEC && (WHOLE || cols >= 8)) {
+        if (ADD) {
+            float old[8];
+            widen8<G>(load8<G, false>(to), old);
 #pragma unroll
-                    for (int q = 0; q < COLS; ++q)
-                        if (q == 0 || c0 + q * apart * 8 < dim) raw[j][q] = load8<T, false>(row + q * apart * 8);
-                }
-#pragma unroll
-            for (int j = 0; j < DEEP; ++j)
-                if (j < m) {
-#pragma unroll
-                    for (int q = 0; q < COLS; ++q)
-                        if (q == 0 || c0 + q * apart * 8 < dim) {
-                            float x[8];
-                            widen8<T>(raw[j][q], x);
-                            drop8<WHOLE>(d, o, (unsigned long long)((long long)pos[j] * dim + c0 + q * apart * 8), x);
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) acc[q][k] = __fadd_rn(acc[q][k], x[k]);
-                        }
-                }
-            a += m;
+            for (int k = 0; k < 8; ++k) x[k] = __fadd_rn(old[k], x[k]);
         }
+        store8<G>(to, x);
     } else {
-        for (; a < b; ++a) {
-            const long long p = __ldg(reinterpret_cast<const unsigned*>(words + a));
-            const unsigned keep = drop_mask8(d, o, (unsigned long long)(p * dim + c0));
-            for (int k = 0; k < 8 && k < dim - c0; ++k)
-                if ((keep >> k) & 1u) acc[0][k] = __fadd_rn(acc[0][k], to_f32<T>(dout[p * ld_out + c0 + k]));
-        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < cols) to[k] = from_f32<G>(ADD ? __fadd_rn(to_f32<G>(to[k]), x[k]) : x[k]);
     }
 }
 
-// The row of table that a word with this token belongs to: its words are [a, b).
-__device__ __forceinline__ void row_of(const unsigned long long* __restrict__ words, const int* __restrict__ first, const long long n,
-                                       const unsigned key, long long* a, long long* b) {
-    if (first) {
-        *a = __ldg(first + key);
-        *b = __ldg(first + key + 1);
-    } else {
-        *a = first_at(words, 0, n, key);
-        *b = first_at(words, *a, n, key + 1u);
-    }
-}
-
-// A row of more than kPiece words is summed in pieces of kPiece, counted from its first word, so
-// that a token that fills half the batch is still spread over the GPU.  A piece that begins at
-// word s leaves its sum in slot 2 (s / kPiece), the row's first piece in the slot behind that:
-// among kPiece neighbouring words there begin at most one first piece and one other.
-template <typename T, bool VEC, bool WHOLE>
-__global__ void __launch_bounds__(128)
-embedding_pieces_kernel(const T* __restrict__ dout, const unsigned long long* __restrict__ words, const int* __restrict__ first,
-                        float* __restrict__ pieces, const int n, const int dim, const int vocab, const int ld_out, const __grid_constant__ Drop d) {
-    __shared__ long long from[2], to[2];
+template <typename T, typename G, bool VEC, bool WHOLE, bool ADD>
+__global__ void __launch_bounds__(kSumThreads)
+embedding_sum_kernel(const T* __restrict__ dout, const unsigned long long* __restrict__ words, const unsigned char* __restrict__ used,
+                     float* __restrict__ pieces, int* split, G* dtable, const int n, const int dim, const int vocab, const int ld_table,
+                     const int ld_out, const float scale, const int piece, const int col_ctas, const int sum_ctas, const __grid_constant__ Drop d) {
+    __shared__ unsigned tok[kPieceMost], pos[kPieceMost];
     const int tid = threadIdx.x;
-    const long long begin = (long long)blockIdx.x * kPiece;
-    if (tid < 2) from[tid] = -1;
-    __syncthreads();
-    if (tid < kPiece && begin + tid < n) {
-        const long long i = begin + tid;
-        const unsigned key = token_at(words, i);
-        // a row of more than kPiece words has a word of its own kPiece places on or back
-        const bool maybe = key < (unsigned)vocab && ((i + kPiece < n && token_at(words, i + kPiece) == key) || (i >= kPiece && token_at(words, i - kPiece) == key));
-        if (maybe) {
-            long long a, b;
-            row_of(words, first, n, key, &a, &b);
-            if ((i - a) % kPiece == 0) {
-                const int side = i == a ? 1 : 0;
-                from[side] = i;
-                to[side] = i + kPiece < b ? i + kPiece : b;
+    const int groups = (int)(((unsigned)dim + 7u) >> 3);
+    const long long before = ADD ? blockIdx.x : (long long)blockIdx.x * sum_ctas / gridDim.x;       // summing CTAs in front of this one
+    if (!ADD && ((long long)blockIdx.x + 1) * sum_ctas / gridDim.x == before) {
+        const long long v0 = (blockIdx.x - before) * kZeroRows;
+        if (tid < kZeroRows) tok[tid] = v0 + tid < vocab ? used[v0 + tid] : 1u;
+        __syncthreads();
+        // lanes over the groups of a row, and several rows at a time where a row is narrow
+        const int lanes = groups >= kSumThreads ? kSumThreads : groups > 32 ? 64 : groups > 16 ? 32 : groups > 8 ? 16 : 8;
+        for (int r = tid / lanes; r < kZeroRows; r += kSumThreads / lanes) {
+            if (tok[r]) continue;
+            G* const row = dtable + (v0 + r) * ld_table;
+            for (int g = tid & (lanes - 1); g < groups; g += lanes) {
+                if (VEC && (WHOLE || g * 8 + 8 <= dim)) {
+                    uint4* to = reinterpret_cast<uint4*>(row + g * 8);
+                    __stcs(to, make_uint4(0u, 0u, 0u, 0u));
+                    if (sizeof(G) == 4) __stcs(to + 1, make_uint4(0u, 0u, 0u, 0u));
+                } else {
+                    for (int k = 0; k < 8 && k < dim - g * 8; ++k) row[g * 8 + k] = from_f32<G>(0.0f);
+                }
             }
         }
+        return;
+    }
+    const long long chunk = before / col_ctas, begin = chunk * piece;
+    const int most = n - begin < piece ? (int)(n - begin) : piece;
+    if (tid < most) {
+        const unsigned long long w = __ldg(words + begin + tid);
+        tok[tid] = (unsigned)(w >> 32);
+        pos[tid] = (unsigned)w;
     }
     __syncthreads();
-    if (from[0] < 0 && from[1] < 0) return;
+    const int len = __syncthreads_count(tid < most && tok[tid] < (unsigned)vocab);     // those without a gradient are behind all others
+    if (len == 0) return;
+    const bool from_before = begin > 0 && token_at(words, begin - 1) == tok[0];
+    const bool goes_on = begin + len < n && token_at(words, begin + len) == tok[len - 1];
+    if (tid == 0 && goes_on && before == chunk * col_ctas && !(from_before && tok[0] == tok[len - 1])) split[1 + atomicAdd(split, 1)] = (int)chunk;
     const DropOffset o = drop_begin(d);
-    const int groups = (int)(((unsigned)dim + 7u) >> 3);
-    for (int g = blockIdx.y * 128 + tid; g < groups; g += gridDim.y * 128) {
-#pragma unroll 1
-        for (int side = 0; side < 2; ++side) {
-            if (from[side] < 0) continue;
-            float acc[1][8] = {};
-            add_rows<T, VEC, WHOLE, 1, 8>(dout, words, from[side], to[side], g, 0, dim, ld_out, d, o, acc);
-            float4* p = reinterpret_cast<float4*>(pieces + ((2 * (long long)blockIdx.x + side) * groups + g) * 8);
-            p[0] = make_float4(acc[0][0], acc[0][1], acc[0][2], acc[0][3]);
-            p[1] = make_float4(acc[0][4], acc[0][5], acc[0][6], acc[0][7]);
+    const float up = __fmul_rn(scale, d.up);
+    const int g = (int)(before - chunk * col_ctas) * kSumThreads + tid, c = g << 3;
+    if (g >= groups) return;
+    const bool vec = VEC && (WHOLE || c + 8 <= dim);
+    bool head = from_before;                                          // the current row began in an earlier chunk
+    float acc[8] = {};
+    for (int base = 0; base < len; base += kSumDeep) {
+        Raw8<T> raw[kSumDeep];
+        if (vec) {
+#pragma unroll
+            for (int j = 0; j < kSumDeep; ++j)
+                if (base + j < len) raw[j] = load8<T, false>(dout + (long long)pos[base + j] * ld_out + c);
+        }
+#pragma unroll
+        for (int j = 0; j < kSumDeep; ++j) {
+            if (base + j >= len) break;
+            float x[8] = {};
+            const long long p = pos[base + j];
+            if (vec) {
+                widen8<T>(raw[j], x);
+            } else {
+                for (int k = 0; k < 8 && k < dim - c; ++k) x[k] = to_f32<T>(dout[p * ld_out + c + k]);
+            }
+            drop8<WHOLE>(d, o, (unsigned long long)(p * dim + c), x);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] = __fadd_rn(acc[k], x[k]);
+            const bool last = base + j + 1 == len;
+            if (last || tok[base + j + 1] != tok[base + j]) {
+                if (head || (last && goes_on)) {
+                    float4* to = reinterpret_cast<float4*>(pieces + ((2 * chunk + (head ? 0 : 1)) * groups + g) * 8);
+                    to[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                    to[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                } else {
+                    put_row<G, VEC, WHOLE, ADD>(dtable + (long long)tok[base + j] * ld_table + c, acc, up, dim - c);
+                }
+                head = false;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) acc[k] = 0.0f;
+            }
         }
     }
 }
 
-// HEADS false: items are the table's rows, every one is written.  HEADS true (accumulate): items
-// are the sorted words; one that begins a row adds to it, the others are passed over.  A CTA is
-// tx lanes, each with COLS groups of eight columns, times ty items at a time, kRowTurns times.
-constexpr int kRowTurns = 8;
-constexpr int kRowLanesLeast = 8;
-template <typename T, typename G, bool VEC, bool WHOLE, bool HEADS, int COLS>
-__global__ void __launch_bounds__(kEmbThreads, 3)
-embedding_rows_kernel(const T* __restrict__ dout, const unsigned long long* __restrict__ words, const int* __restrict__ first,
-                      const float* __restrict__ pieces, G* dtable, const int n, const int dim, const int vocab, const int ld_table,
-                      const int ld_out, const float scale, const __grid_constant__ Drop d) {
-    // where the CTA's rows begin and end (its words' tokens, and the one before), read at once
-    __shared__ int mark[kEmbThreads / kRowLanesLeast * kRowTurns + 1];
-    const int items = blockDim.y * kRowTurns;
-    const long long item0 = (long long)blockIdx.x * items;
-    for (int i = threadIdx.y * blockDim.x + threadIdx.x; i <= items; i += kEmbThreads) {
-        const long long at = HEADS ? item0 + i - 1 : item0 + i;
-        if (HEADS) mark[i] = at >= 0 && at < n ? (int)token_at(words, at) : vocab;
-        else mark[i] = at <= vocab ? __ldg(first + at) : 0;
-    }
-    __syncthreads();
-    const DropOffset o = drop_begin(d);
-    const int groups = (int)(((unsigned)dim + 7u) >> 3), lanes = blockDim.x;
+// Adds up the partial sums of the listed rows: four lanes over a row's chunks, each a contiguous
+// share, joined in order.
+constexpr int kJoinLanes = 64, kJoinWays = 4;
+template <typename G, bool VEC, bool WHOLE, bool ADD>
+__global__ void __launch_bounds__(kJoinLanes * kJoinWays)
+embedding_join_kernel(const unsigned long long* __restrict__ words, const float* __restrict__ pieces, const int* __restrict__ split, G* dtable,
+                      const int n, const int dim, const int ld_table, const float scale, const int piece, const __grid_constant__ Drop d) {
+    __shared__ float4 part[kJoinWays][2][kJoinLanes];
+    const int x = threadIdx.x, y = threadIdx.y;
+    const int groups = (int)(((unsigned)dim + 7u) >> 3), col_blocks = (groups + kJoinLanes - 1) / kJoinLanes;
     const float up = __fmul_rn(scale, d.up);
-#pragma unroll 1
-    for (int turn = 0; turn < kRowTurns; ++turn) {
-        const int slot = turn * blockDim.y + threadIdx.y;
-        const long long item = item0 + slot;
-        int v;
-        long long a, b;
-        if (HEADS) {
-            if (item >= n) return;
-            v = mark[slot + 1];
-            if (v >= vocab || (item > 0 && mark[slot] == v)) continue;
-            a = item;
-            b = item + 1;
-            if (b < n && token_at(words, b) == (unsigned)v) b = first_at(words, b, n, (unsigned)v + 1u);
-        } else {
-            if (item >= vocab) return;
-            v = (int)item;
-            a = mark[slot];
-            b = mark[slot + 1];
+    const long long items = (long long)split[0] * col_blocks;
+    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+        const long long chunk = split[1 + item / col_blocks];
+        const int g = (int)(item % col_blocks) * kJoinLanes + x;
+        const unsigned key = token_at(words, (chunk + 1) * piece);
+        // the row's last chunk: chunks whose first word is the row's, 32 looked at together
+        long long last = chunk;
+        for (;;) {
+            const long long at = (last + 1 + (x & 31)) * piece;
+            const unsigned hit = __ballot_sync(0xffffffffu, at < n && token_at(words, at) == key);
+            last += hit == 0xffffffffu ? 32 : __ffs((int)~hit) - 1;
+            if (hit != 0xffffffffu) break;
         }
-        G* const row = dtable + (long long)v * ld_table;
-        for (int g = blockIdx.y * lanes * COLS + threadIdx.x; g < groups; g += gridDim.y * lanes * COLS) {
-            const int c = g << 3;
-            if (!HEADS && VEC && WHOLE && a == b) {                       // a row of zeros, most of them in a large table
-#pragma unroll
-                for (int q = 0; q < COLS; ++q)
-                    if (q == 0 || c + q * lanes * 8 < dim) {
-                        uint4* to = reinterpret_cast<uint4*>(row + c + q * lanes * 8);
-                        __stcs(to, make_uint4(0u, 0u, 0u, 0u));
-                        if (sizeof(G) == 4) __stcs(to + 1, make_uint4(0u, 0u, 0u, 0u));
-                    }
-                continue;
-            }
-            float acc[COLS][8] = {};
-            if (b - a > kPiece) {
-#pragma unroll 2
-                for (long long s = a; s < b; s += kPiece) {
-                    const float* p = pieces + (2 * (s / kPiece) + (s == a ? 1 : 0)) * groups * 8 + c;
-#pragma unroll
-                    for (int q = 0; q < COLS; ++q)
-                        if (q == 0 || c + q * lanes * 8 < dim) {
-                            const float4* at = reinterpret_cast<const float4*>(p + q * lanes * 8);
-                            const float4 x = at[0], y = at[1];
-                            acc[q][0] = __fadd_rn(acc[q][0], x.x); acc[q][1] = __fadd_rn(acc[q][1], x.y);
-                            acc[q][2] = __fadd_rn(acc[q][2], x.z); acc[q][3] = __fadd_rn(acc[q][3], x.w);
-                            acc[q][4] = __fadd_rn(acc[q][4], y.x); acc[q][5] = __fadd_rn(acc[q][5], y.y);
-                            acc[q][6] = __fadd_rn(acc[q][6], y.z); acc[q][7] = __fadd_rn(acc[q][7], y.w);
-                        }
-                }
-            } else if (b > a) {
-                constexpr int DEEP = COLS == 1 ? (sizeof(T) == 2 ? 8 : 4) : (sizeof(T) == 2 ? 2 : 1);
-                add_rows<T, VEC, WHOLE, COLS, DEEP>(dout, words, a, b, g, lanes, dim, ld_out, d, o, acc);
-            }
-#pragma unroll
-            for (int q = 0; q < COLS; ++q) {
-                if (q > 0 && c + q * lanes * 8 >= dim) break;
-                G* to = row + c + q * lanes * 8;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) acc[q][k] = __fmul_rn(acc[q][k], up);
-                if (VEC && (WHOLE || c + 8 <= dim)) {
-                    if (HEADS) {
-                        float old[8];
-                        widen8<G>(load8<G, false>(to), old);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) acc[q][k] = __fadd_rn(old[k], acc[q][k]);
-                    }
-                    store8<G>(to, acc[q]);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (k < dim - c) to[k] = from_f32<G>(HEADS ? __fadd_rn(to_f32<G>(to[k]), acc[q][k]) : acc[q][k]);
-                }
+        const long long share = (last - chunk + kJoinWays) / kJoinWays;   // chunks [chunk, last] over the ways
+        float acc[8] = {};
+        if (g < groups) {
+            const long long from = chunk + y * share, to = from + share - 1 < last ? from + share - 1 : last;
+#pragma unroll 4
+            for (long long j = from; j <= to; ++j) {
+                const float4* p = reinterpret_cast<const float4*>(pieces + ((2 * j + (j == chunk ? 1 : 0)) * groups + g) * 8);
+                const float4 u = p[0], v = p[1];
+                acc[0] = __fadd_rn(acc[0], u.x); acc[1] = __fadd_rn(acc[1], u.y);
+                acc[2] = __fadd_rn(acc[2], u.z); acc[3] = __fadd_rn(acc[3], u.w);
+                acc[4] = __fadd_rn(acc[4], v.x); acc[5] = __fadd_rn(acc[5], v.y);
+                acc[6] = __fadd_rn(acc[6], v.z); acc[7] = __fadd_rn(acc[7], v.w);
             }
         }
+        part[y][0][x] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        part[y][1][x] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+        __syncthreads();
+        if (y == 0 && g < groups) {
+            for (int w = 1; w < kJoinWays; ++w) {
+                const float4 u = part[w][0][x], v = part[w][1][x];
+                acc[0] = __fadd_rn(acc[0], u.x); acc[1] = __fadd_rn(acc[1], u.y);
+                acc[2] = __fadd_rn(acc[2], u.z); acc[3] = __fadd_rn(acc[3], u.w);
+                acc[4] = __fadd_rn(acc[4], v.x); acc[5] = __fadd_rn(acc[5], v.y);
+                acc[6] = __fadd_rn(acc[6], v.z); acc[7] = __fadd_rn(acc[7], v.w);
+            }
+            put_row<G, VEC, WHOLE, ADD>(dtable + (long long)key * ld_table + (g << 3), acc, up, dim - (g << 3));
+        }
+        __syncthreads();
     }
 }
 
 // ---------------------------------------------------------------- host side
-struct EmbSpace { int64_t words0, words1, first, pieces, total; };
+// Sorted words per chunk.  32 in a large call; 8 where 32 would leave SMs without a CTA: the walk
+// over a chunk is serial, and a small call is as long as one walk.
+static int piece_of(const gm_embedding_t* e) {
+    const int64_t ctas = (e->tokens + 31) / 32 * (((e->dim + 7) / 8 + kSumThreads - 1) / kSumThreads);
+    return ctas >= 148 * 8 ? 32 : 8;
+}
+
+struct EmbSpace { int64_t words0, words1, used, split, pieces, total; };
 
 static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 
@@ -371,9 +356,10 @@ static EmbSpace embedding_space(const gm_embedding_t* e) {
     EmbSpace s;
     s.words0 = 0;
     s.words1 = s.words0 + up256(e->tokens * 8);
-    s.first = s.words1 + up256(e->tokens * 8);
-    s.pieces = s.first + up256((e->vocab + 1) * 4);
-    s.total = s.pieces + up256(2 * ((e->tokens + kPiece - 1) / kPiece) * ((e->dim + 7) / 8 * 8) * 4);
+    s.used = s.words1 + up256(e->tokens * 8);
+    s.split = s.used + up256(e->vocab);
+    s.pieces = s.split + up256(((e->tokens + piece_of(e) - 1) / piece_of(e) + 1) * 4);
+    s.total = s.pieces + up256(2 * ((e->tokens + piece_of(e) - 1) / piece_of(e)) * ((e->dim + 7) / 8 * 8) * 4);
     return s;
 }
 
@@ -386,21 +372,20 @@ static int check_embedding(const gm_embedding_t* e) {
     return GM_OK;
 }
 
-// CTA of tx lanes, each with `cols` column groups, and ty rows; the grid's second axis for wide rows.
-static void row_shape(int64_t dim, int cols, dim3* block, unsigned* grid_y) {
-    const int64_t groups = ((dim + 7) / 8 + cols - 1) / cols;
-    int tx = kRowLanesLeast;
-    while (tx < kEmbThreads && tx < groups) tx <<= 1;
-    *block = dim3((unsigned)tx, (unsigned)(kEmbThreads / tx));
-    const int64_t y = (groups + tx - 1) / tx;
-    *grid_y = (unsigned)(y < 65535 ? y : 65535);
+// A CTA of tx lanes, each with `cols` column groups, and as many rows as make 256 threads.
+static dim3 row_block(int64_t dim, int cols) {
+    const int64_t lanes = ((dim + 7) / 8 + cols - 1) / cols;
+    int tx = 8;
+    while (tx < kEmbThreads && tx < lanes) tx <<= 1;
+    return dim3((unsigned)tx, (unsigned)(kEmbThreads / tx));
 }
 
 template <typename T>
 static int launch_embedding_forward(Device* d, const gm_embedding_t* e, uintptr_t table, uintptr_t tokens, uintptr_t out, const Drop& drop) {
-    dim3 block;
-    unsigned gy = 1;
-    row_shape(e->dim, 1, &block, &gy);
+    const dim3 block = row_block(e->dim, 1);
+    // the grid's second axis spreads a wide row over CTAs
+    const int64_t y = ((e->dim + 7) / 8 + block.x - 1) / block.x;
+    const unsigned gy = (unsigned)(y < 65535 ? y : 65535);
     const bool vec = table % 16 == 0 && out % 16 == 0 && e->ld_table * (int)sizeof(T) % 16 == 0 && e->ld_out * (int)sizeof(T) % 16 == 0;
     // four tokens per thread keep more loads in flight; a call too small for that takes one
     const bool many = e->tokens * gy >= (int64_t)d->sm_count * 8 * block.y;
@@ -424,55 +409,47 @@ static int launch_embedding_backward(Device* d, const gm_embedding_t* e, uintptr
     const EmbSpace s = embedding_space(e);
     unsigned long long* words = (unsigned long long*)(ws + s.words0);
     unsigned long long* other = (unsigned long long*)(ws + s.words1);
-    int* first = (int*)(ws + s.first);
+    unsigned char* used = accumulate ? nullptr : (unsigned char*)(ws + s.used);
+    int* split = (int*)(ws + s.split);
     float* pieces = (float*)(ws + s.pieces);
     const int64_t n = e->tokens;
-    token_sort_tile_kernel<<<(unsigned)((n + kSortTile - 1) / kSortTile), kSortTile, 0, d->stream>>>((const int*)tokens, n, e->vocab, e->padding_token, words);
+    token_sort_tile_kernel<<<(unsigned)((n + kSortTile - 1) / kSortTile), kSortTile, 0, d->stream>>>((const int*)tokens, n, e->vocab, e->padding_token, words, used, split);
     d->launches++;
     for (int64_t run = kSortTile; run < n; run *= kMergeWays) {
-        token_merge_kernel<<<(unsigned)((n + 127) / 128), 128, 0, d->stream>>>(words, other, n, (int)run);
+        token_merge_kernel<<<(unsigned)((n + 127) / 128), 128, 0, d->stream>>>(words, other, n, (int)run, run == kSortTile ? used : nullptr, (unsigned)e->vocab);
         d->launches++;
         unsigned long long* t = words; words = other; other = t;
-    }
-    if (!accumulate) {
-        token_first_kernel<<<(unsigned)((e->vocab + 256) / 256), 256, 0, d->stream>>>(words, n, e->vocab, first);
-        d->launches++;
     }
     const bool vec = dout % 16 == 0 && e->ld_out * (int)sizeof(T) % 16 == 0 && dtable % 16 == 0 && e->ld_table * (int)sizeof(G) % 16 == 0;
     const bool whole = e->dim % 8 == 0;
     const int64_t groups = (e->dim + 7) / 8;
-    if (n > kPiece) {
-        const int64_t y = (groups + 127) / 128;
-        const dim3 grid((unsigned)((n + kPiece - 1) / kPiece), (unsigned)(y < 65535 ? y : 65535));
-        if (vec && whole) embedding_pieces_kernel<T, true, true><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, (int)n, (int)e->dim, (int)e->vocab, (int)e->ld_out, drop);
-        else if (vec) embedding_pieces_kernel<T, true, false><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, (int)n, (int)e->dim, (int)e->vocab, (int)e->ld_out, drop);
-        else embedding_pieces_kernel<T, false, false><<<grid, 128, 0, d->stream>>>((const T*)dout, words, accumulate ? nullptr : first, pieces, (int)n, (int)e->dim, (int)e->vocab, (int)e->ld_out, drop);
-        d->launches++;
-    }
-    // four groups per lane where that still fills a warp: the bookkeeping of a row is paid less often
-    const bool wide = vec && whole && groups >= 128;
-    dim3 block;
-    unsigned gy = 1;
-    row_shape(e->dim, wide ? 4 : 1, &block, &gy);
-    const int64_t items = accumulate ? n : e->vocab;
-    const int64_t per_cta = (int64_t)block.y * kRowTurns;
-    const dim3 grid((unsigned)((items + per_cta - 1) / per_cta), gy);
-#define GM_ROWS(VEC, WHOLE, HEADS, COLS)                                                                                        \
-    embedding_rows_kernel<T, G, VEC, WHOLE, HEADS, COLS><<<grid, block, 0, d->stream>>>(                                         \
-        (const T*)dout, words, first, pieces, (G*)dtable, (int)n, (int)e->dim, (int)e->vocab, (int)e->ld_table, (int)e->ld_out, e->scale, drop)
+    const int piece = piece_of(e);
+    const int64_t chunks = (n + piece - 1) / piece, col_ctas = (groups + kSumThreads - 1) / kSumThreads;
+    const int64_t sum_ctas = chunks * col_ctas, zero_ctas = accumulate ? 0 : (e->vocab + kZeroRows - 1) / kZeroRows;
+    if (sum_ctas + zero_ctas > 0x7fffffff) { set_error("%lld tokens of %lld columns are too many", (long long)n, (long long)e->dim); return GM_ERR_BAD_SIZE; }
+    const int64_t join_most = chunks * ((groups + kJoinLanes - 1) / kJoinLanes);
+    const unsigned join_grid = (unsigned)(join_most < d->sm_count * 8 ? join_most : d->sm_count * 8);
+    const dim3 join_block(kJoinLanes, kJoinWays);
+#define GM_SUM(VEC, WHOLE, ADD)                                                                                                                \
+    do {                                                                                                                                       \
+        embedding_sum_kernel<T, G, VEC, WHOLE, ADD><<<(unsigned)(sum_ctas + zero_ctas), kSumThreads, 0, d->stream>>>(                          \
+            (const T*)dout, words, used, pieces, split, (G*)dtable, (int)n, (int)e->dim, (int)e->vocab, (int)e->ld_table, (int)e->ld_out, e->scale,   \
+            piece, (int)col_ctas, (int)sum_ctas, drop);                                                                                       \
+        if (chunks > 1)                                                                                                                       \
+            embedding_join_kernel<G, VEC, WHOLE, ADD><<<join_grid, join_block, 0, d->stream>>>(                                                 \
+                words, pieces, split, (G*)dtable, (int)n, (int)e->dim, (int)e->ld_table, e->scale, piece, drop);                       \
+    } while (0)
     if (accumulate) {
-        if (wide) GM_ROWS(true, true, true, 4);
-        else if (vec && whole) GM_ROWS(true, true, true, 1);
-        else if (vec) GM_ROWS(true, false, true, 1);
-        else GM_ROWS(false, false, true, 1);
+        if (vec && whole) GM_SUM(true, true, true);
+        else if (vec) GM_SUM(true, false, true);
+        else GM_SUM(false, false, true);
     } else {
-        if (wide) GM_ROWS(true, true, false, 4);
-        else if (vec && whole) GM_ROWS(true, true, false, 1);
-        else if (vec) GM_ROWS(true, false, false, 1);
-        else GM_ROWS(false, false, false, 1);
+        if (vec && whole) GM_SUM(true, true, false);
+        else if (vec) GM_SUM(true, false, false);
+        else GM_SUM(false, false, false);
     }
-#undef GM_ROWS
-    d->launches++;
+#undef GM_SUM
+    d->launches += chunks > 1 ? 2 : 1;
     GM_CUDA_CHECK(cudaGetLastError());
     return GM_OK;
 }
