@@ -53,6 +53,7 @@ xent_index_kernel(const int* __restrict__ targets, const int n, const int vocab,
     __shared__ int warp_sum[32];
     __shared__ int carry;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    cudaGridDependencySynchronize();
     if (tid == 0) carry = 0;
     __syncthreads();
     for (long long base = 0; base < n; base += kIndexThreads * 8) {
@@ -98,19 +99,71 @@ xent_index_kernel(const int* __restrict__ targets, const int n, const int vocab,
     if (tid == 0) { sc->count = carry; sc->ticket = 0u; }
 }
 
+// The same for at most kFewIndex rows inside the gathering kernel: every CTA counts the targets
+// for itself and finds the row that is its own.  Saves a launch where a call is mostly launches.
+constexpr int kGatherThreads = 128;
+constexpr int kFewIndex = kGatherThreads * 16;
+__device__ __forceinline__ void find_row(const int* __restrict__ targets, const int n, const int vocab, const int r, int* count, int* row, int* target) {
+    __shared__ int warp_count[kGatherThreads / 32], found[2];
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int per = (n + kGatherThreads - 1) / kGatherThreads;         // at most 16, consecutive
+    unsigned live = 0;
+    for (int k = 0; k < per; ++k) {
+        const int i = tid * per + k;
+        const int t = i < n ? __ldg(targets + i) : -1;
+        if (t >= 0 && t < vocab) live |= 1u << k;
+    }
+    int scan = __popc(live);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += x;
+    }
+    if (lane == 31) warp_count[tid >> 5] = scan;
+    __syncthreads();
+    int total = 0;
+    for (int w = 0; w < kGatherThreads / 32; ++w) {
+        if (w < (tid >> 5)) scan += warp_count[w];
+        total += warp_count[w];
+    }
+    int at = scan - __popc(live);                                      // rows in front of this thread's
+    if (r >= at && r < scan) {
+        for (int k = 0; k < per; ++k)
+            if ((live >> k) & 1u) {
+                if (at == r) { found[0] = tid * per + k; found[1] = __ldg(targets + tid * per + k); }
+                ++at;
+            }
+    }
+    __syncthreads();
+    *count = total;
+    *row = r < total ? found[0] : 0;
+    *target = r < total ? found[1] : 0;
+}
+
 // Gathers the hidden states of the rows with a target, zeroes the rows behind them up to a
 // whole tile, and clears the outputs of rows without a target.  One CTA per row.  With
 // target_logit (forward) it also takes the dot product of the row with its target's row of W.
-constexpr int kGatherThreads = 128;
 template <typename T>
 __global__ void __launch_bounds__(kGatherThreads)
 xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n, const int dim, const int vocab, const int* __restrict__ targets,
-                   const int* __restrict__ rows, const int* __restrict__ target, const XentScalars* __restrict__ sc, T* __restrict__ packed,
+                   int* rows, int* target, XentScalars* sc, const bool few, T* __restrict__ packed,
                    const long long ld_packed, const T* __restrict__ weight, const long long ld_weight, float* __restrict__ target_logit,
                    float* __restrict__ losses, float* __restrict__ lse, T* __restrict__ dhidden, const bool vec, const bool vec_out) {
     __shared__ float warp_sum[kGatherThreads / 32];
     const int r = blockIdx.x, tid = threadIdx.x;
-    const int count = sc->count;
+    cudaGridDependencySynchronize();
+    int count, row, goal;
+    if (few) {
+        find_row(targets, n, vocab, r, &count, &row, &goal);
+        if (tid == 0) {
+            if (r < count) { rows[r] = row; target[r] = goal; }
+            if (r == 0) { sc->count = count; sc->ticket = 0u; }
+        }
+    } else {
+        count = sc->count;
+        row = r < count ? rows[r] : 0;
+        goal = r < count ? target[r] : 0;
+    }
     const int groups = dim >> 3;
     const T zero = from_f32<T>(0.0f);
     if (r < n) {
@@ -132,8 +185,8 @@ xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n
         for (int c = tid; c < dim; c += kGatherThreads) to[c] = zero;
         return;
     }
-    const T* from = hidden + (long long)__ldg(rows + r) * ld;
-    const T* w = target_logit ? weight + (long long)__ldg(target + r) * ld_weight : nullptr;
+    const T* from = hidden + (long long)row * ld;
+    const T* w = target_logit ? weight + (long long)goal * ld_weight : nullptr;
     float dot = 0.0f;
     int c0 = 0;
     if (vec) {
@@ -166,7 +219,7 @@ xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n
 }
 
 // ---------------------------------------------------------------- epilogues
-constexpr int kGroupM = 8;      // m-tiles walked together: 2,048 rows, so W is read once per 2,048 rows
+constexpr int kGroupM = 8;      // m-tiles walked together in the gradient products
 
 // Row maximum and sum of exponentials of one tile of logits, the target's left out.
 template <typename T>
@@ -175,11 +228,12 @@ struct StatsOps {
     const XentScalars* sc;
     const int* target;
     float2* stats;               // [vocabulary tile][row]
-    int rows_cap, dim, vocab, a0, b0;
-    __device__ __forceinline__ TilePlan plan() const {
-        return {(sc->count + kTileM - 1) / kTileM, (vocab + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, kGroupM};
+    int rows_cap, dim, vocab, group, a0, b0;
+    __device__ __forceinline__ TilePlan plan(int) const {
+        return {(sc->count + kTileM - 1) / kTileM, (vocab + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, group, 1};
     }
-    __device__ __forceinline__ void epilogue(int row, int n, unsigned addr, bool) const {
+    __device__ __forceinline__ void epilogue(const TileAt& tile, int in_tile, unsigned addr) const {
+        const int row = tile.m * kTileM + in_tile, n = tile.n;
         const bool live = row < sc->count;
         const int c0 = n * kTileN;
         const int width = vocab - c0 < kTileN ? vocab - c0 : kTileN;
@@ -217,6 +271,66 @@ struct StatsOps {
     }
 };
 
+// The same for a few rows (at most TN): the vocabulary takes the tile's long side, 256 entries by
+// TN rows, so that nothing but the read of W is left.  A warp holds 32 entries of 32 rows at a
+// time, one entry per lane, and reduces over its lanes by halving exchanges, after which lane j
+// has row j: one {maximum, sum} per 32 entries and row.
+template <bool MAX> __device__ __forceinline__ float lanes_to_columns(float (&v)[32], int lane) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const bool upper = (lane & o) != 0;
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const float keep = upper ? v[i + o] : v[i], send = upper ? v[i] : v[i + o];
+            const float got = __shfl_xor_sync(0xffffffffu, send, o);
+            v[i] = MAX ? fmaxf(keep, got) : keep + got;
+        }
+    }
+    return v[0];
+}
+
+template <typename T, int TN>
+struct FewStatsOps {
+    static constexpr bool kBf16 = Half16<T>::kBf16;
+    const XentScalars* sc;
+    const int* target;
+    float2* stats;               // [32 vocabulary entries][row]
+    int rows_cap, dim, vocab, a0, b0;
+    __device__ __forceinline__ TilePlan plan(int) const {
+        return {(vocab + kTileM - 1) / kTileM, sc->count > 0 ? 1 : 0, (dim + kTileK - 1) / kTileK, 1, 1};
+    }
+    __device__ __forceinline__ void epilogue(const TileAt& tile, int in_tile, unsigned addr) const {
+        const int entry = tile.m * kTileM + in_tile, lane = threadIdx.x & 31;
+        const int count = sc->count;
+        if (entry - lane >= vocab) return;                             // the whole warp is behind the table
+#pragma unroll 1
+        for (int c = 0; c < count; c += 32) {
+            float v[32], w[32];
+            tmem_load32(addr + c, v);
+            if (entry >= vocab) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = -INFINITY;
+            }
+            const int goal = c + lane < count ? __ldg(target + c + lane) : -1;
+            for (unsigned hits = __ballot_sync(0xffffffffu, goal >= entry - lane && goal < entry - lane + 32); hits; hits &= hits - 1) {
+                const int j = __ffs((int)hits) - 1;
+                const bool mine = __shfl_sync(0xffffffffu, goal, j) == entry;
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                    if (k == j && mine) v[k] = -INFINITY;              // the target's logit is added by itself
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w[j] = v[j];
+            const float top = lanes_to_columns<true>(w, lane);
+            const float ref = top == -INFINITY ? 0.0f : top * kLog2e;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = exp2f(fmaf(v[j], kLog2e, -__shfl_sync(0xffffffffu, ref, j)));
+            const float sum = lanes_to_columns<false>(v, lane);
+            if (c + lane < count) stats[(long long)(entry >> 5) * rows_cap + c + lane] = make_float2(top, sum);
+        }
+    }
+};
+
 // S of one tile, rounded to 16 bits, into the workspace; zeros behind the last row and column.
 template <typename T>
 struct SoftmaxGradOps {
@@ -227,11 +341,12 @@ struct SoftmaxGradOps {
     const float* lse;            // by row of the caller
     T* ds;
     long long ld_ds;
-    int dim, v0, v1, a0, b0;
-    __device__ __forceinline__ TilePlan plan() const {
-        return {(sc->count + kTileM - 1) / kTileM, (v1 - v0 + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, kGroupM};
+    int dim, v0, v1, group, a0, b0;
+    __device__ __forceinline__ TilePlan plan(int) const {
+        return {(sc->count + kTileM - 1) / kTileM, (v1 - v0 + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, group, 1};
     }
-    __device__ __forceinline__ void epilogue(int row, int n, unsigned addr, bool) const {
+    __device__ __forceinline__ void epilogue(const TileAt& tile, int in_tile, unsigned addr) const {
+        const int row = tile.m * kTileM + in_tile, n = tile.n;
         const bool live = row < sc->count;
         const int c0 = v0 + n * kTileN;
         const int width = live ? (v1 - c0 < kTileN ? v1 - c0 : kTileN) : 0;
@@ -298,56 +413,112 @@ __device__ __forceinline__ void emit32(T* to, const float (&v)[32], int cols, bo
 }
 
 // dX: S [rows, piece] times W [piece, D]; carried in binary32 over the pieces, scattered to the
-// caller's rows by the last one.
+// caller's rows by the last one.  With shares of K the tiles go to `parts` instead, 256 x 256
+// numbers per item, and xent_hidden_join_kernel does the rest.
+struct HiddenPlan {
+    int dim, v0, v1, most_items;
+    __device__ __forceinline__ TilePlan plan(int count, int pairs) const {
+        TilePlan p{(count + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (v1 - v0 + kTileK - 1) / kTileK, kGroupM, 1};
+        p.splits = choose_splits(p.m_tiles * p.n_tiles, p.k_blocks, pairs, most_items);
+        return p;
+    }
+};
+
 template <typename T>
-struct HiddenGradOps {
-    static constexpr bool kBf16 = Half16<T>::kBf16;
-    const XentScalars* sc;
-    const int* rows;
+struct HiddenOut {
     float* carried;
     long long ld_carried;
     T* out;
     long long ld_out;
     GradScale scale;
-    int dim, v0, v1, a0, b0;
     bool first, last, vec;
-    __device__ __forceinline__ TilePlan plan() const {
-        return {(sc->count + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (v1 - v0 + kTileK - 1) / kTileK, kGroupM};
+    // 32 columns from c of one row: what was carried on top, then carried on or written
+    __device__ __forceinline__ void put(int row, int to_row, int c, float (&v)[32], int cols, float c_all) const {
+        float* acc = carried + (long long)row * ld_carried + c;
+        if (!first) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+                if (j < cols) {
+                    const float4 x = *reinterpret_cast<const float4*>(acc + j);
+                    v[j] = __fadd_rn(x.x, v[j]); v[j + 1] = __fadd_rn(x.y, v[j + 1]);
+                    v[j + 2] = __fadd_rn(x.z, v[j + 2]); v[j + 3] = __fadd_rn(x.w, v[j + 3]);
+                }
+        }
+        if (last) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __fmul_rn(v[j], c_all);
+            emit32<T>(out + (long long)to_row * ld_out + c, v, cols, vec, false);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+                if (j < cols) *reinterpret_cast<float4*>(acc + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        }
     }
-    __device__ __forceinline__ void epilogue(int row, int n, unsigned addr, bool) const {
-        const int count = sc->count;
+};
+
+template <typename T>
+struct HiddenGradOps {
+    static constexpr bool kBf16 = Half16<T>::kBf16;
+    const XentScalars* sc;
+    const int* rows;
+    float* parts;
+    HiddenPlan shape;
+    HiddenOut<T> out;
+    int a0, b0;
+    __device__ __forceinline__ TilePlan plan(int pairs) const { return shape.plan(sc->count, pairs); }
+    __device__ __forceinline__ void epilogue(const TileAt& tile, int in_tile, unsigned addr) const {
+        const int count = sc->count, row = tile.m * kTileM + in_tile, n = tile.n;
         const bool live = row < count;
-        const float c_all = scale.value(count);
-        T* to = live && last ? out + (long long)__ldg(rows + row) * ld_out + n * kTileN : nullptr;
-        float* acc = carried + (long long)row * ld_carried + n * kTileN;
-        const int width = dim - n * kTileN < kTileN ? dim - n * kTileN : kTileN;
+        const bool split = tile.k1 - tile.k0 < (shape.v1 - shape.v0 + kTileK - 1) / kTileK;
+        const float c_all = out.scale.value(count);
+        const int to_row = live ? __ldg(rows + row) : 0;
+        const int width = shape.dim - n * kTileN < kTileN ? shape.dim - n * kTileN : kTileN;
+        float* part = parts + (long long)tile.item * (kTileM * kTileN) + in_tile * kTileN;
 #pragma unroll 1
         for (int c = 0; c < width; c += 32) {
             float v[32];
             tmem_load32(addr + c, v);
             if (!live) continue;
-            const int cols = width - c < 32 ? width - c : 32;
-            if (!first) {
+            if (split) {
 #pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    if (j < cols) {
-                        const float4 x = *reinterpret_cast<const float4*>(acc + c + j);
-                        v[j] = __fadd_rn(x.x, v[j]); v[j + 1] = __fadd_rn(x.y, v[j + 1]);
-                        v[j + 2] = __fadd_rn(x.z, v[j + 2]); v[j + 3] = __fadd_rn(x.w, v[j + 3]);
-                    }
-            }
-            if (last) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __fmul_rn(v[j], c_all);
-                emit32<T>(to + c, v, cols, vec, false);
+                for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(part + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
             } else {
-#pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    if (j < cols) *reinterpret_cast<float4*>(acc + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                out.put(row, to_row, n * kTileN + c, v, width - c < 32 ? width - c : 32, c_all);
             }
         }
     }
 };
+
+// Adds up the shares of K, in order, where there are any; one thread per row and 32 columns.
+template <typename T>
+__global__ void __launch_bounds__(256)
+xent_hidden_join_kernel(const XentScalars* __restrict__ sc, const int* __restrict__ rows, const float* __restrict__ parts, const HiddenPlan shape,
+                        const HiddenOut<T> out, const int pairs) {
+    cudaGridDependencySynchronize();
+    const int count = sc->count;
+    const TilePlan plan = shape.plan(count, pairs);
+    if (plan.splits == 1) return;
+    const float c_all = out.scale.value(count);
+    const int strips = (shape.dim + 31) / 32;
+    const long long work = (long long)count * strips;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < work; i += (long long)gridDim.x * 256) {
+        const int row = (int)(i / strips), c = (int)(i - (long long)row * strips) * 32;
+        const int tile = plan.tile_of(row / kTileM, c / kTileN);
+        const float* p = parts + (long long)tile * plan.splits * (kTileM * kTileN) + (row % kTileM) * kTileN + c % kTileN;
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+        for (int s = 0; s < plan.splits; ++s, p += kTileM * kTileN) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(p + j);
+                v[j] = __fadd_rn(v[j], x.x); v[j + 1] = __fadd_rn(v[j + 1], x.y);
+                v[j + 2] = __fadd_rn(v[j + 2], x.z); v[j + 3] = __fadd_rn(v[j + 3], x.w);
+            }
+        }
+        out.put(row, rows[row], c, v, shape.dim - c < 32 ? shape.dim - c : 32, c_all);
+    }
+}
 
 // dW of a piece: S^T [piece, rows] times X [rows, D].
 template <typename T>
@@ -359,11 +530,12 @@ struct WeightGradOps {
     GradScale scale;
     int dim, v0, v1, a0, b0;
     bool add, vec;
-    __device__ __forceinline__ TilePlan plan() const {
-        return {(v1 - v0 + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (sc->count + kTileK - 1) / kTileK, kGroupM};
+    __device__ __forceinline__ TilePlan plan(int) const {
+        return {(v1 - v0 + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (sc->count + kTileK - 1) / kTileK, kGroupM, 1};
     }
-    __device__ __forceinline__ void epilogue(int row, int n, unsigned addr, bool empty) const {
-        const bool live = row < v1 - v0;
+    __device__ __forceinline__ void epilogue(const TileAt& tile, int in_tile, unsigned addr) const {
+        const int row = tile.m * kTileM + in_tile, n = tile.n;
+        const bool live = row < v1 - v0, empty = tile.k0 == tile.k1;
         const float c_all = scale.value(sc->count);
         T* to = out + (long long)(v0 + row) * ld_out + n * kTileN;
         const int width = dim - n * kTileN < kTileN ? dim - n * kTileN : kTileN;
@@ -380,58 +552,64 @@ struct WeightGradOps {
 };
 
 // ---------------------------------------------------------------- joining the row statistics
-// 32 rows by 8 lanes over the vocabulary tiles; the CTA that finishes last adds up the loss.
+struct MaxSum { float m, s; };                       // sum of exponentials relative to the maximum
+__device__ __forceinline__ MaxSum joined(const MaxSum a, const MaxSum b) {
+    const float m = fmaxf(a.m, b.m);
+    const float ref = m == -INFINITY ? 0.0f : m * kLog2e;
+    return {m, fmaf(a.s, exp2f(fmaf(a.m, kLog2e, -ref)), b.s * exp2f(fmaf(b.m, kLog2e, -ref)))};
+}
+
+// A CTA takes ROWS rows with 256 / ROWS lanes over the vocabulary tiles; the CTA that finishes
+// last adds up the loss.  ROWS is 32 (neighbouring lanes read neighbouring rows), or 1 in a small
+// call, where the number of tiles would make the walk long.
+template <int ROWS>
 __global__ void __launch_bounds__(256)
 xent_join_kernel(XentScalars* sc, const float2* __restrict__ stats, const int rows_cap, const int tiles, const float* __restrict__ target_logit,
                  const int* __restrict__ rows, float* __restrict__ losses, float* __restrict__ lse, float* partial, float* __restrict__ total,
                  const int mean, const int* status) {
-    __shared__ float sm[8][32], ss[8][32];
+    constexpr int WAYS = 256 / ROWS;
+    __shared__ MaxSum part[WAYS][ROWS];
     __shared__ int is_last;
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const int row = blockIdx.x * 32 + x;
+    const int x = threadIdx.x % ROWS, y = threadIdx.x / ROWS;
+    const int row = blockIdx.x * ROWS + x;
+    cudaGridDependencySynchronize();
     const int count = sc->count;
-    float m = -INFINITY, s = 0.0f;
+    MaxSum a = {-INFINITY, 0.0f};
     if (row < count) {
-        for (int t = y; t < tiles; t += 8) {
+        for (int t = y; t < tiles; t += WAYS) {
             const float2 p = __ldcs(stats + (long long)t * rows_cap + row);
-            const float next = fmaxf(m, p.x);
-            const float ref = next == -INFINITY ? 0.0f : next * kLog2e;
-            s = fmaf(s, exp2f(fmaf(m, kLog2e, -ref)), p.y * exp2f(fmaf(p.x, kLog2e, -ref)));
-            m = next;
+            a = joined(a, {p.x, p.y});
         }
     }
-    sm[y][x] = m;
-    ss[y][x] = s;
-    __syncthreads();
-    if (y == 0) {
-        for (int k = 1; k < 8; ++k) {
-            const float next = fmaxf(m, sm[k][x]);
-            const float ref = next == -INFINITY ? 0.0f : next * kLog2e;
-            s = fmaf(s, exp2f(fmaf(m, kLog2e, -ref)), ss[k][x] * exp2f(fmaf(sm[k][x], kLog2e, -ref)));
-            m = next;
-        }
+    part[y][x] = a;
+    for (int o = WAYS / 2; o > 0; o >>= 1) {
+        __syncthreads();
+        if (y < o) part[y][x] = joined(part[y][x], part[y + o][x]);
+    }
+    if (threadIdx.x < 32) {
         float loss = 0.0f;
-        if (row < count) {
+        if (y == 0 && row < count) {
+            a = part[0][x];
             const float z = target_logit[row];
-            loss = z >= m ? log1pf(s * expf(m - z)) : (m - z) + logf(s + expf(z - m));
+            loss = z >= a.m ? log1pf(a.s * expf(a.m - z)) : (a.m - z) + logf(a.s + expf(z - a.m));
             losses[rows[row]] = loss;
             lse[rows[row]] = z + loss;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
-        if (x == 0) {
+        if (threadIdx.x == 0) {
             partial[blockIdx.x] = loss;
             __threadfence();
             is_last = atomicAdd(&sc->ticket, 1u) == gridDim.x - 1;
         }
     }
     __syncthreads();
-    if (!is_last || y != 0) return;
+    if (!is_last || threadIdx.x >= 32) return;
     __threadfence();
     double sum = 0.0;
-    for (int b = x; b < (int)gridDim.x; b += 32) sum += (double)((volatile float*)partial)[b];
+    for (int b = threadIdx.x; b < (int)gridDim.x; b += 32) sum += (double)((volatile float*)partial)[b];
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (x == 0) {
+    if (threadIdx.x == 0) {
         if (*status) sum = NAN;                                   // a wait of the product ran out: say so in the result
         total[0] = (float)(mean && count > 0 ? sum / count : sum);
         total[1] = (float)count;
@@ -472,9 +650,10 @@ static int make_map(CUtensorMap* map, int dtype, uintptr_t base, int64_t rows, i
 }
 
 // Launches one product with as many CTA pairs as fit at once, at most one per tile.
-template <bool MN_A, bool MN_B, typename Ops>
-static int launch_tiles(Device* d, const CUtensorMap& a, const CUtensorMap& b, const Ops& ops, int64_t max_tiles) {
-    auto kernel = tile_gemm_kernel<MN_A, MN_B, Ops>;
+template <int TN, bool MN_A, bool MN_B, typename Ops>
+static int launch_tiles(Device* d, const CUtensorMap& a, const CUtensorMap& b, const Ops& ops, int64_t max_tiles, int* launched = nullptr) {
+    auto kernel = tile_gemm_kernel<TN, MN_A, MN_B, Ops>;
+    constexpr int kGemmSmem = Ring<TN>::kSmem;
     static std::mutex mu;
     static int pairs_of[64] = {0};                   // per device ordinal
     int pairs;
@@ -500,21 +679,34 @@ static int launch_tiles(Device* d, const CUtensorMap& a, const CUtensorMap& b, c
         pairs = known;
     }
     if (max_tiles < pairs) pairs = (int)max_tiles;
-    kernel<<<(unsigned)pairs * 2, kGemmThreads, kGemmSmem, d->stream>>>(a, b, ops, reinterpret_cast<int*>(d->scalars + kXentStatusWord), d->barrier_budget_cycles);
+    if (launched) *launched = pairs;
+    GM_CUDA_CHECK(launch_chained(kernel, dim3((unsigned)pairs * 2), dim3(kGemmThreads), kGemmSmem, d->stream, a, b, ops,
+                                 reinterpret_cast<int*>(d->scalars + kXentStatusWord), d->barrier_budget_cycles));
     d->launches++;
-    GM_CUDA_CHECK(cudaGetLastError());
     return GM_OK;
 }
 
-static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+static int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }   // workspace parts, and rows up to a whole tile
 
 constexpr int64_t kPieceTarget = 512LL << 20;        // bytes of S the recommended workspace holds
+constexpr int kFewRows = 128;                        // rows up to which the vocabulary takes the tiles' long side
+constexpr int kMostItems = 296;                      // shares of dX's tiles that may be waiting to be added up, 256 KB each
+
+static int64_t split_items(const gm_linear_xent_t* h) {
+    const int64_t all = up256(h->tokens) / kTileM * ((h->dim + kTileN - 1) / kTileN) * 16;
+    return all < kMostItems ? all : kMostItems;
+}
+// m-tiles of the logits' products walked together: as many rows of X as take 32 MB, a quarter of L2
+static int logits_group(const gm_linear_xent_t* h) {
+    const int64_t g = (32LL << 20) / (kTileM * 2 * h->dim);
+    return (int)(g < 8 ? 8 : g > 64 ? 64 : g);
+}
 
 struct XentSpace {
     int64_t cap, ld_packed;                          // rows up to a whole tile, stride of the gathered hidden states
     int64_t scalars, rows, target, packed;           // both passes
     int64_t stats, target_logit, partial;            // forward
-    int64_t carried, ld_carried, ds, width;          // backward
+    int64_t parts, carried, ld_carried, ds, width;   // backward
     int64_t total;
 };
 
@@ -532,9 +724,10 @@ static XentSpace common_space(const gm_linear_xent_t* h) {
 static XentSpace forward_space(const gm_linear_xent_t* h) {
     XentSpace s = common_space(h);
     s.stats = s.total;
-    s.target_logit = s.stats + up256((h->vocab + kTileN - 1) / kTileN * s.cap * 8);
+    const int64_t stat_tiles = h->tokens <= kFewRows ? (h->vocab + 31) / 32 : (h->vocab + kTileN - 1) / kTileN;
+    s.target_logit = s.stats + up256(stat_tiles * s.cap * 8);
     s.partial = s.target_logit + up256(s.cap * 4);
-    s.total = s.partial + up256(s.cap / 32 * 4);
+    s.total = s.partial + up256(s.cap * 4);
     return s;
 }
 
@@ -542,6 +735,8 @@ static XentSpace forward_space(const gm_linear_xent_t* h) {
 static XentSpace backward_space(const gm_linear_xent_t* h, int64_t bytes) {
     XentSpace s = common_space(h);
     const int64_t all = up256(h->vocab);
+    s.parts = s.total;
+    s.total = s.parts + split_items(h) * kTileM * kTileN * 4;
     s.ld_carried = s.ld_packed;
     if (s.total + up256(s.cap * all * 2) <= bytes) {              // one piece: nothing is carried
         s.width = all;
@@ -563,8 +758,9 @@ static XentSpace backward_space(const gm_linear_xent_t* h, int64_t bytes) {
 }
 
 static int64_t backward_bytes(const gm_linear_xent_t* h, bool smallest) {
-    const XentSpace s = common_space(h);
+    XentSpace s = common_space(h);
     const int64_t all = up256(h->vocab);
+    s.total += split_items(h) * kTileM * kTileN * 4;
     int64_t width = smallest ? 256 : kPieceTarget / (s.cap * 2) / 256 * 256;
     if (width < 256) width = 256;
     const int64_t whole = s.total + up256(s.cap * all * 2);       // one piece: nothing is carried
@@ -600,36 +796,58 @@ template <typename T>
 static int index_and_gather(const XentCall& c, uintptr_t hidden, uintptr_t targets, uintptr_t weight, float* target_logit, float* losses, float* lse,
                             T* dhidden) {
     const gm_linear_xent_t* h = c.h;
-    xent_index_kernel<<<1, kIndexThreads, 0, c.d->stream>>>((const int*)targets, (int)h->tokens, (int)h->vocab, c.rows(), c.target(), c.sc());
-    c.d->launches++;
-    GM_CUDA_CHECK(cudaGetLastError());
+    const bool few = h->tokens <= kFewIndex;
+    if (!few) {
+        GM_CUDA_CHECK(launch_chained(xent_index_kernel, dim3(1), dim3(kIndexThreads), 0, c.d->stream, (const int*)targets, (int)h->tokens,
+                                     (int)h->vocab, c.rows(), c.target(), c.sc()));
+        c.d->launches++;
+    }
     const bool vec = hidden % 16 == 0 && h->ld_hidden % 8 == 0;
     const bool vec_out = (uintptr_t)dhidden % 16 == 0 && h->ld_hidden % 8 == 0;
-    xent_gather_kernel<T><<<(unsigned)c.s.cap, kGatherThreads, 0, c.d->stream>>>(
-        (const T*)hidden, h->ld_hidden, (int)h->tokens, (int)h->dim, (int)h->vocab, (const int*)targets, c.rows(), c.target(), c.sc(),
-        (T*)(c.ws + c.s.packed), c.s.ld_packed, (const T*)weight, h->ld_weight, target_logit, losses, lse, dhidden, vec, vec_out);
+    GM_CUDA_CHECK(launch_chained(xent_gather_kernel<T>, dim3((unsigned)c.s.cap), dim3(kGatherThreads), 0, c.d->stream, (const T*)hidden, h->ld_hidden,
+                                 (int)h->tokens, (int)h->dim, (int)h->vocab, (const int*)targets, c.rows(), c.target(), c.sc(), few,
+                                 (T*)(c.ws + c.s.packed), c.s.ld_packed, (const T*)weight, h->ld_weight, target_logit, losses, lse, dhidden, vec, vec_out));
     c.d->launches++;
-    GM_CUDA_CHECK(cudaGetLastError());
     return GM_OK;
+}
+
+// The logits of a few rows, 256 vocabulary entries by TN rows to a tile.
+template <typename T, int TN>
+static int few_logits(const XentCall& c, const CUtensorMap& map_w, float2* stats) {
+    const gm_linear_xent_t* h = c.h;
+    CUtensorMap map_x;
+    GM_TRY(make_map(&map_x, h->dtype, c.ws + c.s.packed, c.s.cap, h->dim, c.s.ld_packed, TN / 2));
+    const FewStatsOps<T, TN> ops{c.sc(), c.target(), stats, (int)c.s.cap, (int)h->dim, (int)h->vocab, 0, 0};
+    return launch_tiles<TN, false, false>(c.d, map_w, map_x, ops, (h->vocab + kTileM - 1) / kTileM);
 }
 
 template <typename T>
 static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, uintptr_t targets, float* losses, float* lse, float* total) {
     const gm_linear_xent_t* h = c.h;
     const XentSpace& s = c.s;
-    CUtensorMap map_x, map_w;
-    GM_TRY(make_map(&map_x, h->dtype, c.ws + s.packed, s.cap, h->dim, s.ld_packed, kHalf));
+    CUtensorMap map_w;
     GM_TRY(make_map(&map_w, h->dtype, weight, h->vocab, h->dim, h->ld_weight, kHalf));
     float* target_logit = (float*)(c.ws + s.target_logit);
     GM_TRY(index_and_gather<T>(c, hidden, targets, weight, target_logit, losses, lse, (T*)nullptr));
-    const int tiles = (int)((h->vocab + kTileN - 1) / kTileN);
     float2* stats = (float2*)(c.ws + s.stats);
-    const StatsOps<T> ops{c.sc(), c.target(), stats, (int)s.cap, (int)h->dim, (int)h->vocab, 0, 0};
-    GM_TRY((launch_tiles<false, false>(c.d, map_x, map_w, ops, s.cap / kTileM * tiles)));
-    xent_join_kernel<<<(unsigned)(s.cap / 32), 256, 0, c.d->stream>>>(c.sc(), stats, (int)s.cap, tiles, target_logit, c.rows(), losses, lse,
-                                                                     (float*)(c.ws + s.partial), total, h->mean, reinterpret_cast<const int*>(c.d->scalars + kXentStatusWord));
+    const bool few = h->tokens <= kFewRows;
+    int tiles = (int)((h->vocab + kTileN - 1) / kTileN);
+    if (few) {
+        tiles = (int)((h->vocab + 31) / 32);
+        if (h->tokens <= 32) GM_TRY((few_logits<T, 32>(c, map_w, stats)));
+        else GM_TRY((few_logits<T, kFewRows>(c, map_w, stats)));
+    } else {
+        CUtensorMap map_x;
+        GM_TRY(make_map(&map_x, h->dtype, c.ws + s.packed, s.cap, h->dim, s.ld_packed, kHalf));
+        const StatsOps<T> ops{c.sc(), c.target(), stats, (int)s.cap, (int)h->dim, (int)h->vocab, logits_group(h), 0, 0};
+        GM_TRY((launch_tiles<kTileN, false, false>(c.d, map_x, map_w, ops, s.cap / kTileM * tiles)));
+    }
+    // a CTA per row up to a few rows per SM, 32 rows per CTA beyond
+    auto join = h->tokens <= 1024 ? xent_join_kernel<1> : xent_join_kernel<32>;
+    const int64_t ctas = h->tokens <= 1024 ? h->tokens : s.cap / 32;
+    GM_CUDA_CHECK(launch_chained(join, dim3((unsigned)ctas), dim3(256), 0, c.d->stream, c.sc(), stats, (int)s.cap, tiles, target_logit, c.rows(), losses, lse,
+                                 (float*)(c.ws + s.partial), total, h->mean, reinterpret_cast<const int*>(c.d->scalars + kXentStatusWord)));
     c.d->launches++;
-    GM_CUDA_CHECK(cudaGetLastError());
     return GM_OK;
 }
 
@@ -653,18 +871,24 @@ static int run_backward(const XentCall& c, uintptr_t hidden, uintptr_t weight, u
     for (int64_t v = 0; v < vocab; v += s.width) {
         const int v0 = (int)v, v1 = (int)(v + s.width < vocab ? v + s.width : vocab);
         const int64_t v_tiles = (v1 - v0 + kTileN - 1) / kTileN;
-        const SoftmaxGradOps<T> grad{c.sc(), c.target(), c.rows(), lse, (T*)ds, s.width, dim, v0, v1, 0, v0};
-        GM_TRY((launch_tiles<false, false>(c.d, x_k, w_k, grad, m_tiles * v_tiles)));
+        const SoftmaxGradOps<T> grad{c.sc(), c.target(), c.rows(), lse, (T*)ds, s.width, dim, v0, v1, logits_group(h), 0, v0};
+        GM_TRY((launch_tiles<kTileN, false, false>(c.d, x_k, w_k, grad, m_tiles * v_tiles)));
         if (dhidden) {
             const bool vec = dhidden % 16 == 0 && h->ld_hidden % 8 == 0;
-            const HiddenGradOps<T> ops{c.sc(), c.rows(), (float*)(c.ws + s.carried), s.ld_carried, (T*)dhidden, h->ld_hidden, scale,
-                                       dim, v0, v1, 0, v0, v0 == 0, v1 == vocab, vec};
-            GM_TRY((launch_tiles<false, true>(c.d, ds_k, w_mn, ops, m_tiles * d_tiles)));
+            const HiddenPlan shape{dim, v0, v1, (int)split_items(h)};
+            const HiddenOut<T> out{(float*)(c.ws + s.carried), s.ld_carried, (T*)dhidden, h->ld_hidden, scale, v0 == 0, v1 == vocab, vec};
+            float* parts = (float*)(c.ws + s.parts);
+            int pairs = 0;
+            GM_TRY((launch_tiles<kTileN, false, true>(c.d, ds_k, w_mn, HiddenGradOps<T>{c.sc(), c.rows(), parts, shape, out, 0, v0}, m_tiles * d_tiles * 16, &pairs)));
+            // the number of shares follows from the rows with a target, which only the device knows
+            GM_CUDA_CHECK(launch_chained(xent_hidden_join_kernel<T>, dim3((unsigned)c.d->sm_count * 4), dim3(256), 0, c.d->stream, c.sc(), c.rows(), parts, shape,
+                                         out, pairs));
+            c.d->launches++;
         }
         if (dweight) {
             const bool vec = dweight % 16 == 0;
             const WeightGradOps<T> ops{c.sc(), (T*)dweight, h->ld_weight, scale, dim, v0, v1, 0, 0, accumulate, vec};
-            GM_TRY((launch_tiles<true, true>(c.d, ds_mn, x_mn, ops, v_tiles * d_tiles)));
+            GM_TRY((launch_tiles<kTileN, true, true>(c.d, ds_mn, x_mn, ops, v_tiles * d_tiles)));
         }
     }
     return GM_OK;

@@ -179,6 +179,23 @@ int check_matrix(int64_t rows, int64_t cols, int64_t ld, const char* what);
 // Bytes from a matrix's first element to behind its last one.
 inline int64_t matrix_bytes(int64_t rows, int64_t cols, int64_t ld, int eb) { return rows > 0 ? ((rows - 1) * ld + cols) * eb : 0; }
 
+// A launch that may begin while the kernel before it in the stream ends (programmatic stream
+// serialization); the kernel calls cudaGridDependencySynchronize() before it touches memory.
+template <typename... P, typename... A>
+inline cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 #define GM_TRY(expr)                      \
     do {                                  \
         const int rc__ = (expr);          \

@@ -1,14 +1,17 @@
 // gm_tile_gemm.cuh -- the matrix products of the vocabulary loss on the fifth-generation
-// tensor cores: a persistent kernel of CTA pairs, C[256 x 256] per pair and tile.
+// tensor cores: a persistent kernel of CTA pairs, C[256 x N] per pair and tile.
 //
 //   warp 0    one lane copies operand tiles into a ring of shared-memory stages (TMA)
 //   warp 1    one lane of the pair's first CTA issues tcgen05.mma (M = 256 over both SMs,
-//             N = 256, K = 16, fp16 or bf16 in, binary32 accumulators in TMEM)
+//             N = 256 or less, K = 16, fp16 or bf16 in, binary32 accumulators in TMEM)
 //   warps 2-5 read the accumulators (each thread one row) and run the epilogue
 //
-// The accumulators take 256 TMEM columns and there are two sets of them, so the epilogue of
+// The accumulators take N TMEM columns and there are two sets of them, so the epilogue of
 // one tile runs while the next one is multiplied.  Of the pair, each CTA holds 128 rows of A
-// and 128 of the 256 rows of B: a stage is 32 KB per CTA and six of them fit.
+// and half of the N rows of B: with N = 256 a stage is 32 KB per CTA and six of them fit.
+//
+// Where a product has too few tiles for the GPU, a tile's K range is split over several pairs,
+// and a kernel of its own adds up what they leave (TilePlan::splits).
 //
 // Operands are read as they lie in memory, K-major or MN-major, always with the 128-byte
 // swizzle: a K-major tile is rows of 64 elements (128 bytes), eight rows to a 1,024-byte
@@ -25,12 +28,16 @@
 namespace gm {
 
 constexpr int kTileM = 256, kTileN = 256, kTileK = 64;
-constexpr int kHalf = 128;                       // rows of A and of B that one CTA of the pair holds
-constexpr int kStages = 6;
+constexpr int kHalf = 128;                       // rows of A that one CTA of the pair holds
 constexpr int kOperandBytes = kHalf * kTileK * 2;
-constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kGemmThreads = 192;
-constexpr int kGemmSmem = kStages * kStageBytes + 1024;
+template <int TN> struct Ring {                  // the ring of stages for tiles of TN columns
+    static constexpr int kRowsB = TN / 2;
+    static constexpr int kStageBytes = kOperandBytes + kRowsB * kTileK * 2;
+    static constexpr int kFit = 200 * 1024 / kStageBytes;
+    static constexpr int kStages = kFit < 12 ? kFit : 12;
+    static constexpr int kSmem = kStages * kStageBytes + 1024;
+};
 
 // ---- mbarriers ----
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -117,31 +124,60 @@ __device__ __forceinline__ void tmem_load32(unsigned addr, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// One product.  All tiles: m_tiles x n_tiles, walked m first inside groups of `group` m-tiles,
-// so that the operands of the tiles in flight are shared in L2.
+// Where the work of one turn lies: tile, its share of K, and the turn's number.
+struct TileAt { int m, n, split, item, k0, k1; };
+
+// One product: m_tiles x n_tiles tiles, walked m first inside groups of `group` m-tiles, so that
+// the operands of the tiles in flight are shared in L2; each in `splits` shares of K.
 struct TilePlan {
-    int m_tiles, n_tiles, k_blocks, group;
-    __device__ __forceinline__ void at(int t, int* m, int* n) const {
-        const int per = group * n_tiles;
+    int m_tiles, n_tiles, k_blocks, group, splits;
+    __device__ __forceinline__ int items() const { return m_tiles * n_tiles * splits; }
+    __device__ __forceinline__ TileAt at(int item) const {
+        TileAt x;
+        const int t = item / splits, per = group * n_tiles;
         const int g = t / per, m0 = g * group;
         const int rows = m_tiles - m0 < group ? m_tiles - m0 : group;
         const int r = t - g * per;
-        *n = r / rows;
-        *m = m0 + (r - *n * rows);
+        x.item = item;
+        x.n = r / rows;
+        x.m = m0 + (r - x.n * rows);
+        x.split = item - t * splits;
+        x.k0 = (int)((long long)k_blocks * x.split / splits);
+        x.k1 = (int)((long long)k_blocks * (x.split + 1) / splits);
+        return x;
+    }
+    // the inverse: number of the tile at (m, n)
+    __device__ __forceinline__ int tile_of(int m, int n) const {
+        const int m0 = m / group * group;
+        const int rows = m_tiles - m0 < group ? m_tiles - m0 : group;
+        return m0 * n_tiles + n * rows + (m - m0);
     }
 };
 
+// Shares of K per tile, at most 16 and `most_items` in all, for the shortest run on `pairs` CTA
+// pairs: rounds of items, each as long as its k-blocks plus a start and an epilogue (about eight).
+__device__ __forceinline__ int choose_splits(int tiles, int k_blocks, int pairs, int most_items) {
+    int best = 1, best_cost = 0x7fffffff;
+    for (int s = 1; s <= 16 && s <= k_blocks && (s == 1 || tiles * s <= most_items); ++s) {
+        const int cost = (tiles * s + pairs - 1) / pairs * ((k_blocks + s - 1) / s + 8) + (s > 1 ? 8 : 0);
+        if (cost < best_cost) { best_cost = cost; best = s; }
+    }
+    return best;
+}
+
 // MN_A / MN_B: that operand is MN-major.  Ops provides
 //   kBf16             whether the inputs are bf16 (else fp16)
-//   plan()            the tiles, read on the device
+//   plan(pairs)       the tiles, read on the device
 //   a0, b0            first row of A and of B (first K-row of an MN-major operand) in their maps
-//   epilogue(row, n, addr, empty)   row of C, tile column, TMEM address of the row's first
-//                     column, and whether there was nothing to multiply (C is zero); called by
-//                     whole warps, also for rows behind the last one
-template <bool MN_A, bool MN_B, typename Ops>
+//   epilogue(at, row, addr)   the turn, the row inside the tile, the TMEM address of its first
+//                     column; called by whole warps, also for rows behind the last one; with an
+//                     empty share of K (at.k0 == at.k1) the accumulators hold nothing and C is zero
+template <int TN, bool MN_A, bool MN_B, typename Ops>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Ops ops,
                  int* status, const long long budget) {
+    constexpr int kStages = Ring<TN>::kStages, kStageBytes = Ring<TN>::kStageBytes, kRowsB = Ring<TN>::kRowsB;
+    static_assert(!MN_B || TN == 256, "an MN-major B comes in two blocks of 64 columns per CTA");
     extern __shared__ unsigned char dyn[];
     __shared__ __align__(8) unsigned long long full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
     __shared__ unsigned tmem_base;
@@ -150,8 +186,6 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const unsigned rank = cluster_rank();
     const unsigned ring = (smem_u32(dyn) + 1023u) & ~1023u;
-    const TilePlan plan = ops.plan();
-    const int tiles = plan.m_tiles * plan.n_tiles;
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (tid == 0) {
@@ -170,16 +204,19 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     cluster_sync_all();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = tmem_base;
+    // all of the above may run while the kernel before this one ends
+    cudaGridDependencySynchronize();
+    const TilePlan plan = ops.plan(pairs);
+    const int items = plan.items();
 
     unsigned issued = 0;                                         // k-blocks this thread copied; stage and parity follow from it
     if (warp == 0 && lane == 0) {
         // ---- copies ----
         bool ok = true;
-        for (int t = pair; t < tiles && ok; t += pairs) {
-            int m, n;
-            plan.at(t, &m, &n);
-            const int row_a = m * kTileM + (int)rank * kHalf, row_b = n * kTileN + (int)rank * kHalf;
-            for (int k = 0; k < plan.k_blocks; ++k, ++issued) {
+        for (int t = pair; t < items && ok; t += pairs) {
+            const TileAt at = plan.at(t);
+            const int row_a = at.m * kTileM + (int)rank * kHalf, row_b = at.n * TN + (int)rank * kRowsB;
+            for (int k = at.k0; k < at.k1; ++k, ++issued) {
                 const int s = issued % kStages;
                 const unsigned turn = issued / kStages;
                 if (!mbar_wait(smem_u32(&empty[s]), (turn & 1u) ^ 1u, &abort_flag, budget)) { ok = false; break; }
@@ -205,16 +242,17 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         // accumulators binary32, inputs fp16 or bf16, N / 8 in bits 17-22, M / 16 in bits 24-28
         const unsigned in = Ops::kBf16 ? 1u : 0u;
         const unsigned idesc = (1u << 4) | (in << 7) | (in << 10) | ((MN_A ? 1u : 0u) << 15) | ((MN_B ? 1u : 0u) << 16) |
-                               ((unsigned)(kTileN / 8) << 17) | ((unsigned)(kTileM / 16) << 24);
+                               ((unsigned)(TN / 8) << 17) | ((unsigned)(kTileM / 16) << 24);
         unsigned used = 0;
         int count = 0;
         bool ok = true;
-        for (int t = pair; t < tiles && ok; t += pairs, ++count) {
+        for (int t = pair; t < items && ok; t += pairs, ++count) {
+            const TileAt at = plan.at(t);
             const int b = count & 1;
             if (!mbar_wait(smem_u32(&acc_empty[b]), ((count >> 1) & 1) ^ 1, &abort_flag, budget)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const unsigned d = tmem + (unsigned)b * kTileN;
-            for (int k = 0; k < plan.k_blocks; ++k, ++used) {
+            const unsigned d = tmem + (unsigned)b * TN;
+            for (int k = at.k0; k < at.k1; ++k, ++used) {
                 const int s = used % kStages;
                 if (!mbar_wait(smem_u32(&full[s]), (used / kStages) & 1u, &abort_flag, budget)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -222,7 +260,7 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 const unsigned long long da = mat_desc(a, MN_A), db = mat_desc(a + kOperandBytes, MN_B);
 #pragma unroll
                 for (int i = 0; i < kTileK / 16; ++i)
-                    mma_pair(d, da + (MN_A ? 128 * i : 2 * i), db + (MN_B ? 128 * i : 2 * i), idesc, k > 0 || i > 0);
+                    mma_pair(d, da + (MN_A ? 128 * i : 2 * i), db + (MN_B ? 128 * i : 2 * i), idesc, k > at.k0 || i > 0);
                 mma_commit_pair(smem_u32(&empty[s]));
             }
             if (ok) mma_commit_pair(smem_u32(&acc_full[b]));
@@ -237,14 +275,13 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const int quarter = warp & 3;                            // the TMEM lanes this warp may read
         const int row = quarter * 32 + lane;
         int count = 0;
-        for (int t = pair; t < tiles; t += pairs, ++count) {
-            int m, n;
-            plan.at(t, &m, &n);
+        for (int t = pair; t < items; t += pairs, ++count) {
+            const TileAt at = plan.at(t);
             const int b = count & 1;
             const bool ok = mbar_wait(smem_u32(&acc_full[b]), (count >> 1) & 1, &abort_flag, budget);
             if (!__all_sync(0xffffffffu, ok)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            ops.epilogue(m * kTileM + (int)rank * kHalf + row, n, tmem + (unsigned)b * kTileN + ((unsigned)(quarter * 32) << 16), plan.k_blocks == 0);
+            ops.epilogue(at, (int)rank * kHalf + row, tmem + (unsigned)b * TN + ((unsigned)(quarter * 32) << 16));
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(pair_leader_addr(smem_u32(&acc_empty[b])));
