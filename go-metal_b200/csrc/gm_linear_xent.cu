@@ -4,8 +4,8 @@
 //   l = X W^T,  lse_n = log sum_v exp l_nv,  loss_n = lse_n - l_{n, t_n}
 //   S = softmax(l) - onehot(t),  dX = c S W,  dW = c S^T X,  c = grad_scale * scale / count
 //
-// Forward: one matrix product whose epilogue leaves, per row and tile of 256 vocabulary
-// entries, the maximum and the sum of exponentials (8 bytes for 256 logits) of all entries but
+// Forward: one matrix product whose epilogue leaves, per row and 128 vocabulary entries, the
+// maximum and the sum of exponentials (8 bytes for 128 logits) of all entries but
 // the target's, then a small kernel joins them with the target's logit, which comes from a dot
 // product of its own.  loss = log(1 + sum of the others / the target's) then loses nothing when the
 // model is sure of the target, and the target's logit is as good as binary32 makes it (the
@@ -21,7 +21,8 @@
 //
 // Roundings: S is rounded once to the inputs' type, as the operand of a tensor-core product
 // has to be.  In fp16 it is first multiplied by 2^15 (|S| <= 1), which keeps probabilities
-// down to 2^-29 normal; the factor is taken out in binary32 in the epilogue.
+// down to 2^-29 normal, in bf16 by 2^32, so that the exponential's flush to zero at 2^-126 lies
+// below what bf16 holds; the factor is taken out in binary32 in the epilogue.
 #include <mutex>
 
 #include "gm_tile_gemm.cuh"
@@ -32,8 +33,8 @@ constexpr int kXentStatusWord = 48;      // of the device's scalars: 1 when a wa
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T> struct Half16;
-template <> struct Half16<__half> { static constexpr bool kBf16 = false; static constexpr float kUp = 32768.0f; };
-template <> struct Half16<__nv_bfloat16> { static constexpr bool kBf16 = true; static constexpr float kUp = 1.0f; };
+template <> struct Half16<__half> { static constexpr bool kBf16 = false; static constexpr float kUp = 32768.0f, kUpLog2 = 15.0f; };
+template <> struct Half16<__nv_bfloat16> { static constexpr bool kBf16 = true; static constexpr float kUp = 4294967296.0f, kUpLog2 = 32.0f; };
 
 // Scalars at the workspace's begin.
 struct XentScalars {
@@ -42,6 +43,13 @@ struct XentScalars {
 };
 
 __device__ __forceinline__ int up_to(int x, int m) { return (x + m - 1) / m * m; }
+
+// 2^x, results below 2^-126 as zero (PTX ex2.approx.ftz: two units in the last place).
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // ---------------------------------------------------------------- index and gather
 // rows[i] = the i-th row with a target, target[i] = that target.  One CTA: eight rows per
@@ -54,6 +62,7 @@ xent_index_kernel(const int* __restrict__ targets, const int n, const int vocab,
     __shared__ int carry;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
     if (tid == 0) carry = 0;
     __syncthreads();
     for (long long base = 0; base < n; base += kIndexThreads * 8) {
@@ -152,6 +161,7 @@ xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n
     __shared__ float warp_sum[kGatherThreads / 32];
     const int r = blockIdx.x, tid = threadIdx.x;
     cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
     int count, row, goal;
     if (few) {
         find_row(targets, n, vocab, r, &count, &row, &goal);
@@ -221,53 +231,51 @@ xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n
 // ---------------------------------------------------------------- epilogues
 constexpr int kGroupM = 8;      // m-tiles walked together in the gradient products
 
-// Row maximum and sum of exponentials of one tile of logits, the target's left out.
+// Row maximum and sum of exponentials of half a tile's logits (128), the target's left out.
+struct Goal { int at; };        // a row's target
 template <typename T>
 struct StatsOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
+    static constexpr bool kStaging = false;
     const XentScalars* sc;
     const int* target;
-    float2* stats;               // [vocabulary tile][row]
+    float2* stats;               // [128 vocabulary entries][row]
     int rows_cap, dim, vocab, group, a0, b0;
     __device__ __forceinline__ TilePlan plan(int) const {
-        return {(sc->count + kTileM - 1) / kTileM, (vocab + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, group, 1};
+        const int count = sc->count;
+        return {count, (count + kTileM - 1) / kTileM, (vocab + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, group, 1};
     }
-    __device__ __forceinline__ void epilogue(const TileAt& tile, int in_tile, unsigned addr) const {
-        const int row = tile.m * kTileM + in_tile, n = tile.n;
-        const bool live = row < sc->count;
-        const int c0 = n * kTileN;
-        const int width = vocab - c0 < kTileN ? vocab - c0 : kTileN;
-        const int at = live ? __ldg(target + row) - c0 : -1;
-        float m = -INFINITY, s = 0.0f;
-#pragma unroll 1
-        for (int c = 0; c < width; c += 32) {
-            float v[32];
-            tmem_load32(addr + c, v);
-            if (width - c < 32) {
+    __device__ __forceinline__ Goal prepare(const TilePlan& plan, const TileAt& tile, int in_tile) const {
+        const int row = tile.m * kTileM + in_tile;
+        return {row < plan.count ? __ldg(target + row) - tile.n * kTileN : -1};
+    }
+    __device__ __forceinline__ void epilogue(const TilePlan& plan, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned,
+                                             const Goal goal) const {
+        const int row = tile.m * kTileM + in_tile;
+        const int width = vocab - tile.n * kTileN - half * 128;           // columns that exist
+        if (width <= 0) return;
+        if (width < 128) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (c + j >= width) v[j] = -INFINITY;
-            }
-            if ((unsigned)(at - c) < 32u) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (at - c == j) v[j] = -INFINITY;
-            }
-            float top = v[0];
-#pragma unroll
-            for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
-            const float next = fmaxf(m, top);
-            const float ref = next == -INFINITY ? 0.0f : next * kLog2e;       // nothing but -inf so far: exponentials are zero
-            float a0_ = 0.0f, a1_ = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-                a0_ += exp2f(fmaf(v[j], kLog2e, -ref));
-                a1_ += exp2f(fmaf(v[j + 1], kLog2e, -ref));
-            }
-            s = fmaf(s, exp2f(fmaf(m, kLog2e, -ref)), a0_ + a1_);
-            m = next;
+            for (int j = 0; j < 128; ++j)
+                if (j >= width) v[j] = -INFINITY;
         }
-        if (live) stats[(long long)n * rows_cap + row] = make_float2(m, s);
+        const int at = goal.at - half * 128;
+        if ((unsigned)at < 128u) {
+#pragma unroll
+            for (int j = 0; j < 128; ++j)
+                if (at == j) v[j] = -INFINITY;
+        }
+        float top[8], sum[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { top[j] = v[j]; sum[j] = 0.0f; }
+#pragma unroll
+        for (int j = 8; j < 128; ++j) top[j & 7] = fmaxf(top[j & 7], v[j]);
+        const float m = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
+        const float ref = m == -INFINITY ? 0.0f : m * kLog2e;              // nothing but -inf: exponentials are zero
+#pragma unroll
+        for (int j = 0; j < 128; ++j) sum[j & 7] += exp2_fast(fmaf(v[j], kLog2e, -ref));
+        const float s = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
+        if (row < plan.count) stats[(long long)(2 * tile.n + half) * rows_cap + row] = make_float2(m, s);
     }
 };
 
@@ -292,25 +300,29 @@ template <bool MAX> __device__ __forceinline__ float lanes_to_columns(float (&v)
 template <typename T, int TN>
 struct FewStatsOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
+    static constexpr bool kStaging = false;
     const XentScalars* sc;
     const int* target;
     float2* stats;               // [32 vocabulary entries][row]
     int rows_cap, dim, vocab, a0, b0;
     __device__ __forceinline__ TilePlan plan(int) const {
-        return {(vocab + kTileM - 1) / kTileM, sc->count > 0 ? 1 : 0, (dim + kTileK - 1) / kTileK, 1, 1};
-    }
-    __device__ __forceinline__ void epilogue(const TileAt& tile, int in_tile, unsigned addr) const {
-        const int entry = tile.m * kTileM + in_tile, lane = threadIdx.x & 31;
         const int count = sc->count;
-        if (entry - lane >= vocab) return;                             // the whole warp is behind the table
-#pragma unroll 1
-        for (int c = 0; c < count; c += 32) {
-            float v[32], w[32];
-            tmem_load32(addr + c, v);
-            if (entry >= vocab) {
+        return {count, (vocab + kTileM - 1) / kTileM, count > 0 ? 1 : 0, (dim + kTileK - 1) / kTileK, 1, 1};
+    }
+    __device__ __forceinline__ Goal prepare(const TilePlan&, const TileAt&, int) const { return {0}; }
+    static constexpr int kColumns = TN / 2 < 32 ? 32 : TN / 2;
+    __device__ __forceinline__ void epilogue(const TilePlan& plan, const TileAt& tile, int in_tile, float (&all)[kColumns], int half, unsigned,
+                                             const Goal) const {
+        const int entry = tile.m * kTileM + in_tile, lane = threadIdx.x & 31;
+        const int count = plan.count;
+        if (entry - lane >= vocab || half * kColumns >= TN) return;     // the whole warp is behind the table, or has no columns
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = -INFINITY;
-            }
+        for (int q = 0; q < kColumns; q += 32) {
+            const int c = half * kColumns + q;
+            if (c >= count) break;
+            float v[32], w[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = entry < vocab ? all[q + j] : -INFINITY;
             const int goal = c + lane < count ? __ldg(target + c + lane) : -1;
             for (unsigned hits = __ballot_sync(0xffffffffu, goal >= entry - lane && goal < entry - lane + 32); hits; hits &= hits - 1) {
                 const int j = __ffs((int)hits) - 1;
@@ -324,7 +336,7 @@ struct FewStatsOps {
             const float top = lanes_to_columns<true>(w, lane);
             const float ref = top == -INFINITY ? 0.0f : top * kLog2e;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = exp2f(fmaf(v[j], kLog2e, -__shfl_sync(0xffffffffu, ref, j)));
+            for (int j = 0; j < 32; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -__shfl_sync(0xffffffffu, ref, j)));
             const float sum = lanes_to_columns<false>(v, lane);
             if (c + lane < count) stats[(long long)(entry >> 5) * rows_cap + c + lane] = make_float2(top, sum);
         }
@@ -335,6 +347,7 @@ struct FewStatsOps {
 template <typename T>
 struct SoftmaxGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
+    static constexpr bool kStaging = true;
     const XentScalars* sc;
     const int* target;
     const int* rows;
@@ -342,36 +355,34 @@ struct SoftmaxGradOps {
     T* ds;
     long long ld_ds;
     int dim, v0, v1, group, a0, b0;
+    struct Row { int at; float ref; };       // target in the tile; log2 of what the row's exponentials are divided by
     __device__ __forceinline__ TilePlan plan(int) const {
-        return {(sc->count + kTileM - 1) / kTileM, (v1 - v0 + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, group, 1};
+        const int count = sc->count;
+        return {count, (count + kTileM - 1) / kTileM, (v1 - v0 + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, group, 1};
     }
-    __device__ __forceinline__ void epilogue(const TileAt& tile, int in_tile, unsigned addr) const {
-        const int row = tile.m * kTileM + in_tile, n = tile.n;
-        const bool live = row < sc->count;
-        const int c0 = v0 + n * kTileN;
-        const int width = live ? (v1 - c0 < kTileN ? v1 - c0 : kTileN) : 0;
-        const int at = live ? __ldg(target + row) - c0 : -1;
-        const float ref = live ? lse[__ldg(rows + row)] * kLog2e : 0.0f;
-        T* to = ds + (long long)row * ld_ds + n * kTileN;
-#pragma unroll 1
-        for (int c = 0; c < kTileN; c += 32) {
-            float v[32];
-            tmem_load32(addr + c, v);
+    __device__ __forceinline__ Row prepare(const TilePlan& plan, const TileAt& tile, int in_tile) const {
+        const int row = tile.m * kTileM + in_tile;
+        if (row >= plan.count) return {-1, INFINITY};             // zeros: such a row's logits are 0, 2^(0 - inf) = 0
+        return {__ldg(target + row) - v0 - tile.n * kTileN, fmaf(__ldg(lse + __ldg(rows + row)), kLog2e, -Half16<T>::kUpLog2)};
+    }
+    __device__ __forceinline__ void epilogue(const TilePlan&, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned stage,
+                                             const Row row) const {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                v[j] = exp2f(fmaf(v[j], kLog2e, -ref));
-                v[j] = c + j < width ? v[j] * Half16<T>::kUp : 0.0f;
-            }
-            if ((unsigned)(at - c) < 32u) {
+        for (int j = 0; j < 128; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -row.ref));
+        const int at = row.at - half * 128;
+        if ((unsigned)at < 128u) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (at - c == j) v[j] -= Half16<T>::kUp;
-            }
-#pragma unroll
-            for (int j = 0; j < 32; j += 8)
-                *reinterpret_cast<uint4*>(to + c + j) =
-                    make_uint4(pack2<T>(v[j], v[j + 1]), pack2<T>(v[j + 2], v[j + 3]), pack2<T>(v[j + 4], v[j + 5]), pack2<T>(v[j + 6], v[j + 7]));
+            for (int j = 0; j < 128; ++j)
+                if (at == j) v[j] -= Half16<T>::kUp;
         }
+        const int width = v1 - v0 - tile.n * kTileN - half * 128;        // columns that exist, the others are zeros
+        if (width < 128) {
+#pragma unroll
+            for (int j = 0; j < 128; ++j)
+                if (j >= width) v[j] = 0.0f;
+        }
+        T* first = ds + (long long)(tile.m * kTileM + (in_tile & ~31)) * ld_ds + tile.n * kTileN + half * 128;
+        rows_to_memory<T>(stage, v, 128, [&](int r) { return first + r * ld_ds; });
     }
 };
 
@@ -388,37 +399,39 @@ struct GradScale {
     }
 };
 
-// 32 columns of a row to memory in the output's type; cols of them exist.
+// Four columns of a row in a 16-bit type, `cols` of which exist.
 template <typename T>
-__device__ __forceinline__ void emit32(T* to, const float (&v)[32], int cols, bool vec, bool add) {
+__device__ __forceinline__ float4 get4(const T* from, int cols, bool vec) {
+    if (vec && cols >= 4) {
+        const uint2 w = *reinterpret_cast<const uint2*>(from);
+        const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-        if (vec && j + 8 <= cols) {
-            float x[8];
+    for (int j = 0; j < 4; ++j)
+        if (j < cols) v[j] = to_f32<T>(from[j]);
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+template <typename T>
+__device__ __forceinline__ void put4(T* to, const float4 x, int cols, bool vec) {
+    if (vec && cols >= 4) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
+    } else {
+        const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = v[j + k];
-            if (add) {
-                float old[8];
-                widen8<T>(load8<T, false>(to + j), old);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = __fadd_rn(old[k], x[k]);
-            }
-            store8<T>(to + j, x);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (j + k < cols) to[j + k] = from_f32<T>(add ? __fadd_rn(to_f32<T>(to[j + k]), v[j + k]) : v[j + k]);
-        }
+        for (int j = 0; j < 4; ++j)
+            if (j < cols) to[j] = from_f32<T>(v[j]);
     }
 }
 
 // dX: S [rows, piece] times W [piece, D]; carried in binary32 over the pieces, scattered to the
 // caller's rows by the last one.  With shares of K the tiles go to `parts` instead, 256 x 256
-// numbers per item, and xent_hidden_join_kernel does the rest.
+// numbers per turn, and xent_hidden_join_kernel does the rest.
 struct HiddenPlan {
     int dim, v0, v1, most_items;
     __device__ __forceinline__ TilePlan plan(int count, int pairs) const {
-        TilePlan p{(count + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (v1 - v0 + kTileK - 1) / kTileK, kGroupM, 1};
+        TilePlan p{count, (count + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (v1 - v0 + kTileK - 1) / kTileK, kGroupM, 1};
         p.splits = choose_splits(p.m_tiles * p.n_tiles, p.k_blocks, pairs, most_items);
         return p;
     }
@@ -432,33 +445,24 @@ struct HiddenOut {
     long long ld_out;
     GradScale scale;
     bool first, last, vec;
-    // 32 columns from c of one row: what was carried on top, then carried on or written
-    __device__ __forceinline__ void put(int row, int to_row, int c, float (&v)[32], int cols, float c_all) const {
+    // four columns from c of one row: what was carried, and that with more on top carried on or written
+    __device__ __forceinline__ float4 get(int row, int c) const {
+        return first ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : *reinterpret_cast<const float4*>(carried + (long long)row * ld_carried + c);
+    }
+    __device__ __forceinline__ void put(int row, int to_row, int c, float4 x, const float4 old, int cols, float c_all) const {
         float* acc = carried + (long long)row * ld_carried + c;
-        if (!first) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 4)
-                if (j < cols) {
-                    const float4 x = *reinterpret_cast<const float4*>(acc + j);
-                    v[j] = __fadd_rn(x.x, v[j]); v[j + 1] = __fadd_rn(x.y, v[j + 1]);
-                    v[j + 2] = __fadd_rn(x.z, v[j + 2]); v[j + 3] = __fadd_rn(x.w, v[j + 3]);
-                }
-        }
-        if (last) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __fmul_rn(v[j], c_all);
-            emit32<T>(out + (long long)to_row * ld_out + c, v, cols, vec, false);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 32; j += 4)
-                if (j < cols) *reinterpret_cast<float4*>(acc + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-        }
+        x = make_float4(__fadd_rn(old.x, x.x), __fadd_rn(old.y, x.y), __fadd_rn(old.z, x.z), __fadd_rn(old.w, x.w));
+        if (last)
+            put4<T>(out + (long long)to_row * ld_out + c, make_float4(__fmul_rn(x.x, c_all), __fmul_rn(x.y, c_all), __fmul_rn(x.z, c_all), __fmul_rn(x.w, c_all)),
+                    cols, vec);
+        else *reinterpret_cast<float4*>(acc) = x;
     }
 };
 
 template <typename T>
 struct HiddenGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
+    static constexpr bool kStaging = true;
     const XentScalars* sc;
     const int* rows;
     float* parts;
@@ -466,57 +470,53 @@ struct HiddenGradOps {
     HiddenOut<T> out;
     int a0, b0;
     __device__ __forceinline__ TilePlan plan(int pairs) const { return shape.plan(sc->count, pairs); }
-    __device__ __forceinline__ void epilogue(const TileAt& tile, int in_tile, unsigned addr) const {
-        const int count = sc->count, row = tile.m * kTileM + in_tile, n = tile.n;
-        const bool live = row < count;
-        const bool split = tile.k1 - tile.k0 < (shape.v1 - shape.v0 + kTileK - 1) / kTileK;
-        const float c_all = out.scale.value(count);
-        const int to_row = live ? __ldg(rows + row) : 0;
-        const int width = shape.dim - n * kTileN < kTileN ? shape.dim - n * kTileN : kTileN;
-        float* part = parts + (long long)tile.item * (kTileM * kTileN) + in_tile * kTileN;
-#pragma unroll 1
-        for (int c = 0; c < width; c += 32) {
-            float v[32];
-            tmem_load32(addr + c, v);
-            if (!live) continue;
-            if (split) {
-#pragma unroll
-                for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(part + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-            } else {
-                out.put(row, to_row, n * kTileN + c, v, width - c < 32 ? width - c : 32, c_all);
-            }
+    struct Row { int to; float c_all; };     // the caller's row, -1 behind the last one; the factor
+    __device__ __forceinline__ Row prepare(const TilePlan& plan, const TileAt& tile, int in_tile) const {
+        const int row = tile.m * kTileM + in_tile;
+        return {row < plan.count ? __ldg(rows + row) : -1, out.scale.value(plan.count)};
+    }
+    __device__ __forceinline__ void epilogue(const TilePlan& plan, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned stage,
+                                             const Row to) const {
+        const int col = tile.n * kTileN + half * 128, cols = shape.dim - col;
+        const int first_row = tile.m * kTileM + (in_tile & ~31);
+        if (plan.splits > 1) {
+            float* part = parts + (long long)tile.item * (kTileM * kTileN) + (in_tile & ~31) * kTileN + half * 128;
+            rows_by_fours(stage, v, cols, 0, [](int, int, int) { return 0; },
+                          [&](int r, int, int c, float4 x, int) { *reinterpret_cast<float4*>(part + r * kTileN + c) = x; });
+        } else {
+            rows_by_fours(stage, v, cols, to.to,
+                          [&](int r, int to_row, int c) { return to_row >= 0 ? out.get(first_row + r, col + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f); },
+                          [&](int r, int to_row, int c, float4 x, const float4 old) {
+                              if (to_row >= 0) out.put(first_row + r, to_row, col + c, x, old, cols - c, to.c_all);
+                          });
         }
     }
 };
 
-// Adds up the shares of K, in order, where there are any; one thread per row and 32 columns.
+// Adds up the shares of K, in order, where there are any; one thread per row and four columns.
 template <typename T>
 __global__ void __launch_bounds__(256)
 xent_hidden_join_kernel(const XentScalars* __restrict__ sc, const int* __restrict__ rows, const float* __restrict__ parts, const HiddenPlan shape,
                         const HiddenOut<T> out, const int pairs) {
     cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
     const int count = sc->count;
     const TilePlan plan = shape.plan(count, pairs);
     if (plan.splits == 1) return;
     const float c_all = out.scale.value(count);
-    const int strips = (shape.dim + 31) / 32;
+    const int strips = (shape.dim + 3) / 4;
     const long long work = (long long)count * strips;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < work; i += (long long)gridDim.x * 256) {
-        const int row = (int)(i / strips), c = (int)(i - (long long)row * strips) * 32;
-        const int tile = plan.tile_of(row / kTileM, c / kTileN);
-        const float* p = parts + (long long)tile * plan.splits * (kTileM * kTileN) + (row % kTileM) * kTileN + c % kTileN;
-        float v[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-        for (int s = 0; s < plan.splits; ++s, p += kTileM * kTileN) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(p + j);
-                v[j] = __fadd_rn(v[j], x.x); v[j + 1] = __fadd_rn(v[j + 1], x.y);
-                v[j + 2] = __fadd_rn(v[j + 2], x.z); v[j + 3] = __fadd_rn(v[j + 3], x.w);
-            }
+        const int row = (int)(i / strips), c = (int)(i - (long long)row * strips) * 4;
+        const int part = plan.item_of(row / kTileM, c / kTileN);
+        const float4* p = reinterpret_cast<const float4*>(parts + (long long)part * (kTileM * kTileN) + (row % kTileM) * kTileN + c % kTileN);
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int s = 0; s < plan.splits; ++s) {
+            const float4 x = __ldcs(p + s * (kTileM * kTileN / 4));
+            sum = make_float4(__fadd_rn(sum.x, x.x), __fadd_rn(sum.y, x.y), __fadd_rn(sum.z, x.z), __fadd_rn(sum.w, x.w));
         }
-        out.put(row, rows[row], c, v, shape.dim - c < 32 ? shape.dim - c : 32, c_all);
+        out.put(row, rows[row], c, sum, out.get(row, c), shape.dim - c, c_all);
     }
 }
 
@@ -524,6 +524,7 @@ xent_hidden_join_kernel(const XentScalars* __restrict__ sc, const int* __restric
 template <typename T>
 struct WeightGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
+    static constexpr bool kStaging = true;
     const XentScalars* sc;
     T* out;
     long long ld_out;
@@ -531,23 +532,27 @@ struct WeightGradOps {
     int dim, v0, v1, a0, b0;
     bool add, vec;
     __device__ __forceinline__ TilePlan plan(int) const {
-        return {(v1 - v0 + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (sc->count + kTileK - 1) / kTileK, kGroupM, 1};
+        const int count = sc->count;
+        return {count, (v1 - v0 + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (count + kTileK - 1) / kTileK, kGroupM, 1};
     }
-    __device__ __forceinline__ void epilogue(const TileAt& tile, int in_tile, unsigned addr) const {
-        const int row = tile.m * kTileM + in_tile, n = tile.n;
-        const bool live = row < v1 - v0, empty = tile.k0 == tile.k1;
-        const float c_all = scale.value(sc->count);
-        T* to = out + (long long)(v0 + row) * ld_out + n * kTileN;
-        const int width = dim - n * kTileN < kTileN ? dim - n * kTileN : kTileN;
-#pragma unroll 1
-        for (int c = 0; c < width; c += 32) {
-            float v[32];
-            tmem_load32(addr + c, v);
-            if (!live) continue;
+    __device__ __forceinline__ float prepare(const TilePlan& plan, const TileAt&, int) const { return scale.value(plan.count); }
+    __device__ __forceinline__ void epilogue(const TilePlan&, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned stage,
+                                             const float c_all) const {
+        const int col = tile.n * kTileN + half * 128, cols = dim - col;
+        const int first_row = tile.m * kTileM + (in_tile & ~31), rows = v1 - v0 - first_row;
+        T* first = out + (long long)(v0 + first_row) * ld_out + col;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = empty ? 0.0f : __fmul_rn(v[j], c_all);
-            emit32<T>(to + c, v, width - c < 32 ? width - c : 32, vec, add);
-        }
+        for (int j = 0; j < 128; ++j) v[j] = __fmul_rn(v[j], c_all);
+        if (vec && !add) rows_to_memory<T>(stage, v, cols, [&](int r) { return r < rows ? first + r * ld_out : nullptr; });
+        else
+            rows_by_fours(stage, v, cols, 0,
+                          [&](int r, int, int c) {
+                              return add && r < rows ? get4<T>(first + r * ld_out + c, cols - c, vec) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                          },
+                          [&](int r, int, int c, const float4 x, const float4 old) {
+                              const float4 y = make_float4(__fadd_rn(old.x, x.x), __fadd_rn(old.y, x.y), __fadd_rn(old.z, x.z), __fadd_rn(old.w, x.w));
+                              if (r < rows) put4<T>(first + r * ld_out + c, y, cols - c, vec);
+                          });
     }
 };
 
@@ -653,7 +658,7 @@ static int make_map(CUtensorMap* map, int dtype, uintptr_t base, int64_t rows, i
 template <int TN, bool MN_A, bool MN_B, typename Ops>
 static int launch_tiles(Device* d, const CUtensorMap& a, const CUtensorMap& b, const Ops& ops, int64_t max_tiles, int* launched = nullptr) {
     auto kernel = tile_gemm_kernel<TN, MN_A, MN_B, Ops>;
-    constexpr int kGemmSmem = Ring<TN>::kSmem;
+    constexpr int kGemmSmem = Ring<TN>::kSmem + (Ops::kStaging ? 8 * kStagingBytes : 0);
     static std::mutex mu;
     static int pairs_of[64] = {0};                   // per device ordinal
     int pairs;
@@ -724,7 +729,7 @@ static XentSpace common_space(const gm_linear_xent_t* h) {
 static XentSpace forward_space(const gm_linear_xent_t* h) {
     XentSpace s = common_space(h);
     s.stats = s.total;
-    const int64_t stat_tiles = h->tokens <= kFewRows ? (h->vocab + 31) / 32 : (h->vocab + kTileN - 1) / kTileN;
+    const int64_t stat_tiles = h->tokens <= kFewRows ? (h->vocab + 31) / 32 : (h->vocab + kTileN / 2 - 1) / (kTileN / 2);
     s.target_logit = s.stats + up256(stat_tiles * s.cap * 8);
     s.partial = s.target_logit + up256(s.cap * 4);
     s.total = s.partial + up256(s.cap * 4);
@@ -831,7 +836,8 @@ static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
     GM_TRY(index_and_gather<T>(c, hidden, targets, weight, target_logit, losses, lse, (T*)nullptr));
     float2* stats = (float2*)(c.ws + s.stats);
     const bool few = h->tokens <= kFewRows;
-    int tiles = (int)((h->vocab + kTileN - 1) / kTileN);
+    const int64_t n_tiles = (h->vocab + kTileN - 1) / kTileN;
+    int tiles = (int)((h->vocab + kTileN / 2 - 1) / (kTileN / 2));
     if (few) {
         tiles = (int)((h->vocab + 31) / 32);
         if (h->tokens <= 32) GM_TRY((few_logits<T, 32>(c, map_w, stats)));
@@ -840,7 +846,7 @@ static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
         CUtensorMap map_x;
         GM_TRY(make_map(&map_x, h->dtype, c.ws + s.packed, s.cap, h->dim, s.ld_packed, kHalf));
         const StatsOps<T> ops{c.sc(), c.target(), stats, (int)s.cap, (int)h->dim, (int)h->vocab, logits_group(h), 0, 0};
-        GM_TRY((launch_tiles<kTileN, false, false>(c.d, map_x, map_w, ops, s.cap / kTileM * tiles)));
+        GM_TRY((launch_tiles<kTileN, false, false>(c.d, map_x, map_w, ops, s.cap / kTileM * n_tiles)));
     }
     // a CTA per row up to a few rows per SM, 32 rows per CTA beyond
     auto join = h->tokens <= 1024 ? xent_join_kernel<1> : xent_join_kernel<32>;

@@ -1,14 +1,21 @@
 // gm_tile_gemm.cuh -- the matrix products of the vocabulary loss on the fifth-generation
-// tensor cores: a persistent kernel of CTA pairs, C[256 x N] per pair and tile.
+// tensor cores: a persistent kernel of CTA pairs.
 //
 //   warp 0    one lane copies operand tiles into a ring of shared-memory stages (TMA)
 //   warp 1    one lane of the pair's first CTA issues tcgen05.mma (M = 256 over both SMs,
 //             N = 256 or less, K = 16, fp16 or bf16 in, binary32 accumulators in TMEM)
-//   warps 2-5 read the accumulators (each thread one row) and run the epilogue
+//   warps 2-9 read the accumulators (each thread half of a row) and run the epilogue
 //
-// The accumulators take N TMEM columns and there are two sets of them, so the epilogue of
-// one tile runs while the next one is multiplied.  Of the pair, each CTA holds 128 rows of A
-// and half of the N rows of B: with N = 256 a stage is 32 KB per CTA and six of them fit.
+// C is made of tiles of 256 rows by TN columns; TMEM holds two of them, in two slots that take
+// turns.  Of a tile's operands each CTA holds 128 rows of A and half of the TN rows of B: with
+// N = 256 a stage is 32 KB per CTA and six of them fit.  The epilogue takes a slot's numbers into
+// registers, 128 per thread, and frees the slot before it works on them.
+//
+// Measured on B200 at 8,192 x 4,096 x 32,768: the tensor core is busy in 95 % of the cycles.  In
+// a loop of seconds the card's power limit holds it near 1,350 TFLOP/s (the library's products of the
+// same shapes reach 1,340 to 1,410).  Tiles of 512 x 256 per pair, whose operands cross L2 a
+// quarter less often, were built too and were 5 % slower (81 % of the cycles, TMEM leaves no second
+// slot); waiting with the default poll interval cost 6 %, rows stored lane by lane 3 %.
 //
 // Where a product has too few tiles for the GPU, a tile's K range is split over several pairs,
 // and a kernel of its own adds up what they leave (TilePlan::splits).
@@ -30,13 +37,13 @@ namespace gm {
 constexpr int kTileM = 256, kTileN = 256, kTileK = 64;
 constexpr int kHalf = 128;                       // rows of A that one CTA of the pair holds
 constexpr int kOperandBytes = kHalf * kTileK * 2;
-constexpr int kGemmThreads = 192;
-template <int TN> struct Ring {                  // the ring of stages for tiles of TN columns
+constexpr int kGemmThreads = 320;
+template <int TN> struct Ring {                  // a stage: a block of A, then one of B
     static constexpr int kRowsB = TN / 2;
     static constexpr int kStageBytes = kOperandBytes + kRowsB * kTileK * 2;
-    static constexpr int kFit = 200 * 1024 / kStageBytes;
+    static constexpr int kFit = 193 * 1024 / kStageBytes;
     static constexpr int kStages = kFit < 12 ? kFit : 12;
-    static constexpr int kSmem = kStages * kStageBytes + 1024;
+    static constexpr int kSmem = kStages * kStageBytes + 1024;        // and 8 x kStagingBytes with kStaging
 };
 
 // ---- mbarriers ----
@@ -55,12 +62,15 @@ __device__ __forceinline__ unsigned pair_leader_addr(unsigned addr) {
 __device__ __forceinline__ void mbar_arrive_cluster(unsigned cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// A try sleeps up to this long in hardware.  Short sleeps are polls, and a poll is an access to the
+// shared memory that feeds the tensor core: with the default the waiting epilogue warps cost 6 %.
+constexpr unsigned kPollNs = 10000000;
 __device__ __forceinline__ bool mbar_try(unsigned bar, unsigned parity) {
     unsigned done;
     asm volatile("{\n\t.reg .pred p;\n\t"
-                 "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+                 "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
                  "selp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+                 : "=r"(done) : "r"(bar), "r"(parity), "r"(kPollNs) : "memory");
     return done != 0;
 }
 // False when the wait ran out or another role gave up.
@@ -108,54 +118,146 @@ __device__ __forceinline__ void mma_commit_pair(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(bar), "h"((unsigned short)3) : "memory");
 }
-__device__ __forceinline__ void tmem_load32(unsigned addr, float (&v)[32]) {
-    unsigned r[32];
-    __syncwarp();                                    // the load is for whole, converged warps
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-                   "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-                   "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+// COUNT columns (a multiple of 32) of this thread's TMEM lane, for whole, converged warps.
+template <int COUNT>
+__device__ __forceinline__ void tmem_read(unsigned addr, float (&v)[COUNT]) {
+    unsigned r[COUNT];
+    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int c = 0; c < COUNT; c += 32)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                     "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                     "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                     : "=r"(r[c]), "=r"(r[c + 1]), "=r"(r[c + 2]), "=r"(r[c + 3]), "=r"(r[c + 4]), "=r"(r[c + 5]), "=r"(r[c + 6]), "=r"(r[c + 7]),
+                       "=r"(r[c + 8]), "=r"(r[c + 9]), "=r"(r[c + 10]), "=r"(r[c + 11]), "=r"(r[c + 12]), "=r"(r[c + 13]), "=r"(r[c + 14]),
+                       "=r"(r[c + 15]), "=r"(r[c + 16]), "=r"(r[c + 17]), "=r"(r[c + 18]), "=r"(r[c + 19]), "=r"(r[c + 20]), "=r"(r[c + 21]),
+                       "=r"(r[c + 22]), "=r"(r[c + 23]), "=r"(r[c + 24]), "=r"(r[c + 25]), "=r"(r[c + 26]), "=r"(r[c + 27]), "=r"(r[c + 28]),
+                       "=r"(r[c + 29]), "=r"(r[c + 30]), "=r"(r[c + 31])
+                     : "r"(addr + c));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    // the registers are valid from here on: nothing that uses them may move in front of the wait
+#pragma unroll
+    for (int c = 0; c < COUNT; c += 8)
+        asm volatile("" : "+r"(r[c]), "+r"(r[c + 1]), "+r"(r[c + 2]), "+r"(r[c + 3]), "+r"(r[c + 4]), "+r"(r[c + 5]), "+r"(r[c + 6]), "+r"(r[c + 7]));
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// Where the work of one turn lies: tile, its share of K, and the turn's number.
+// ---- rows to memory ----
+// A warp holds 32 rows, one per lane.  Stored as they are, each lane's 16 bytes would be a line of
+// their own, and a line is a cycle of the memory that feeds the tensor core; so they go through 4 KB of
+// shared memory per warp and leave as whole lines.  The 16-byte units of a row are exchanged by the
+// row's number so that neither side has bank conflicts.
+constexpr int kStagingBytes = 4096;
+__device__ __forceinline__ void stage_put(unsigned stage, int row, int unit, uint4 x) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(stage + row * 128 + ((unit ^ (row & 7)) << 4)), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+}
+__device__ __forceinline__ uint4 stage_get(unsigned stage, int row, int unit) {
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(stage + row * 128 + ((unit ^ (row & 7)) << 4)) : "memory");
+    return x;
+}
+
+// 128 columns of 32 rows in a 16-bit type: to(row in the warp) is where its first column goes, null
+// for a row that is not written; `cols` columns exist; rows begin on 16-byte boundaries.
+template <typename T, typename To>
+__device__ __forceinline__ void rows_to_memory(unsigned stage, const float (&v)[128], int cols, To to) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int c = 0; c < 128; c += 64) {
+        if (c >= cols) break;
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            stage_put(stage, lane, u, make_uint4(pack2<T>(v[c + 8 * u], v[c + 8 * u + 1]), pack2<T>(v[c + 8 * u + 2], v[c + 8 * u + 3]),
+                                                 pack2<T>(v[c + 8 * u + 4], v[c + 8 * u + 5]), pack2<T>(v[c + 8 * u + 6], v[c + 8 * u + 7])));
+        __syncwarp();
+        const int unit = lane & 7, at = c + unit * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = i * 4 + (lane >> 3);
+            const uint4 x = stage_get(stage, row, unit);
+            T* p = to(row);
+            if (p == nullptr) continue;
+            if (at + 8 <= cols) {
+                *reinterpret_cast<uint4*>(p + at) = x;
+            } else {
+                const unsigned w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (at + k < cols) reinterpret_cast<unsigned short*>(p)[at + k] = (unsigned short)(w[k >> 1] >> (16 * (k & 1)));
+            }
+        }
+    }
+}
+
+// 128 columns of 32 rows as they are (binary32), four at a time, neighbouring lanes with neighbouring
+// columns: first old = get(row in the warp, that row's lane's tag, column) for eight of them, so that
+// what is read is in flight together, then put(row, tag, column, four values, old).
+template <typename Get, typename Put>
+__device__ __forceinline__ void rows_by_fours(unsigned stage, const float (&v)[128], int cols, int tag, Get get, Put put) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int c = 0; c < 128; c += 32) {
+        if (c >= cols) break;
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            stage_put(stage, lane, u, make_uint4(__float_as_uint(v[c + 4 * u]), __float_as_uint(v[c + 4 * u + 1]), __float_as_uint(v[c + 4 * u + 2]),
+                                                 __float_as_uint(v[c + 4 * u + 3])));
+        __syncwarp();
+        const int unit = lane & 7, at = c + unit * 4;
+        decltype(get(0, 0, 0)) old[8];
+        int tags[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            tags[i] = __shfl_sync(0xffffffffu, tag, i * 4 + (lane >> 3));
+            if (at < cols) old[i] = get(i * 4 + (lane >> 3), tags[i], at);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = i * 4 + (lane >> 3);
+            const uint4 x = stage_get(stage, row, unit);
+            if (at < cols) put(row, tags[i], at, make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w)), old[i]);
+        }
+    }
+}
+
+// The work of one turn: a tile, its share of K, and the turn's number.
 struct TileAt { int m, n, split, item, k0, k1; };
 
 // One product: m_tiles x n_tiles tiles, walked m first inside groups of `group` m-tiles, so that
-// the operands of the tiles in flight are shared in L2; each in `splits` shares of K.
+// the operands of the tiles in flight are shared in L2; each tile in `splits` shares of K.
 struct TilePlan {
+    int count;                                                // rows with a target
     int m_tiles, n_tiles, k_blocks, group, splits;
     __device__ __forceinline__ int items() const { return m_tiles * n_tiles * splits; }
     __device__ __forceinline__ TileAt at(int item) const {
         TileAt x;
         const int t = item / splits, per = group * n_tiles;
         const int g = t / per, m0 = g * group;
-        const int rows = m_tiles - m0 < group ? m_tiles - m0 : group;
+        const int high = m_tiles - m0 < group ? m_tiles - m0 : group;
         const int r = t - g * per;
         x.item = item;
-        x.n = r / rows;
-        x.m = m0 + (r - x.n * rows);
+        x.n = r / high;
+        x.m = m0 + (r - x.n * high);
         x.split = item - t * splits;
         x.k0 = (int)((long long)k_blocks * x.split / splits);
         x.k1 = (int)((long long)k_blocks * (x.split + 1) / splits);
         return x;
     }
-    // the inverse: number of the tile at (m, n)
-    __device__ __forceinline__ int tile_of(int m, int n) const {
+    // the inverse: the turn that has the first share of tile (m, n)
+    __device__ __forceinline__ int item_of(int m, int n) const {
         const int m0 = m / group * group;
-        const int rows = m_tiles - m0 < group ? m_tiles - m0 : group;
-        return m0 * n_tiles + n * rows + (m - m0);
+        const int high = m_tiles - m0 < group ? m_tiles - m0 : group;
+        return (m0 * n_tiles + n * high + (m - m0)) * splits;
     }
 };
 
 // Shares of K per tile, at most 16 and `most_items` in all, for the shortest run on `pairs` CTA
-// pairs: rounds of items, each as long as its k-blocks plus a start and an epilogue (about eight).
+// pairs: rounds of turns, each as long as its k-blocks plus a start and an epilogue (about eight).
 __device__ __forceinline__ int choose_splits(int tiles, int k_blocks, int pairs, int most_items) {
     int best = 1, best_cost = 0x7fffffff;
     for (int s = 1; s <= 16 && s <= k_blocks && (s == 1 || tiles * s <= most_items); ++s) {
@@ -167,11 +269,14 @@ __device__ __forceinline__ int choose_splits(int tiles, int k_blocks, int pairs,
 
 // MN_A / MN_B: that operand is MN-major.  Ops provides
 //   kBf16             whether the inputs are bf16 (else fp16)
+//   kStaging          whether the epilogue wants shared memory
 //   plan(pairs)       the tiles, read on the device
 //   a0, b0            first row of A and of B (first K-row of an MN-major operand) in their maps
-//   epilogue(at, row, addr)   the turn, the row inside the tile, the TMEM address of its first
-//                     column; called by whole warps, also for rows behind the last one; with an
-//                     empty share of K (at.k0 == at.k1) the accumulators hold nothing and C is zero
+//   prepare(plan, at, row)   what the epilogue of this turn needs for the row inside the tile, read
+//                     while the product runs
+//   epilogue(plan, at, row, v, half, stage, prepared)   the row inside the tile, half of its
+//                     columns (zeros with an empty share of K), which half, 4 KB of shared memory for
+//                     the warp (with kStaging); called by whole warps, also for rows behind the last one
 template <int TN, bool MN_A, bool MN_B, typename Ops>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Ops ops,
@@ -191,7 +296,7 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     if (tid == 0) {
         abort_flag = 0;
         for (int s = 0; s < kStages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(smem_u32(&acc_full[b]), 1); mbar_init(smem_u32(&acc_empty[b]), 8); }
+        for (int b = 0; b < 2; ++b) { mbar_init(smem_u32(&acc_full[b]), 1); mbar_init(smem_u32(&acc_empty[b]), 16); }
         mbar_init(smem_u32(&drain), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -206,6 +311,7 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const unsigned tmem = tmem_base;
     // all of the above may run while the kernel before this one ends
     cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
     const TilePlan plan = ops.plan(pairs);
     const int items = plan.items();
 
@@ -221,7 +327,7 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 const unsigned turn = issued / kStages;
                 if (!mbar_wait(smem_u32(&empty[s]), (turn & 1u) ^ 1u, &abort_flag, budget)) { ok = false; break; }
                 const unsigned bar = pair_leader_addr(smem_u32(&full[s]));
-                if (rank == 0) mbar_expect(smem_u32(&full[s]), 2 * kStageBytes);
+                if (rank == 0) mbar_expect(smem_u32(&full[s]), 2 * kStageBytes);          // both CTAs' copies
                 const unsigned a = ring + s * kStageBytes, b = a + kOperandBytes;
                 if (MN_A) {
                     tma_load(a, &map_a, row_a, ops.a0 + k * kTileK, bar);
@@ -243,15 +349,15 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const unsigned in = Ops::kBf16 ? 1u : 0u;
         const unsigned idesc = (1u << 4) | (in << 7) | (in << 10) | ((MN_A ? 1u : 0u) << 15) | ((MN_B ? 1u : 0u) << 16) |
                                ((unsigned)(TN / 8) << 17) | ((unsigned)(kTileM / 16) << 24);
-        unsigned used = 0;
+        unsigned used = 0;                                       // k-blocks consumed
         int count = 0;
         bool ok = true;
         for (int t = pair; t < items && ok; t += pairs, ++count) {
             const TileAt at = plan.at(t);
-            const int b = count & 1;
-            if (!mbar_wait(smem_u32(&acc_empty[b]), ((count >> 1) & 1) ^ 1, &abort_flag, budget)) { ok = false; break; }
+            const int slot = count & 1;
+            if (!mbar_wait(smem_u32(&acc_empty[slot]), ((count >> 1) & 1) ^ 1, &abort_flag, budget)) { ok = false; break; }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const unsigned d = tmem + (unsigned)b * TN;
+            const unsigned d = tmem + (unsigned)slot * 256u;
             for (int k = at.k0; k < at.k1; ++k, ++used) {
                 const int s = used % kStages;
                 if (!mbar_wait(smem_u32(&full[s]), (used / kStages) & 1u, &abort_flag, budget)) { ok = false; break; }
@@ -263,7 +369,7 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     mma_pair(d, da + (MN_A ? 128 * i : 2 * i), db + (MN_B ? 128 * i : 2 * i), idesc, k > at.k0 || i > 0);
                 mma_commit_pair(smem_u32(&empty[s]));
             }
-            if (ok) mma_commit_pair(smem_u32(&acc_full[b]));
+            if (ok) mma_commit_pair(smem_u32(&acc_full[slot]));
         }
         if (!ok) {
             mma_commit_pair(smem_u32(&drain));
@@ -273,18 +379,28 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     } else if (warp >= 2) {
         // ---- epilogue ----
         const int quarter = warp & 3;                            // the TMEM lanes this warp may read
-        const int row = quarter * 32 + lane;
+        const int half = (warp - 2) >> 2;
+        const int row = (int)rank * kHalf + quarter * 32 + lane;
+        const unsigned staging = ring + kStages * kStageBytes + (warp - 2) * kStagingBytes;
+        constexpr int kColumns = TN / 2 < 32 ? 32 : TN / 2;       // a narrow tile is all the first half's
         int count = 0;
         for (int t = pair; t < items; t += pairs, ++count) {
             const TileAt at = plan.at(t);
-            const int b = count & 1;
-            const bool ok = mbar_wait(smem_u32(&acc_full[b]), (count >> 1) & 1, &abort_flag, budget);
+            const int slot = count & 1;
+            const auto prepared = ops.prepare(plan, at, row);
+            const bool ok = mbar_wait(smem_u32(&acc_full[slot]), (count >> 1) & 1, &abort_flag, budget);
             if (!__all_sync(0xffffffffu, ok)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            ops.epilogue(at, (int)rank * kHalf + row, tmem + (unsigned)b * TN + ((unsigned)(quarter * 32) << 16));
+            float v[kColumns];
+            tmem_read<kColumns>(tmem + (unsigned)(slot * 256 + half * kColumns) + ((unsigned)(quarter * 32) << 16), v);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(pair_leader_addr(smem_u32(&acc_empty[b])));
+            if (lane == 0) mbar_arrive_cluster(pair_leader_addr(smem_u32(&acc_empty[slot])));
+            if (at.k0 == at.k1) {
+#pragma unroll
+                for (int j = 0; j < kColumns; ++j) v[j] = 0.0f;
+            }
+            ops.epilogue(plan, at, row, v, half, staging, prepared);
         }
     }
     __syncwarp();
