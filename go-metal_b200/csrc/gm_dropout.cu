@@ -54,6 +54,7 @@ template <typename T, bool RES, bool FLAT>
 __global__ void __launch_bounds__(kDropThreads)
 dropout_vec_kernel(const T* x, const T* res, T* y, const long long n, const int row_groups,
                    const long long ld_x, const long long ld_r, const long long ld_y, const __grid_constant__ Drop d) {
+    chain_begin();
     const DropOffset o = drop_begin(d);
     const long long groups = n >> 3;
     const long long g0 = (long long)blockIdx.x * (kDropThreads * kDropVec) + threadIdx.x;
@@ -100,6 +101,7 @@ template <typename T, bool RES>
 __global__ void __launch_bounds__(kDropThreads)
 dropout_any_kernel(const T* x, const T* res, T* y, const long long n, const long long cols,
                    const long long ld_x, const long long ld_r, const long long ld_y, const __grid_constant__ Drop d) {
+    chain_begin();
     const DropOffset o = drop_begin(d);
     const long long g = (long long)blockIdx.x * kDropThreads + threadIdx.x;
     if (g * 8 >= n) return;
@@ -127,11 +129,11 @@ static int launch_dropout(Device* d, int64_t rows, int64_t cols, uintptr_t x, in
     const int64_t per_cta = kDropThreads * (vec ? kDropVec : 1);
     const int64_t grid = ((n + 7) / 8 + per_cta - 1) / per_cta;
     if (grid > 0x7fffffff) { set_error("%lld x %lld elements are too many", (long long)rows, (long long)cols); return GM_ERR_BAD_SIZE; }
-    if (vec && flat) dropout_vec_kernel<T, RES, true><<<(unsigned)grid, kDropThreads, 0, d->stream>>>(px, pr, py, n, 0, 0, 0, 0, drop);
-    else if (vec) dropout_vec_kernel<T, RES, false><<<(unsigned)grid, kDropThreads, 0, d->stream>>>(px, pr, py, n, (int)(cols / 8), ld_x, ld_r, ld_y, drop);
-    else dropout_any_kernel<T, RES><<<(unsigned)grid, kDropThreads, 0, d->stream>>>(px, pr, py, n, cols, ld_x, ld_r, ld_y, drop);
+    const dim3 g((unsigned)grid), t(kDropThreads);
+    if (vec && flat) GM_CUDA_CHECK(launch_chained(dropout_vec_kernel<T, RES, true>, g, t, 0, d->stream, px, pr, py, n, 0, 0, 0, 0, drop));
+    else if (vec) GM_CUDA_CHECK(launch_chained(dropout_vec_kernel<T, RES, false>, g, t, 0, d->stream, px, pr, py, n, (int)(cols / 8), ld_x, ld_r, ld_y, drop));
+    else GM_CUDA_CHECK(launch_chained(dropout_any_kernel<T, RES>, g, t, 0, d->stream, px, pr, py, n, cols, ld_x, ld_r, ld_y, drop));
     d->launches++;
-    GM_CUDA_CHECK(cudaGetLastError());
     return GM_OK;
 }
 

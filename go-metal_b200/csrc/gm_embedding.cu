@@ -25,6 +25,7 @@ template <typename T, bool VEC, bool WHOLE, int ROWS>
 __global__ void __launch_bounds__(kEmbThreads, 4)
 embedding_forward_kernel(const T* __restrict__ table, const int* __restrict__ tokens, T* __restrict__ out, const int n, const int dim,
                          const int vocab, const int ld_table, const int ld_out, const float scale, const __grid_constant__ Drop d) {
+    chain_begin();
     const DropOffset o = drop_begin(d);
     const float up = __fmul_rn(scale, d.up);
     const int groups = (int)(((unsigned)dim + 7u) >> 3);
@@ -86,6 +87,7 @@ token_sort_tile_kernel(const int* __restrict__ tokens, const long long n, const 
     __shared__ unsigned long long buf[kSortTile];
     const int tid = threadIdx.x;
     const long long i = (long long)blockIdx.x * kSortTile + tid;
+    chain_begin();
     unsigned long long key = i < n ? sort_word(tokens, i, vocab, padding) : ~0ull;
     if (i == 0) *split = 0;
     if (used)
@@ -138,6 +140,7 @@ __global__ void __launch_bounds__(128)
 token_merge_kernel(const unsigned long long* __restrict__ in, unsigned long long* __restrict__ out, const long long n, const int run,
                    unsigned char* used, const unsigned vocab) {
     const long long i = (long long)blockIdx.x * 128 + threadIdx.x;
+    chain_begin();
     if (i >= n) return;
     const unsigned long long word = __ldg(in + i);
     const unsigned token = (unsigned)(word >> 32);
@@ -205,6 +208,7 @@ embedding_sum_kernel(const T* __restrict__ dout, const unsigned long long* __res
                      const int ld_out, const float scale, const int piece, const int col_ctas, const int sum_ctas, const __grid_constant__ Drop d) {
     __shared__ unsigned tok[kPieceMost], pos[kPieceMost];
     const int tid = threadIdx.x;
+    chain_begin();
     const int groups = (int)(((unsigned)dim + 7u) >> 3);
     const long long before = ADD ? blockIdx.x : (long long)blockIdx.x * sum_ctas / gridDim.x;       // summing CTAs in front of this one
     if (!ADD && ((long long)blockIdx.x + 1) * sum_ctas / gridDim.x == before) {
@@ -294,6 +298,7 @@ embedding_join_kernel(const unsigned long long* __restrict__ words, const float*
                       const int n, const int dim, const int ld_table, const float scale, const int piece, const __grid_constant__ Drop d) {
     __shared__ float4 part[kJoinWays][2][kJoinLanes];
     const int x = threadIdx.x, y = threadIdx.y;
+    chain_begin();
     const int groups = (int)(((unsigned)dim + 7u) >> 3), col_blocks = (groups + kJoinLanes - 1) / kJoinLanes;
     const float up = __fmul_rn(scale, d.up);
     const long long items = (long long)split[0] * col_blocks;
@@ -389,9 +394,11 @@ static int launch_embedding_forward(Device* d, const gm_embedding_t* e, uintptr_
     const bool vec = table % 16 == 0 && out % 16 == 0 && e->ld_table * (int)sizeof(T) % 16 == 0 && e->ld_out * (int)sizeof(T) % 16 == 0;
     // four tokens per thread keep more loads in flight; a call too small for that takes one
     const bool many = e->tokens * gy >= (int64_t)d->sm_count * 8 * block.y;
-#define GM_FORWARD(VEC, WHOLE, ROWS)                                                                                                            \
-    embedding_forward_kernel<T, VEC, WHOLE, ROWS><<<dim3((unsigned)((e->tokens + block.y * ROWS - 1) / (block.y * ROWS)), gy), block, 0, d->stream>>>( \
-        (const T*)table, (const int*)tokens, (T*)out, (int)e->tokens, (int)e->dim, (int)e->vocab, (int)e->ld_table, (int)e->ld_out, e->scale, drop)
+#define GM_FORWARD(VEC, WHOLE, ROWS)                                                                                                       \
+    GM_CUDA_CHECK(launch_chained(embedding_forward_kernel<T, VEC, WHOLE, ROWS>,                                                             \
+                                 dim3((unsigned)((e->tokens + block.y * ROWS - 1) / (block.y * ROWS)), gy), block, 0, d->stream,             \
+                                 (const T*)table, (const int*)tokens, (T*)out, (int)e->tokens, (int)e->dim, (int)e->vocab, (int)e->ld_table, \
+                                 (int)e->ld_out, e->scale, drop))
     const bool whole = e->dim % 8 == 0;
     if (!vec) GM_FORWARD(false, false, 1);
     else if (!whole) GM_FORWARD(true, false, 1);
@@ -413,10 +420,12 @@ static int launch_embedding_backward(Device* d, const gm_embedding_t* e, uintptr
     int* split = (int*)(ws + s.split);
     float* pieces = (float*)(ws + s.pieces);
     const int64_t n = e->tokens;
-    token_sort_tile_kernel<<<(unsigned)((n + kSortTile - 1) / kSortTile), kSortTile, 0, d->stream>>>((const int*)tokens, n, e->vocab, e->padding_token, words, used, split);
+    GM_CUDA_CHECK(launch_chained(token_sort_tile_kernel, dim3((unsigned)((n + kSortTile - 1) / kSortTile)), dim3(kSortTile), 0, d->stream, (const int*)tokens, n,
+                                 e->vocab, e->padding_token, words, used, split));
     d->launches++;
     for (int64_t run = kSortTile; run < n; run *= kMergeWays) {
-        token_merge_kernel<<<(unsigned)((n + 127) / 128), 128, 0, d->stream>>>(words, other, n, (int)run, run == kSortTile ? used : nullptr, (unsigned)e->vocab);
+        GM_CUDA_CHECK(launch_chained(token_merge_kernel, dim3((unsigned)((n + 127) / 128)), dim3(128), 0, d->stream, words, other, n, (int)run,
+                                     run == kSortTile ? used : nullptr, (unsigned)e->vocab));
         d->launches++;
         unsigned long long* t = words; words = other; other = t;
     }
@@ -430,14 +439,14 @@ static int launch_embedding_backward(Device* d, const gm_embedding_t* e, uintptr
     const int64_t join_most = chunks * ((groups + kJoinLanes - 1) / kJoinLanes);
     const unsigned join_grid = (unsigned)(join_most < d->sm_count * 8 ? join_most : d->sm_count * 8);
     const dim3 join_block(kJoinLanes, kJoinWays);
-#define GM_SUM(VEC, WHOLE, ADD)                                                                                                                \
-    do {                                                                                                                                       \
-        embedding_sum_kernel<T, G, VEC, WHOLE, ADD><<<(unsigned)(sum_ctas + zero_ctas), kSumThreads, 0, d->stream>>>(                          \
-            (const T*)dout, words, used, pieces, split, (G*)dtable, (int)n, (int)e->dim, (int)e->vocab, (int)e->ld_table, (int)e->ld_out, e->scale,   \
-            piece, (int)col_ctas, (int)sum_ctas, drop);                                                                                       \
-        if (chunks > 1)                                                                                                                       \
-            embedding_join_kernel<G, VEC, WHOLE, ADD><<<join_grid, join_block, 0, d->stream>>>(                                                 \
-                words, pieces, split, (G*)dtable, (int)n, (int)e->dim, (int)e->ld_table, e->scale, piece, drop);                       \
+#define GM_SUM(VEC, WHOLE, ADD)                                                                                                              \
+    do {                                                                                                                                     \
+        GM_CUDA_CHECK(launch_chained(embedding_sum_kernel<T, G, VEC, WHOLE, ADD>, dim3((unsigned)(sum_ctas + zero_ctas)), dim3(kSumThreads), \
+                                     0, d->stream, (const T*)dout, words, used, pieces, split, (G*)dtable, (int)n, (int)e->dim,              \
+                                     (int)e->vocab, (int)e->ld_table, (int)e->ld_out, e->scale, piece, (int)col_ctas, (int)sum_ctas, drop)); \
+        if (chunks > 1)                                                                                                                      \
+            GM_CUDA_CHECK(launch_chained(embedding_join_kernel<G, VEC, WHOLE, ADD>, dim3(join_grid), join_block, 0, d->stream, words,        \
+                                         pieces, split, (G*)dtable, (int)n, (int)e->dim, (int)e->ld_table, e->scale, piece, drop));          \
     } while (0)
     if (accumulate) {
         if (vec && whole) GM_SUM(true, true, true);
@@ -450,7 +459,6 @@ static int launch_embedding_backward(Device* d, const gm_embedding_t* e, uintptr
     }
 #undef GM_SUM
     d->launches += chunks > 1 ? 2 : 1;
-    GM_CUDA_CHECK(cudaGetLastError());
     return GM_OK;
 }
 

@@ -61,17 +61,23 @@ xent_index_kernel(const int* __restrict__ targets, const int n, const int vocab,
     __shared__ int warp_sum[32];
     __shared__ int carry;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    cudaGridDependencySynchronize();
-    cudaTriggerProgrammaticLaunchCompletion();
+    const bool wide = (reinterpret_cast<uintptr_t>(targets) & 15) == 0;
+    chain_begin();
     if (tid == 0) carry = 0;
     __syncthreads();
     for (long long base = 0; base < n; base += kIndexThreads * 8) {
         int t[8];
         int mine = 0;
+        const long long i0 = base + tid * 8;
+        if (wide && i0 + 8 <= n) {
+            const int4 a = __ldg(reinterpret_cast<const int4*>(targets + i0)), b = __ldg(reinterpret_cast<const int4*>(targets + i0) + 1);
+            t[0] = a.x; t[1] = a.y; t[2] = a.z; t[3] = a.w; t[4] = b.x; t[5] = b.y; t[6] = b.z; t[7] = b.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = i0 + k < n ? __ldg(targets + i0 + k) : -1;
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const long long i = base + tid * 8 + k;
-            t[k] = i < n ? __ldg(targets + i) : -1;
             if (t[k] >= vocab) t[k] = -1;
             mine += t[k] >= 0;
         }
@@ -160,8 +166,7 @@ xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n
                    float* __restrict__ losses, float* __restrict__ lse, T* __restrict__ dhidden, const bool vec, const bool vec_out) {
     __shared__ float warp_sum[kGatherThreads / 32];
     const int r = blockIdx.x, tid = threadIdx.x;
-    cudaGridDependencySynchronize();
-    cudaTriggerProgrammaticLaunchCompletion();
+    chain_begin();
     int count, row, goal;
     if (few) {
         find_row(targets, n, vocab, r, &count, &row, &goal);
@@ -236,7 +241,7 @@ struct Goal { int at; };        // a row's target
 template <typename T>
 struct StatsOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
-    static constexpr bool kStaging = false;
+    static constexpr bool kStaging = false, kEarlyA = false;
     const XentScalars* sc;
     const int* target;
     float2* stats;               // [128 vocabulary entries][row]
@@ -300,14 +305,17 @@ template <bool MAX> __device__ __forceinline__ float lanes_to_columns(float (&v)
 template <typename T, int TN>
 struct FewStatsOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
-    static constexpr bool kStaging = false;
+    static constexpr bool kStaging = false, kEarlyA = true;
     const XentScalars* sc;
     const int* target;
     float2* stats;               // [32 vocabulary entries][row]
     int rows_cap, dim, vocab, a0, b0;
+    // one column of tiles, also where no row has a target: then the epilogue writes nothing
+    __device__ __forceinline__ TilePlan shape() const { return {0, (vocab + kTileM - 1) / kTileM, 1, (dim + kTileK - 1) / kTileK, 1, 1}; }
     __device__ __forceinline__ TilePlan plan(int) const {
-        const int count = sc->count;
-        return {count, (vocab + kTileM - 1) / kTileM, count > 0 ? 1 : 0, (dim + kTileK - 1) / kTileK, 1, 1};
+        TilePlan p = shape();
+        p.count = sc->count;
+        return p;
     }
     __device__ __forceinline__ Goal prepare(const TilePlan&, const TileAt&, int) const { return {0}; }
     static constexpr int kColumns = TN / 2 < 32 ? 32 : TN / 2;
@@ -347,7 +355,7 @@ struct FewStatsOps {
 template <typename T>
 struct SoftmaxGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
-    static constexpr bool kStaging = true;
+    static constexpr bool kStaging = true, kEarlyA = false;
     const XentScalars* sc;
     const int* target;
     const int* rows;
@@ -462,7 +470,7 @@ struct HiddenOut {
 template <typename T>
 struct HiddenGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
-    static constexpr bool kStaging = true;
+    static constexpr bool kStaging = true, kEarlyA = false;
     const XentScalars* sc;
     const int* rows;
     float* parts;
@@ -498,8 +506,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 xent_hidden_join_kernel(const XentScalars* __restrict__ sc, const int* __restrict__ rows, const float* __restrict__ parts, const HiddenPlan shape,
                         const HiddenOut<T> out, const int pairs) {
-    cudaGridDependencySynchronize();
-    cudaTriggerProgrammaticLaunchCompletion();
+    chain_begin();
     const int count = sc->count;
     const TilePlan plan = shape.plan(count, pairs);
     if (plan.splits == 1) return;
@@ -524,7 +531,7 @@ xent_hidden_join_kernel(const XentScalars* __restrict__ sc, const int* __restric
 template <typename T>
 struct WeightGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
-    static constexpr bool kStaging = true;
+    static constexpr bool kStaging = true, kEarlyA = false;
     const XentScalars* sc;
     T* out;
     long long ld_out;
@@ -564,9 +571,9 @@ __device__ __forceinline__ MaxSum joined(const MaxSum a, const MaxSum b) {
     return {m, fmaf(a.s, exp2f(fmaf(a.m, kLog2e, -ref)), b.s * exp2f(fmaf(b.m, kLog2e, -ref)))};
 }
 
-// A CTA takes ROWS rows with 256 / ROWS lanes over the vocabulary tiles; the CTA that finishes
-// last adds up the loss.  ROWS is 32 (neighbouring lanes read neighbouring rows), or 1 in a small
-// call, where the number of tiles would make the walk long.
+// A CTA takes ROWS rows with 256 / ROWS lanes over the vocabulary's pieces; the CTA that finishes
+// last adds up the loss.  ROWS is 8 (64 bytes of neighbouring rows; with 32 the walk over the pieces
+// is 4 times as long and took 17 us instead of 9 at 1,640 rows), or 1 in a small call.
 template <int ROWS>
 __global__ void __launch_bounds__(256)
 xent_join_kernel(XentScalars* sc, const float2* __restrict__ stats, const int rows_cap, const int tiles, const float* __restrict__ target_logit,
@@ -591,6 +598,7 @@ xent_join_kernel(XentScalars* sc, const float2* __restrict__ stats, const int ro
         __syncthreads();
         if (y < o) part[y][x] = joined(part[y][x], part[y + o][x]);
     }
+    __syncthreads();
     if (threadIdx.x < 32) {
         float loss = 0.0f;
         if (y == 0 && row < count) {
@@ -848,9 +856,9 @@ static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
         const StatsOps<T> ops{c.sc(), c.target(), stats, (int)s.cap, (int)h->dim, (int)h->vocab, logits_group(h), 0, 0};
         GM_TRY((launch_tiles<kTileN, false, false>(c.d, map_x, map_w, ops, s.cap / kTileM * n_tiles)));
     }
-    // a CTA per row up to a few rows per SM, 32 rows per CTA beyond
-    auto join = h->tokens <= 1024 ? xent_join_kernel<1> : xent_join_kernel<32>;
-    const int64_t ctas = h->tokens <= 1024 ? h->tokens : s.cap / 32;
+    // a CTA per row up to a few rows per SM, 8 rows per CTA beyond
+    auto join = h->tokens <= 1024 ? xent_join_kernel<1> : xent_join_kernel<8>;
+    const int64_t ctas = h->tokens <= 1024 ? h->tokens : s.cap / 8;
     GM_CUDA_CHECK(launch_chained(join, dim3((unsigned)ctas), dim3(256), 0, c.d->stream, c.sc(), stats, (int)s.cap, tiles, target_logit, c.rows(), losses, lse,
                                  (float*)(c.ws + s.partial), total, h->mean, reinterpret_cast<const int*>(c.d->scalars + kXentStatusWord)));
     c.d->launches++;

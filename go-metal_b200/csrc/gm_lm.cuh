@@ -164,6 +164,11 @@ __device__ __forceinline__ void drop8(const Drop& d, const DropOffset& o, const 
     }
 }
 
+__device__ __forceinline__ void chain_begin() {
+    cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
+}
+
 // ---- host side ----
 inline int dtype_bytes(int dtype) { return dtype == GM_F32 ? 4 : dtype == GM_F16 || dtype == GM_BF16 ? 2 : 0; }
 
@@ -180,7 +185,8 @@ int check_matrix(int64_t rows, int64_t cols, int64_t ld, const char* what);
 inline int64_t matrix_bytes(int64_t rows, int64_t cols, int64_t ld, int eb) { return rows > 0 ? ((rows - 1) * ld + cols) * eb : 0; }
 
 // A launch that may begin while the kernel before it in the stream ends (programmatic stream
-// serialization); the kernel calls cudaGridDependencySynchronize() before it touches memory.
+// serialization).  The kernel calls chain_begin() before it touches memory: it waits for the kernel
+// before, and lets the one behind start its own wait.
 template <typename... P, typename... A>
 inline cudaError_t launch_chained(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
     cudaLaunchConfig_t cfg = {};

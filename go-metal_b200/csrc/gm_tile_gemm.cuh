@@ -270,6 +270,8 @@ __device__ __forceinline__ int choose_splits(int tiles, int k_blocks, int pairs,
 // MN_A / MN_B: that operand is MN-major.  Ops provides
 //   kBf16             whether the inputs are bf16 (else fp16)
 //   kStaging          whether the epilogue wants shared memory
+//   kEarlyA           the kernel before this one does not write A, the tiles do not depend on it, and
+//                     shape(pairs) gives them: the copies of A start before that kernel has ended
 //   plan(pairs)       the tiles, read on the device
 //   a0, b0            first row of A and of B (first K-row of an MN-major operand) in their maps
 //   prepare(plan, at, row)   what the epilogue of this turn needs for the row inside the tile, read
@@ -282,6 +284,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Ops ops,
                  int* status, const long long budget) {
     constexpr int kStages = Ring<TN>::kStages, kStageBytes = Ring<TN>::kStageBytes, kRowsB = Ring<TN>::kRowsB;
+    static_assert(!Ops::kEarlyA || !MN_A, "the early copies are of a K-major A");
     static_assert(!MN_B || TN == 256, "an MN-major B comes in two blocks of 64 columns per CTA");
     extern __shared__ unsigned char dyn[];
     __shared__ __align__(8) unsigned long long full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
@@ -300,6 +303,10 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         mbar_init(smem_u32(&drain), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (tid == 64) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+    }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -309,9 +316,21 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     cluster_sync_all();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = tmem_base;
-    // all of the above may run while the kernel before this one ends
-    cudaGridDependencySynchronize();
-    cudaTriggerProgrammaticLaunchCompletion();
+    // All of the above may run while the kernel before this one ends, and so may the first copies of A:
+    // every kernel of the chain lets the next one start only after its own wait, so what lies two
+    // kernels back is complete.
+    unsigned early = 0;
+    if constexpr (Ops::kEarlyA) if (warp == 0 && lane == 0) {
+        const TilePlan plan = ops.shape();
+        if (pair < plan.items()) {
+            const TileAt at = plan.at(pair);
+            for (; early < (unsigned)kStages && at.k0 + (int)early < at.k1; ++early) {
+                if (rank == 0) mbar_expect(smem_u32(&full[early]), 2 * kStageBytes);
+                tma_load(ring + early * kStageBytes, &map_a, (at.k0 + (int)early) * kTileK, ops.a0 + at.m * kTileM + (int)rank * kHalf, pair_leader_addr(smem_u32(&full[early])));
+            }
+        }
+    }
+    chain_begin();
     const TilePlan plan = ops.plan(pairs);
     const int items = plan.items();
 
@@ -327,9 +346,11 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 const unsigned turn = issued / kStages;
                 if (!mbar_wait(smem_u32(&empty[s]), (turn & 1u) ^ 1u, &abort_flag, budget)) { ok = false; break; }
                 const unsigned bar = pair_leader_addr(smem_u32(&full[s]));
-                if (rank == 0) mbar_expect(smem_u32(&full[s]), 2 * kStageBytes);          // both CTAs' copies
+                const bool begun = Ops::kEarlyA && issued < early;                        // A is on its way
+                if (rank == 0 && !begun) mbar_expect(smem_u32(&full[s]), 2 * kStageBytes);   // both CTAs' copies
                 const unsigned a = ring + s * kStageBytes, b = a + kOperandBytes;
-                if (MN_A) {
+                if (begun) {
+                } else if (MN_A) {
                     tma_load(a, &map_a, row_a, ops.a0 + k * kTileK, bar);
                     tma_load(a + 8192, &map_a, row_a + 64, ops.a0 + k * kTileK, bar);
                 } else {
