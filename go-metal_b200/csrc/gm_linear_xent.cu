@@ -241,7 +241,9 @@ struct Goal { int at; };        // a row's target
 template <typename T>
 struct StatsOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
-    static constexpr bool kStaging = false, kEarlyA = false;
+    static constexpr bool kStaging = false;
+    __device__ __forceinline__ void begin() const {}
+    __device__ __forceinline__ int rows_a() const { return kHalf; }
     const XentScalars* sc;
     const int* target;
     float2* stats;               // [128 vocabulary entries][row]
@@ -284,10 +286,12 @@ struct StatsOps {
     }
 };
 
-// The same for a few rows (at most TN): the vocabulary takes the tile's long side, 256 entries by
-// TN rows, so that nothing but the read of W is left.  A warp holds 32 entries of 32 rows at a
-// time, one entry per lane, and reduces over its lanes by halving exchanges, after which lane j
-// has row j: one {maximum, sum} per 32 entries and row.
+// The same for a few rows (at most TN): the vocabulary takes the tile's long side, up to 256 entries by
+// TN rows, so that nothing but the read of W is left.  `height` entries per CTA are chosen so that
+// all pairs have the same share of the vocabulary.  Rows without a target are multiplied like the
+// others, and nothing reads what comes of them.  A warp holds 32 entries of 32 rows at a time, one
+// entry per lane, and reduces over its lanes by halving exchanges, after which lane j has row j: one
+// {maximum, sum} per warp and row.
 template <bool MAX> __device__ __forceinline__ float lanes_to_columns(float (&v)[32], int lane) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -305,36 +309,35 @@ template <bool MAX> __device__ __forceinline__ float lanes_to_columns(float (&v)
 template <typename T, int TN>
 struct FewStatsOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
-    static constexpr bool kStaging = false, kEarlyA = true;
-    const XentScalars* sc;
-    const int* target;
-    float2* stats;               // [32 vocabulary entries][row]
-    int rows_cap, dim, vocab, a0, b0;
-    // one column of tiles, also where no row has a target: then the epilogue writes nothing
-    __device__ __forceinline__ TilePlan shape() const { return {0, (vocab + kTileM - 1) / kTileM, 1, (dim + kTileK - 1) / kTileK, 1, 1}; }
+    static constexpr bool kStaging = false;
+    static constexpr int kColumns = TN / 2 < 32 ? 32 : TN / 2;
+    XentScalars* sc;
+    const int* target;           // by row of the caller
+    float2* stats;               // [warp's share of a tile][row]
+    int n, rows_cap, dim, vocab, height, a0, b0;
+    __device__ __forceinline__ void begin() const { sc->ticket = 0u; }
+    __device__ __forceinline__ int rows_a() const { return height; }
     __device__ __forceinline__ TilePlan plan(int) const {
-        TilePlan p = shape();
-        p.count = sc->count;
-        return p;
+        return {n, (vocab + 2 * height - 1) / (2 * height), 1, (dim + kTileK - 1) / kTileK, 1, 1};
     }
     __device__ __forceinline__ Goal prepare(const TilePlan&, const TileAt&, int) const { return {0}; }
-    static constexpr int kColumns = TN / 2 < 32 ? 32 : TN / 2;
-    __device__ __forceinline__ void epilogue(const TilePlan& plan, const TileAt& tile, int in_tile, float (&all)[kColumns], int half, unsigned,
-                                             const Goal) const {
-        const int entry = tile.m * kTileM + in_tile, lane = threadIdx.x & 31;
-        const int count = plan.count;
-        if (entry - lane >= vocab || half * kColumns >= TN) return;     // the whole warp is behind the table, or has no columns
+    __device__ __forceinline__ void epilogue(const TilePlan&, const TileAt& tile, int in_tile, float (&all)[kColumns], int half, unsigned, const Goal) const {
+        const int cta = in_tile / kHalf, local = in_tile % kHalf, lane = threadIdx.x & 31;
+        const int base = (tile.m * 2 + cta) * height + (local & ~31);      // entry of the warp's first lane
+        const bool real = local < height && base + lane < vocab;
+        if (half * kColumns >= TN) return;
+        float2* to = stats + (long long)(tile.m * 8 + in_tile / 32) * rows_cap;
 #pragma unroll
         for (int q = 0; q < kColumns; q += 32) {
             const int c = half * kColumns + q;
-            if (c >= count) break;
+            if (c >= n) break;
             float v[32], w[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = entry < vocab ? all[q + j] : -INFINITY;
-            const int goal = c + lane < count ? __ldg(target + c + lane) : -1;
-            for (unsigned hits = __ballot_sync(0xffffffffu, goal >= entry - lane && goal < entry - lane + 32); hits; hits &= hits - 1) {
+            for (int j = 0; j < 32; ++j) v[j] = real ? all[q + j] : -INFINITY;
+            const int goal = c + lane < n ? __ldg(target + c + lane) : -1;
+            for (unsigned hits = __ballot_sync(0xffffffffu, goal >= base && goal < base + 32); hits; hits &= hits - 1) {
                 const int j = __ffs((int)hits) - 1;
-                const bool mine = __shfl_sync(0xffffffffu, goal, j) == entry;
+                const bool mine = __shfl_sync(0xffffffffu, goal, j) == base + lane;
 #pragma unroll
                 for (int k = 0; k < 32; ++k)
                     if (k == j && mine) v[k] = -INFINITY;              // the target's logit is added by itself
@@ -346,7 +349,7 @@ struct FewStatsOps {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -__shfl_sync(0xffffffffu, ref, j)));
             const float sum = lanes_to_columns<false>(v, lane);
-            if (c + lane < count) stats[(long long)(entry >> 5) * rows_cap + c + lane] = make_float2(top, sum);
+            if (c + lane < n) to[c + lane] = make_float2(top, sum);
         }
     }
 };
@@ -355,7 +358,9 @@ struct FewStatsOps {
 template <typename T>
 struct SoftmaxGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
-    static constexpr bool kStaging = true, kEarlyA = false;
+    static constexpr bool kStaging = true;
+    __device__ __forceinline__ void begin() const {}
+    __device__ __forceinline__ int rows_a() const { return kHalf; }
     const XentScalars* sc;
     const int* target;
     const int* rows;
@@ -470,7 +475,9 @@ struct HiddenOut {
 template <typename T>
 struct HiddenGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
-    static constexpr bool kStaging = true, kEarlyA = false;
+    static constexpr bool kStaging = true;
+    __device__ __forceinline__ void begin() const {}
+    __device__ __forceinline__ int rows_a() const { return kHalf; }
     const XentScalars* sc;
     const int* rows;
     float* parts;
@@ -531,7 +538,9 @@ xent_hidden_join_kernel(const XentScalars* __restrict__ sc, const int* __restric
 template <typename T>
 struct WeightGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
-    static constexpr bool kStaging = true, kEarlyA = false;
+    static constexpr bool kStaging = true;
+    __device__ __forceinline__ void begin() const {}
+    __device__ __forceinline__ int rows_a() const { return kHalf; }
     const XentScalars* sc;
     T* out;
     long long ld_out;
@@ -628,6 +637,79 @@ xent_join_kernel(XentScalars* sc, const float2* __restrict__ stats, const int ro
         total[1] = (float)count;
         sc->ticket = 0u;
     }
+}
+
+// A few rows: a CTA per row takes the target's logit while the product still runs (it reads only what
+// the caller gave), then joins the row's statistics; the last one adds up the loss.
+template <typename T>
+__global__ void __launch_bounds__(256)
+xent_few_join_kernel(XentScalars* sc, const T* __restrict__ hidden, const long long ld, const T* __restrict__ weight, const long long ld_weight,
+                     const int* __restrict__ targets, const int dim, const int vocab, const float2* __restrict__ stats, const int rows_cap, const int pieces,
+                     float* __restrict__ losses, float* __restrict__ lse, float* partial, float* __restrict__ total, const int mean, const int* status) {
+    __shared__ MaxSum part[256];
+    __shared__ float dots[8];
+    __shared__ int is_last;
+    const int row = blockIdx.x, n = gridDim.x, tid = threadIdx.x;
+    const int goal = __ldg(targets + row);
+    const bool live = goal >= 0 && goal < vocab;
+    float z = 0.0f;
+    if (live) {
+        const T *x = hidden + row * ld, *w = weight + goal * ld_weight;
+        for (int c = tid; c < dim; c += 256) z = fmaf(to_f32<T>(x[c]), to_f32<T>(w[c]), z);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    if ((tid & 31) == 0) dots[tid >> 5] = z;
+    chain_begin();
+    MaxSum a = {-INFINITY, 0.0f};
+    if (live)
+        for (int t = tid; t < pieces; t += 256) {
+            const float2 p = __ldcs(stats + (long long)t * rows_cap + row);
+            a = joined(a, {p.x, p.y});
+        }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a = joined(a, {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
+    if ((tid & 31) == 0) part[tid >> 5] = a;
+    __syncthreads();
+    if (tid == 0) {
+        float loss = 0.0f, l = 0.0f;
+        if (live) {
+            z = dots[0];
+            for (int k = 1; k < 8; ++k) { z += dots[k]; a = joined(a, part[k]); }
+            loss = z >= a.m ? log1pf(a.s * expf(a.m - z)) : (a.m - z) + logf(a.s + expf(z - a.m));
+            l = z + loss;
+        }
+        losses[row] = loss;
+        lse[row] = l;
+        partial[row] = loss;
+        __threadfence();
+        is_last = atomicAdd(&sc->ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!is_last || tid >= 32) return;
+    __threadfence();
+    double sum = 0.0;
+    int count = 0;
+    for (int r = tid; r < n; r += 32) {
+        const int t = __ldg(targets + r);
+        sum += (double)((volatile float*)partial)[r];
+        count += t >= 0 && t < vocab;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { sum += __shfl_xor_sync(0xffffffffu, sum, o); count += __shfl_xor_sync(0xffffffffu, count, o); }
+    if (tid == 0) {
+        if (*status) sum = NAN;
+        total[0] = (float)(mean && count > 0 ? sum / count : sum);
+        total[1] = (float)count;
+    }
+}
+
+// Rows that TMA cannot read in place (their address or stride is not a multiple of 16 bytes).
+template <typename T>
+__global__ void __launch_bounds__(256)
+xent_copy_kernel(const T* __restrict__ hidden, const long long ld, const int dim, T* __restrict__ packed, const long long ld_packed) {
+    chain_begin();
+    for (int c = threadIdx.x; c < dim; c += 256) packed[blockIdx.x * ld_packed + c] = hidden[blockIdx.x * ld + c];
 }
 
 // ---------------------------------------------------------------- host side
@@ -737,7 +819,9 @@ static XentSpace common_space(const gm_linear_xent_t* h) {
 static XentSpace forward_space(const gm_linear_xent_t* h) {
     XentSpace s = common_space(h);
     s.stats = s.total;
-    const int64_t stat_tiles = h->tokens <= kFewRows ? (h->vocab + 31) / 32 : (h->vocab + kTileN / 2 - 1) / (kTileN / 2);
+    // a few rows: eight pieces per tile of at least 16 entries, and no more tiles than rounds of half the SMs
+    const int64_t few_tiles = (h->vocab + 15) / 16 < 1024 ? (h->vocab + 15) / 16 : 1024 + (h->vocab + 127) / 128;
+    const int64_t stat_tiles = h->tokens <= kFewRows ? few_tiles * 8 : (h->vocab + kTileN / 2 - 1) / (kTileN / 2);
     s.target_logit = s.stats + up256(stat_tiles * s.cap * 8);
     s.partial = s.target_logit + up256(s.cap * 4);
     s.total = s.partial + up256(s.cap * 4);
@@ -824,38 +908,51 @@ static int index_and_gather(const XentCall& c, uintptr_t hidden, uintptr_t targe
     return GM_OK;
 }
 
-// The logits of a few rows, 256 vocabulary entries by TN rows to a tile.
+// A few rows: one product that reads W once, and the kernel that joins.
 template <typename T, int TN>
-static int few_logits(const XentCall& c, const CUtensorMap& map_w, float2* stats) {
+static int forward_few(const XentCall& c, uintptr_t hidden, uintptr_t weight, uintptr_t targets, float* losses, float* lse, float* total) {
     const gm_linear_xent_t* h = c.h;
-    CUtensorMap map_x;
-    GM_TRY(make_map(&map_x, h->dtype, c.ws + c.s.packed, c.s.cap, h->dim, c.s.ld_packed, TN / 2));
-    const FewStatsOps<T, TN> ops{c.sc(), c.target(), stats, (int)c.s.cap, (int)h->dim, (int)h->vocab, 0, 0};
-    return launch_tiles<TN, false, false>(c.d, map_w, map_x, ops, (h->vocab + kTileM - 1) / kTileM);
+    const XentSpace& s = c.s;
+    const bool in_place = hidden % 16 == 0 && h->ld_hidden % 8 == 0;
+    const uintptr_t x = in_place ? hidden : c.ws + s.packed;
+    // entries per CTA and tile: the rounds that 128 would take, evenly filled
+    const int64_t ctas = c.d->sm_count / 2 * 2, rounds = (h->vocab + kHalf * ctas - 1) / (kHalf * ctas);
+    const int height = (int)(((h->vocab + rounds * ctas - 1) / (rounds * ctas) + 7) / 8 * 8);
+    const int64_t tiles = (h->vocab + 2 * height - 1) / (2 * height);
+    CUtensorMap map_w, map_x;
+    GM_TRY(make_map(&map_w, h->dtype, weight, h->vocab, h->dim, h->ld_weight, height));
+    GM_TRY(make_map(&map_x, h->dtype, x, h->tokens, h->dim, in_place ? h->ld_hidden : s.ld_packed, TN / 2));
+    if (!in_place) {
+        GM_CUDA_CHECK(launch_chained(xent_copy_kernel<T>, dim3((unsigned)h->tokens), dim3(256), 0, c.d->stream, (const T*)hidden, h->ld_hidden, (int)h->dim,
+                                     (T*)x, s.ld_packed));
+        c.d->launches++;
+    }
+    float2* stats = (float2*)(c.ws + s.stats);
+    const FewStatsOps<T, TN> ops{c.sc(), (const int*)targets, stats, (int)h->tokens, (int)s.cap, (int)h->dim, (int)h->vocab, height, 0, 0};
+    GM_TRY((launch_tiles<TN, false, false>(c.d, map_w, map_x, ops, tiles)));
+    GM_CUDA_CHECK(launch_chained(xent_few_join_kernel<T>, dim3((unsigned)h->tokens), dim3(256), 0, c.d->stream, c.sc(), (const T*)hidden, h->ld_hidden,
+                                 (const T*)weight, h->ld_weight, (const int*)targets, (int)h->dim, (int)h->vocab, stats, (int)s.cap, (int)tiles * 8, losses, lse,
+                                 (float*)(c.ws + s.partial), total, h->mean, reinterpret_cast<const int*>(c.d->scalars + kXentStatusWord)));
+    c.d->launches++;
+    return GM_OK;
 }
 
 template <typename T>
 static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, uintptr_t targets, float* losses, float* lse, float* total) {
     const gm_linear_xent_t* h = c.h;
     const XentSpace& s = c.s;
-    CUtensorMap map_w;
+    if (h->tokens <= 32) return forward_few<T, 32>(c, hidden, weight, targets, losses, lse, total);
+    if (h->tokens <= kFewRows) return forward_few<T, kFewRows>(c, hidden, weight, targets, losses, lse, total);
+    CUtensorMap map_w, map_x;
     GM_TRY(make_map(&map_w, h->dtype, weight, h->vocab, h->dim, h->ld_weight, kHalf));
+    GM_TRY(make_map(&map_x, h->dtype, c.ws + s.packed, s.cap, h->dim, s.ld_packed, kHalf));
     float* target_logit = (float*)(c.ws + s.target_logit);
     GM_TRY(index_and_gather<T>(c, hidden, targets, weight, target_logit, losses, lse, (T*)nullptr));
     float2* stats = (float2*)(c.ws + s.stats);
-    const bool few = h->tokens <= kFewRows;
     const int64_t n_tiles = (h->vocab + kTileN - 1) / kTileN;
-    int tiles = (int)((h->vocab + kTileN / 2 - 1) / (kTileN / 2));
-    if (few) {
-        tiles = (int)((h->vocab + 31) / 32);
-        if (h->tokens <= 32) GM_TRY((few_logits<T, 32>(c, map_w, stats)));
-        else GM_TRY((few_logits<T, kFewRows>(c, map_w, stats)));
-    } else {
-        CUtensorMap map_x;
-        GM_TRY(make_map(&map_x, h->dtype, c.ws + s.packed, s.cap, h->dim, s.ld_packed, kHalf));
-        const StatsOps<T> ops{c.sc(), c.target(), stats, (int)s.cap, (int)h->dim, (int)h->vocab, logits_group(h), 0, 0};
-        GM_TRY((launch_tiles<kTileN, false, false>(c.d, map_x, map_w, ops, s.cap / kTileM * n_tiles)));
-    }
+    const int tiles = (int)((h->vocab + kTileN / 2 - 1) / (kTileN / 2));
+    const StatsOps<T> ops{c.sc(), c.target(), stats, (int)s.cap, (int)h->dim, (int)h->vocab, logits_group(h), 0, 0};
+    GM_TRY((launch_tiles<kTileN, false, false>(c.d, map_x, map_w, ops, s.cap / kTileM * n_tiles)));
     // a CTA per row up to a few rows per SM, 8 rows per CTA beyond
     auto join = h->tokens <= 1024 ? xent_join_kernel<1> : xent_join_kernel<8>;
     const int64_t ctas = h->tokens <= 1024 ? h->tokens : s.cap / 8;

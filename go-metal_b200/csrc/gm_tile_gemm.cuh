@@ -270,8 +270,9 @@ __device__ __forceinline__ int choose_splits(int tiles, int k_blocks, int pairs,
 // MN_A / MN_B: that operand is MN-major.  Ops provides
 //   kBf16             whether the inputs are bf16 (else fp16)
 //   kStaging          whether the epilogue wants shared memory
-//   kEarlyA           the kernel before this one does not write A, the tiles do not depend on it, and
-//                     shape(pairs) gives them: the copies of A start before that kernel has ended
+//   begin()           run by one thread before anything else
+//   rows_a()          rows of A per CTA, 128 or a smaller multiple of 8 (K-major A only); the box of
+//                     its map has as many, the accumulators' other rows hold anything
 //   plan(pairs)       the tiles, read on the device
 //   a0, b0            first row of A and of B (first K-row of an MN-major operand) in their maps
 //   prepare(plan, at, row)   what the epilogue of this turn needs for the row inside the tile, read
@@ -284,7 +285,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
 tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Ops ops,
                  int* status, const long long budget) {
     constexpr int kStages = Ring<TN>::kStages, kStageBytes = Ring<TN>::kStageBytes, kRowsB = Ring<TN>::kRowsB;
-    static_assert(!Ops::kEarlyA || !MN_A, "the early copies are of a K-major A");
     static_assert(!MN_B || TN == 256, "an MN-major B comes in two blocks of 64 columns per CTA");
     extern __shared__ unsigned char dyn[];
     __shared__ __align__(8) unsigned long long full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
@@ -316,21 +316,9 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     cluster_sync_all();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = tmem_base;
-    // All of the above may run while the kernel before this one ends, and so may the first copies of A:
-    // every kernel of the chain lets the next one start only after its own wait, so what lies two
-    // kernels back is complete.
-    unsigned early = 0;
-    if constexpr (Ops::kEarlyA) if (warp == 0 && lane == 0) {
-        const TilePlan plan = ops.shape();
-        if (pair < plan.items()) {
-            const TileAt at = plan.at(pair);
-            for (; early < (unsigned)kStages && at.k0 + (int)early < at.k1; ++early) {
-                if (rank == 0) mbar_expect(smem_u32(&full[early]), 2 * kStageBytes);
-                tma_load(ring + early * kStageBytes, &map_a, (at.k0 + (int)early) * kTileK, ops.a0 + at.m * kTileM + (int)rank * kHalf, pair_leader_addr(smem_u32(&full[early])));
-            }
-        }
-    }
+    // all of the above may run while the kernel before this one ends
     chain_begin();
+    if (blockIdx.x == 0 && tid == 0) ops.begin();
     const TilePlan plan = ops.plan(pairs);
     const int items = plan.items();
 
@@ -338,19 +326,20 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     if (warp == 0 && lane == 0) {
         // ---- copies ----
         bool ok = true;
+        const int rows_a = ops.rows_a();
+        const unsigned bytes = 2u * (unsigned)(rows_a + kRowsB) * (kTileK * 2);              // both CTAs' copies
+
         for (int t = pair; t < items && ok; t += pairs) {
             const TileAt at = plan.at(t);
-            const int row_a = at.m * kTileM + (int)rank * kHalf, row_b = at.n * TN + (int)rank * kRowsB;
+            const int row_a = (at.m * 2 + (int)rank) * rows_a, row_b = at.n * TN + (int)rank * kRowsB;
             for (int k = at.k0; k < at.k1; ++k, ++issued) {
                 const int s = issued % kStages;
                 const unsigned turn = issued / kStages;
                 if (!mbar_wait(smem_u32(&empty[s]), (turn & 1u) ^ 1u, &abort_flag, budget)) { ok = false; break; }
                 const unsigned bar = pair_leader_addr(smem_u32(&full[s]));
-                const bool begun = Ops::kEarlyA && issued < early;                        // A is on its way
-                if (rank == 0 && !begun) mbar_expect(smem_u32(&full[s]), 2 * kStageBytes);   // both CTAs' copies
+                if (rank == 0) mbar_expect(smem_u32(&full[s]), bytes);
                 const unsigned a = ring + s * kStageBytes, b = a + kOperandBytes;
-                if (begun) {
-                } else if (MN_A) {
+                if (MN_A) {
                     tma_load(a, &map_a, row_a, ops.a0 + k * kTileK, bar);
                     tma_load(a + 8192, &map_a, row_a + 64, ops.a0 + k * kTileK, bar);
                 } else {
