@@ -225,46 +225,57 @@ __device__ __forceinline__ void rows_by_fours(unsigned stage, const float (&v)[1
     }
 }
 
-// The work of one turn: a tile, its share of K, and the turn's number.
-struct TileAt { int m, n, split, item, k0, k1; };
+// The work of one turn: a tile, its share of K, and the part it leaves (-1: the whole tile).
+struct TileAt { int m, n, part, k0, k1; };
 
 // One product: m_tiles x n_tiles tiles, walked m first inside groups of `group` m-tiles, so that
-// the operands of the tiles in flight are shared in L2; each tile in `splits` shares of K.
+// the operands of the tiles in flight are shared in L2.  The first `whole` tiles are a turn each, the
+// others `splits` turns, each with a share of K.
 struct TilePlan {
     int count;                                                // rows with a target
-    int m_tiles, n_tiles, k_blocks, group, splits;
-    __device__ __forceinline__ int items() const { return m_tiles * n_tiles * splits; }
-    __device__ __forceinline__ TileAt at(int item) const {
-        TileAt x;
-        const int t = item / splits, per = group * n_tiles;
-        const int g = t / per, m0 = g * group;
+    int m_tiles, n_tiles, k_blocks, group, whole, splits;
+    __device__ __forceinline__ int tiles() const { return m_tiles * n_tiles; }
+    __device__ __forceinline__ int items() const { return whole + (tiles() - whole) * splits; }
+    __device__ __forceinline__ void place(int tile, int* m, int* n) const {
+        const int per = group * n_tiles, g = tile / per, m0 = g * group;
         const int high = m_tiles - m0 < group ? m_tiles - m0 : group;
-        const int r = t - g * per;
-        x.item = item;
-        x.n = r / high;
-        x.m = m0 + (r - x.n * high);
-        x.split = item - t * splits;
-        x.k0 = (int)((long long)k_blocks * x.split / splits);
-        x.k1 = (int)((long long)k_blocks * (x.split + 1) / splits);
-        return x;
+        const int r = tile - g * per;
+        *n = r / high;
+        *m = m0 + (r - *n * high);
     }
-    // the inverse: the turn that has the first share of tile (m, n)
-    __device__ __forceinline__ int item_of(int m, int n) const {
-        const int m0 = m / group * group;
-        const int high = m_tiles - m0 < group ? m_tiles - m0 : group;
-        return (m0 * n_tiles + n * high + (m - m0)) * splits;
+    __device__ __forceinline__ TileAt at(int item) const {
+        TileAt x{0, 0, -1, 0, k_blocks};
+        int tile = item;
+        if (item >= whole) {
+            x.part = item - whole;
+            tile = whole + x.part / splits;
+            const int share = x.part % splits;
+            x.k0 = (int)((long long)k_blocks * share / splits);
+            x.k1 = (int)((long long)k_blocks * (share + 1) / splits);
+        }
+        place(tile, &x.m, &x.n);
+        return x;
     }
 };
 
-// Shares of K per tile, at most 16 and `most_items` in all, for the shortest run on `pairs` CTA
-// pairs: rounds of turns, each as long as its k-blocks plus a start and an epilogue (about eight).
-__device__ __forceinline__ int choose_splits(int tiles, int k_blocks, int pairs, int most_items) {
-    int best = 1, best_cost = 0x7fffffff;
-    for (int s = 1; s <= 16 && s <= k_blocks && (s == 1 || tiles * s <= most_items); ++s) {
-        const int cost = (tiles * s + pairs - 1) / pairs * ((k_blocks + s - 1) / s + 8) + (s > 1 ? 8 : 0);
-        if (cost < best_cost) { best_cost = cost; best = s; }
-    }
-    return best;
+// A plan without shares of K.
+__device__ __forceinline__ TilePlan whole_tiles(int count, int m_tiles, int n_tiles, int k_blocks, int group) {
+    return {count, m_tiles, n_tiles, k_blocks, group, m_tiles * n_tiles, 1};
+}
+
+// Splits the tiles behind the last full round of `pairs` (or of the round before, too), into at
+// most 16 shares each and `most_parts` in all, for the shortest run: rounds of turns, each as long as
+// its k-blocks plus a start and an epilogue (about eight).
+__device__ __forceinline__ void split_tail(TilePlan* p, int pairs, int most_parts) {
+    const int tiles = p->tiles(), k = p->k_blocks;
+    p->whole = tiles;
+    p->splits = 1;
+    int best = (tiles + pairs - 1) / pairs * (k + 8);
+    for (int tail = tiles % pairs; tail <= tiles && tail <= tiles % pairs + pairs; tail += pairs)
+        for (int s = 2; s <= 16 && s <= k && tail * s <= most_parts; ++s) {
+            const int cost = (tiles - tail) / pairs * (k + 8) + (tail * s + pairs - 1) / pairs * ((k + s - 1) / s + 8) + 8;
+            if (tail > 0 && cost < best) { best = cost; p->whole = tiles - tail; p->splits = s; }
+        }
 }
 
 // MN_A / MN_B: that operand is MN-major.  Ops provides
