@@ -425,6 +425,57 @@ def workload_small(gm, dev, torch, reps):
     return out
 
 
+def workload_lm(gm, dev, torch, reps):
+    """A tied language model's two ends and its optimizer step in one chain on the device's stream:
+    8,192 tokens, 1,024 columns, 50,257 vocabulary rows, fp16 with a device-resident loss scale.
+    Lookup with dropout, vocabulary loss, both gradients into the table's one fp16 gradient, mixed
+    Adam on it.  All operands together are larger than L2."""
+    L = gm.lib
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(SEED + 60)
+    n, dim, vocab = 8192, 1024, 50257
+    P = lambda t: t.data_ptr()
+    master = torch.empty(vocab, dim, device="cuda").normal_(0.0, 0.02, generator=gen)
+    m, v = torch.zeros_like(master), torch.zeros_like(master)
+    table, grad = master.half(), torch.empty(vocab, dim, dtype=torch.float16, device="cuda")
+    tok = torch.randint(0, vocab, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    goal = torch.randint(0, vocab, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    hidden = torch.empty(n, dim, dtype=torch.float16, device="cuda")
+    dhidden = torch.empty_like(hidden)
+    losses, lse, total = (torch.empty(k, device="cuda") for k in (n, n, 2))
+    e = gm.Embedding(dtype=gm.F16, tokens=n, dim=dim, vocab=vocab, ld_table=dim, ld_out=dim, padding_token=-1, scale=32.0)
+    x = gm.LinearXent(dtype=gm.F16, tokens=n, dim=dim, vocab=vocab, ld_hidden=dim, ld_weight=dim, mean=1)
+    room = torch.empty(max(L.gm_embedding_workspace_bytes(e), L.gm_linear_xent_workspace_bytes(x, 1)), dtype=torch.uint8, device="cuda")
+    drop = gm.dropout(0.1, SEED)
+    lst = dev.tensor_list([[P(grad)], [P(master)], [P(m)], [P(v)], [P(table)]], [vocab * dim], [2, 4, 4, 4, 2])
+    mixed = L.gm_mixed_create(dev.h, None, B1, B2, 0)
+    torch.cuda.synchronize()
+    parts = {
+        "embedding_forward": lambda: L.gm_embedding_forward_async(dev.h, e, P(table), P(tok), P(hidden), drop),
+        "loss_forward": lambda: L.gm_linear_xent_forward_async(dev.h, x, P(hidden), P(table), P(goal), P(losses), P(lse), P(total), P(room), room.numel()),
+        "loss_backward": lambda: L.gm_linear_xent_backward_async(dev.h, x, P(hidden), P(table), P(goal), P(lse), L.gm_mixed_state_device_ptr(mixed), 1.0,
+                                                                 P(dhidden), P(grad), 0, P(room), room.numel()),
+        "embedding_backward": lambda: L.gm_embedding_backward_async(dev.h, e, P(tok), P(dhidden), drop, P(grad), gm.F16, 1, P(room), room.numel()),
+        "mixed_adam": lambda: L.gm_mixed_step_async(dev.h, mixed, lst, LR, EPS, 0.0),
+    }
+
+    def one():
+        for name, call in parts.items():
+            gm.check(call(), name)
+
+    one()
+    dev.sync()
+    # each part again on what the step left: the same work, apart from the lookup's accumulation
+    out = {"name": "tied language model ends + mixed Adam", "tokens": n, "dim": dim, "vocab": vocab, "dtype": "fp16",
+           "ms_per_step": _event_timed(gm, dev, one, max(reps, 10)),
+           "ms_by_part": {name: _event_timed(gm, dev, call, max(reps, 10)) for name, call in parts.items()},
+           "loss_tflop_per_step": 8e-12 * n * dim * vocab}
+    gm.check(L.gm_linear_xent_status(dev.h), "loss products")
+    L.gm_mixed_destroy(mixed)
+    L.gm_tensor_list_destroy(lst)
+    return out
+
+
 def run_only(args):
     """Profiler captures: one of the other configurations alone, a few repetitions, one JSON line."""
     import torch
@@ -435,7 +486,8 @@ def run_only(args):
     dev = gm.Device(0)
     peak, _ = measured_peak_gbs()
     fn = {"mixed": workload_mixed, "mixed_clip": lambda *a: workload_mixed(*a, clip=True), "lbfgs": workload_lbfgs,
-          "rules": workload_rules, "small": lambda gm_, dev_, torch_, peak_, reps_: workload_small(gm_, dev_, torch_, reps_)}[args.only]
+          "rules": workload_rules, "small": lambda gm_, dev_, torch_, peak_, reps_: workload_small(gm_, dev_, torch_, reps_),
+          "lm": lambda gm_, dev_, torch_, peak_, reps_: workload_lm(gm_, dev_, torch_, reps_)}[args.only]
     out = fn(gm, dev, torch, peak, max(args.steps, 1))
     dev.close()
     print(json.dumps({"only": args.only, "result": out}))
@@ -977,7 +1029,7 @@ def main():
     ap.add_argument("--skip-e2e", action="store_true", help="profiling runs: leave out the host-buffer leg")
     ap.add_argument("--tensors", type=int, default=256,
                     help="profiling runs only: fewer 4 Mi tensors than the 256 of the workload")
-    ap.add_argument("--only", choices=["mixed", "mixed_clip", "lbfgs", "rules", "small"],
+    ap.add_argument("--only", choices=["mixed", "mixed_clip", "lbfgs", "rules", "small", "lm"],
                     help="profiling runs only: time one of the other configurations alone for --steps repetitions")
     args = ap.parse_args()
     if args.impl == "reference":
