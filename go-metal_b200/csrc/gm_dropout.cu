@@ -34,8 +34,8 @@ int check_buffer(const Device* d, uintptr_t p, int64_t need, int64_t align, cons
 }
 
 int check_matrix(int64_t rows, int64_t cols, int64_t ld, const char* what) {
-    if (rows <= 0 || cols <= 0 || rows > 0x7fffffffLL || cols > 0x7fffffffLL) {
-        set_error("%s: size %lld x %lld is outside [1, 2^31)", what, (long long)rows, (long long)cols);
+    if (rows <= 0 || cols <= 0 || rows > 0x7fffffffLL || cols > (1LL << 30)) {
+        set_error("%s: size %lld x %lld is outside [1, 2^31) x [1, 2^30]", what, (long long)rows, (long long)cols);
         return GM_ERR_BAD_SIZE;
     }
     if (ld > 0x7fffffffLL) { set_error("%s: row stride %lld is outside [1, 2^31)", what, (long long)ld); return GM_ERR_BAD_SIZE; }

@@ -714,6 +714,20 @@ xent_copy_kernel(const T* __restrict__ hidden, const long long ld, const int dim
     for (int c = threadIdx.x; c < dim; c += 256) packed[blockIdx.x * ld_packed + c] = hidden[blockIdx.x * ld + c];
 }
 
+// Self-check: the products' wait on a barrier that nothing arrives at.
+__global__ void xent_timeout_kernel(int* status, const long long budget, int* gave_up) {
+    __shared__ __align__(8) unsigned long long bar;
+    __shared__ volatile int abort_flag;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        mbar_init(smem_u32(&bar), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        const bool done = mbar_wait(smem_u32(&bar), 0, &abort_flag, budget);
+        if (abort_flag) *status = 1;
+        *gave_up = !done && abort_flag;
+    }
+}
+
 // ---------------------------------------------------------------- host side
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1066,6 +1080,20 @@ int gm_linear_xent_backward_async(uintptr_t device_ptr, const gm_linear_xent_t* 
     if (h->dtype == GM_F16)
         return run_backward<__half>(c, hidden, weight, targets, (const float*)lse, (const float*)scale_device, grad_scale, dhidden, dweight, accumulate != 0);
     return run_backward<__nv_bfloat16>(c, hidden, weight, targets, (const float*)lse, (const float*)scale_device, grad_scale, dhidden, dweight, accumulate != 0);
+}
+
+int gm_selftest_xent_timeout(uintptr_t device_ptr, long long budget_cycles, int* gave_up) {
+    Device* d = as_device(device_ptr);
+    if (!d) return GM_ERR_NIL_DEVICE;
+    if (!gave_up || budget_cycles <= 0) { set_error("bad self-check arguments"); return GM_ERR_BAD_ARG; }
+    DeviceGuard g(d);
+    int* words = reinterpret_cast<int*>(d->scalars + kXentStatusWord);       // the status, and a word for the answer
+    xent_timeout_kernel<<<1, 32, 0, d->stream>>>(words, budget_cycles, words + 1);
+    d->launches++;
+    GM_CUDA_CHECK(cudaGetLastError());
+    GM_CUDA_CHECK(cudaStreamSynchronize(d->stream));
+    GM_CUDA_CHECK(cudaMemcpy(gave_up, words + 1, sizeof(int), cudaMemcpyDeviceToHost));
+    return GM_OK;
 }
 
 int gm_linear_xent_status(uintptr_t device_ptr) {

@@ -166,6 +166,7 @@ _SIGS = {
     "gm_zero1_mixed_push_step_async": (i, [u, u, u, f, f, f]),
     "gm_selftest_const_div": (i, [u, f, C.POINTER(C.c_uint64), C.POINTER(C.c_uint32), ip]),
     "gm_selftest_barrier_timeout": (i, [u, C.c_longlong, ip]),
+    "gm_selftest_xent_timeout": (i, [u, C.c_longlong, ip]),
     "gm_device_set_tuning": (i, [u, C.c_char_p, C.c_longlong]),
     "gm_device_get_tuning": (C.c_longlong, [u, C.c_char_p]),
     "gm_timer_start": (i, [u]),

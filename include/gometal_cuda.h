@@ -335,7 +335,7 @@ int gm_dot_canonical_static(uintptr_t a, uintptr_t b, int64_t n, uintptr_t out_d
  * captured into a graph (on gm_device_stream).  Workspaces are the caller's, 256-byte aligned,
  * and hold nothing between calls; two calls or captured graphs that can run at the same
  * time need workspaces of their own.  Matrices are row-major with a row stride (ld, in
- * elements) of at least their columns.  Buffers are read and written only inside the
+ * elements) of at least their columns, below 2^31 rows and at most 2^30 columns.  Buffers are read and written only inside the
  * rows and columns named. */
 
 /* Element types: the codes of memory/tensor.go:12-17, and one more for bfloat16. */
@@ -495,6 +495,11 @@ int gm_selftest_const_div(uintptr_t device_ptr, float c, uint64_t* mismatches, u
  * budget_cycles GPU clock cycles: it must return with *gave_up == 1 and leave the device
  * usable (a step whose barrier gives up reports GM_ERR_TIMEOUT). */
 int gm_selftest_barrier_timeout(uintptr_t device_ptr, long long budget_cycles, int* gave_up);
+
+/* The same for the products of the vocabulary loss: runs their bounded wait on a barrier that
+ * nothing arrives at.  *gave_up must be 1; afterwards a forward pass reports NaN as its total and
+ * gm_linear_xent_status returns GM_ERR_TIMEOUT once, as after a product whose wait ran out. */
+int gm_selftest_xent_timeout(uintptr_t device_ptr, long long budget_cycles, int* gave_up);
 
 /* ---- timing on the device's stream (CUDA events) ---- */
 int gm_timer_start(uintptr_t device_ptr);                  /* records the start event */

@@ -6,6 +6,8 @@ log-sum-exp adds the two-ulp exponential, the rounded reference (2^-22 of the la
 sums of at most 256 + V / 2048 steps.  A probability is then off by e + the error of lse,
 relatively; S is rounded to the type (half a step); a gradient is a sum of products of those in
 binary32 and rounded once more."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -324,6 +326,80 @@ def test_captured_forward_and_backward_replay_on_new_inputs(gm, dev):
     del g
     for p in (ws, dx, dw):
         dev.free(p)
+    call.close()
+
+
+@pytest.mark.gpu
+def test_a_wait_that_runs_out_is_reported_and_the_device_stays_usable(gm, dev):
+    """The bounded wait of the products, on a barrier that nothing arrives at, with a budget of a few
+    milliseconds; what follows is what a product that gave up would leave."""
+    L = gm.lib
+    x, w, t = make(F16, 140, 32, 300, 1)
+    call = Call(gm, dev, F16, x, w, t)
+    good = call.forward()
+    gave_up = C.c_int(0)
+    assert L.gm_linear_xent_status(dev.h) == 0
+    gm.check(L.gm_selftest_xent_timeout(dev.h, 4_000_000, C.byref(gave_up)))
+    assert gave_up.value == 1
+    assert np.isnan(call.forward()[2][0])
+    assert L.gm_linear_xent_status(dev.h) == -12 and "ran out" in gm.last_error()
+    assert L.gm_linear_xent_status(dev.h) == 0
+    assert all(np.array_equal(a, b) for a, b in zip(good, call.forward()))
+    assert L.gm_selftest_xent_timeout(dev.h, 0, C.byref(gave_up)) == -10 and L.gm_selftest_xent_timeout(dev.h, 1, None) == -10
+    call.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n", [1, 31, 32, 33, 64, 65, 127, 128, 129, 1024, 1025, 2048, 2049])
+def test_every_form_of_the_forward_pass(gm, dev, dtype, n):
+    """Around the row counts where another form takes over, with hidden states that can and cannot be read in place."""
+    for vocab, ex, shift in [(1000, 0, 0), (37, 3, 0), (5000, 8, 1)]:
+        x, w, t = make(dtype, n, 72, vocab, n + vocab, 0.3 if n > 1 else 0.0)
+        call = Call(gm, dev, dtype, x, w, t, 1, ex, 0, shift)
+        ref, err, count = reference(x, w, t, 1.0)
+        check_forward(call.forward(), ref, err, count, 1)
+        call.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,dim,vocab", [(700, 1300, 2000), (5000, 300, 700), (256, 2048, 257), (1000, 600, 9000)])
+def test_shares_of_k_and_pieces(gm, dev, n, dim, vocab):
+    """Sizes whose dX has whole rounds of tiles, a split last round, or nothing but split tiles, in one
+    piece of the vocabulary and in many."""
+    x, w, t = make(BF16, n, dim, vocab, 5, 0.1)
+    call = Call(gm, dev, BF16, x, w, t)
+    count = int((t >= 0).sum())
+    ref, err, _ = reference(x, w, t, 1.0 / count)
+    call.forward()
+    for which in (1, 2):
+        check_backward(call.backward(which=which), ref, err, call)
+    call.close()
+
+
+@pytest.mark.gpu
+def test_table_gradient_at_an_odd_address(gm, dev):
+    """dW needs no alignment beyond its type's, with and without accumulation."""
+    L = gm.lib
+    x, w, t = make(F16, 90, 40, 300, 12)
+    call = Call(gm, dev, F16, x, w, t)
+    call.forward()
+    want = call.backward(dx=False)[1]
+    base = R.rounded(np.random.default_rng(3).standard_normal(w.shape), F16)
+    ws, size = call.room(1)
+    for add in (0, 1):
+        raw = np.concatenate([np.zeros(2, np.uint8), R.bytes_of(base, F16), np.zeros(62, np.uint8)])
+        p = dev.to_device(raw)
+        gm.check(L.gm_linear_xent_backward_async(dev.h, call.h, call.x, call.w, call.t, call.lse, 0, 1.0, 0, p + 2, add, ws, size))
+        got = dev.to_host(p, raw.size, np.uint8)
+        v = R.values_of(got[2:2 + base.size * 2].copy(), F16).reshape(base.shape)
+        if add:
+            assert np.all(np.abs(v - (base + want)) <= R.HALF_STEP[F16] * (np.abs(base + want) + np.abs(want) * 1.01) + 2 * R.TINY[F16])
+        else:
+            assert np.array_equal(v, want)
+        assert not got[:2].any() and not got[2 + base.size * 2:].any()
+        dev.free(p)
+    call.end_room(ws, size)
     call.close()
 
 
