@@ -19,8 +19,8 @@ constexpr int kMergeWays = 8;            // sorted runs that one merge pass join
 // ---------------------------------------------------------------- forward
 // A CTA is tx lanes over groups of eight columns times ty tokens; each thread takes ROWS
 // tokens and issues all its loads first.  VEC: rows begin on 16-byte boundaries; the last
-// dim % 8 columns, and everything without VEC, go element by element.  WHOLE: dim is a multiple
-// of eight, so a group is a block of dropout's generator.
+// dim % 8 columns go element by element.  WHOLE: dim is a multiple of eight, so a group is a block
+// of dropout's generator.
 template <typename T, bool VEC, bool WHOLE, int ROWS>
 __global__ void __launch_bounds__(kEmbThreads, 4)
 embedding_forward_kernel(const T* __restrict__ table, const int* __restrict__ tokens, T* __restrict__ out, const int n, const int dim,
@@ -39,22 +39,22 @@ embedding_forward_kernel(const T* __restrict__ table, const int* __restrict__ to
     const int live = n - t0 < ROWS ? (int)(n - t0) : ROWS;           // tokens of this thread (may be none)
     for (int g = blockIdx.y * blockDim.x + threadIdx.x; g < groups; g += gridDim.y * blockDim.x) {
         const int c = g << 3;
-        if (VEC && (WHOLE || c + 8 <= dim)) {
-            Raw8<T> raw[ROWS];
+        if (WHOLE || c + 8 <= dim) {
+            Eight<T, VEC> raw[ROWS];
 #pragma unroll
             for (int r = 0; r < ROWS; ++r)
-                if (tok[r] >= 0) raw[r] = load8<T, true>(table + (long long)tok[r] * ld_table + c);
+                if (tok[r] >= 0) raw[r].template load<true>(table + (long long)tok[r] * ld_table + c);
 #pragma unroll
             for (int r = 0; r < ROWS; ++r) {
                 if (r >= live) break;
                 float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
                 if (tok[r] >= 0) {
-                    widen8<T>(raw[r], x);
+                    widen8<T>(raw[r].r, x);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[k] = __fmul_rn(x[k], up);
                     drop8<WHOLE>(d, o, (unsigned long long)((t0 + r) * dim + c), x);
                 }
-                store8<T>(out + (t0 + r) * ld_out + c, x);
+                Eight<T, VEC>::store(out + (t0 + r) * ld_out + c, x);
             }
         } else {
             for (int r = 0; r < live; ++r) {
@@ -186,14 +186,16 @@ template <typename G, bool VEC, bool WHOLE, bool ADD>
 __device__ __forceinline__ void put_row(G* to, float (&x)[8], const float up, const int cols) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] = __fmul_rn(x[k], up);
-    if (VEC && (WHOLE || cols >= 8)) {
+    if (WHOLE || cols >= 8) {
         if (ADD) {
             float old[8];
-            widen8<G>(load8<G, false>(to), old);
+            Eight<G, VEC> there;
+            there.template load<false>(to);
+            widen8<G>(there.r, old);
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] = __fadd_rn(old[k], x[k]);
         }
-        store8<G>(to, x);
+        Eight<G, VEC>::store(to, x);
     } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -215,20 +217,22 @@ embedding_sum_kernel(const T* __restrict__ dout, const unsigned long long* __res
         const long long v0 = (blockIdx.x - before) * kZeroRows;
         if (tid < kZeroRows) tok[tid] = v0 + tid < vocab ? used[v0 + tid] : 1u;
         __syncthreads();
-        // lanes over the groups of a row, and several rows at a time where a row is narrow
-        const int lanes = groups >= kSumThreads ? kSumThreads : groups > 32 ? 64 : groups > 16 ? 32 : groups > 8 ? 16 : 8;
+        // lanes over the 16-byte words of a row, and several rows at a time where a row is narrow; a row
+        // that begins or ends inside a word has those elements zeroed by themselves
+        constexpr int PER = 16 / sizeof(G);
+        const int words_of_row = (dim + PER - 1) / PER;
+        const int lanes = words_of_row >= kSumThreads ? kSumThreads : words_of_row > 32 ? 64 : words_of_row > 16 ? 32 : words_of_row > 8 ? 16 : 8;
+        const int lane = tid & (lanes - 1);
         for (int r = tid / lanes; r < kZeroRows; r += kSumThreads / lanes) {
             if (tok[r]) continue;
             G* const row = dtable + (v0 + r) * ld_table;
-            for (int g = tid & (lanes - 1); g < groups; g += lanes) {
-                if (VEC && (WHOLE || g * 8 + 8 <= dim)) {
-                    uint4* to = reinterpret_cast<uint4*>(row + g * 8);
-                    __stcs(to, make_uint4(0u, 0u, 0u, 0u));
-                    if (sizeof(G) == 4) __stcs(to + 1, make_uint4(0u, 0u, 0u, 0u));
-                } else {
-                    for (int k = 0; k < 8 && k < dim - g * 8; ++k) row[g * 8 + k] = from_f32<G>(0.0f);
-                }
-            }
+            int head = VEC ? 0 : (int)((16u - (unsigned)(reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / (int)sizeof(G);
+            if (head > dim) head = dim;
+            const int body = (dim - head) / PER;
+            for (int w = lane; w < body; w += lanes) __stcs(reinterpret_cast<uint4*>(row + head) + w, make_uint4(0u, 0u, 0u, 0u));
+            const int rest = head + body * PER;
+            if (lane < head) row[lane] = from_f32<G>(0.0f);
+            if (lane < dim - rest) row[rest + lane] = from_f32<G>(0.0f);
         }
         return;
     }
@@ -249,23 +253,24 @@ embedding_sum_kernel(const T* __restrict__ dout, const unsigned long long* __res
     const float up = __fmul_rn(scale, d.up);
     const int g = (int)(before - chunk * col_ctas) * kSumThreads + tid, c = g << 3;
     if (g >= groups) return;
-    const bool vec = VEC && (WHOLE || c + 8 <= dim);
+    const bool full = WHOLE || c + 8 <= dim;
     bool head = from_before;                                          // the current row began in an earlier chunk
     float acc[8] = {};
-    for (int base = 0; base < len; base += kSumDeep) {
-        Raw8<T> raw[kSumDeep];
-        if (vec) {
+    constexpr int kDeep = VEC ? kSumDeep : kSumDeep / 2;
+    for (int base = 0; base < len; base += kDeep) {
+        Eight<T, VEC> raw[kDeep];
+        if (full) {
 #pragma unroll
-            for (int j = 0; j < kSumDeep; ++j)
-                if (base + j < len) raw[j] = load8<T, false>(dout + (long long)pos[base + j] * ld_out + c);
+            for (int j = 0; j < kDeep; ++j)
+                if (base + j < len) raw[j].template load<false>(dout + (long long)pos[base + j] * ld_out + c);
         }
 #pragma unroll
-        for (int j = 0; j < kSumDeep; ++j) {
+        for (int j = 0; j < kDeep; ++j) {
             if (base + j >= len) break;
             float x[8] = {};
             const long long p = pos[base + j];
-            if (vec) {
-                widen8<T>(raw[j], x);
+            if (full) {
+                widen8<T>(raw[j].r, x);
             } else {
                 for (int k = 0; k < 8 && k < dim - c; ++k) x[k] = to_f32<T>(dout[p * ld_out + c + k]);
             }
@@ -400,7 +405,8 @@ static int launch_embedding_forward(Device* d, const gm_embedding_t* e, uintptr_
                                  (const T*)table, (const int*)tokens, (T*)out, (int)e->tokens, (int)e->dim, (int)e->vocab, (int)e->ld_table, \
                                  (int)e->ld_out, e->scale, drop))
     const bool whole = e->dim % 8 == 0;
-    if (!vec) GM_FORWARD(false, false, 1);
+    if (!vec && many) GM_FORWARD(false, false, 2);
+    else if (!vec) GM_FORWARD(false, false, 1);
     else if (!whole) GM_FORWARD(true, false, 1);
     else if (many) GM_FORWARD(true, true, 4);
     else GM_FORWARD(true, true, 1);

@@ -74,6 +74,86 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float (
     }
 }
 
+// Eight elements at any address, read as the 16-byte words that hold them (each word holds at least
+// one of the eight, so nothing outside their 16-byte words is touched) and shifted into place when
+// they are used.  Matrices whose rows do not begin on 16-byte boundaries come this way: element
+// by element the same traffic took 4 times as long.
+template <typename T> struct Any8 {
+    uint4 a, b, c;               // c: fp32 only
+    unsigned off;                // bytes from a's begin to the first element
+};
+
+template <typename T> __device__ __forceinline__ Any8<T> load8_any(const T* p) {
+    Any8<T> r;
+    r.off = (unsigned)(reinterpret_cast<uintptr_t>(p) & 15u);
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
+    r.a = q[0];
+    if (sizeof(T) == 4) {
+        r.b = q[1];
+        r.c = r.off ? q[2] : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+        r.b = r.off ? q[1] : make_uint4(0u, 0u, 0u, 0u);
+        r.c = make_uint4(0u, 0u, 0u, 0u);
+    }
+    return r;
+}
+
+template <typename T> __device__ __forceinline__ void widen8(const Any8<T>& r, float (&x)[8]) {
+    unsigned w[12] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w, r.c.x, r.c.y, r.c.z, r.c.w};
+    constexpr int N = sizeof(T) == 4 ? 8 : 4;                        // words of eight elements
+    if (r.off & 8u) {
+#pragma unroll
+        for (int k = 0; k < N + 2; ++k) w[k] = w[k + 2];
+    }
+    if (r.off & 4u) {
+#pragma unroll
+        for (int k = 0; k < N + 1; ++k) w[k] = w[k + 1];
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(w[k]);
+    } else {
+        const unsigned bits = (r.off & 2u) * 8u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 f = unpack2<T>(__funnelshift_r(w[k], w[k + 1], bits));
+            x[2 * k] = f.x;
+            x[2 * k + 1] = f.y;
+        }
+    }
+}
+
+// Eight elements to any address, in 32-bit stores and two of 16 bits where they straddle.
+template <typename T> __device__ __forceinline__ void store8_any(T* p, const float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p[k] = x[k];
+    } else if ((reinterpret_cast<uintptr_t>(p) & 2u) == 0) {
+        unsigned* q = reinterpret_cast<unsigned*>(p);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = pack2<T>(x[2 * k], x[2 * k + 1]);
+    } else {
+        p[0] = from_f32<T>(x[0]);
+        unsigned* q = reinterpret_cast<unsigned*>(p + 1);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) q[k] = pack2<T>(x[2 * k + 1], x[2 * k + 2]);
+        p[7] = from_f32<T>(x[7]);
+    }
+}
+
+// Both kinds under one name: VEC says that the address is a multiple of 16 bytes.
+template <typename T, bool VEC> struct Eight;
+template <typename T> struct Eight<T, true> {
+    Raw8<T> r;
+    template <bool CACHED> __device__ __forceinline__ void load(const T* p) { r = load8<T, CACHED>(p); }
+    static __device__ __forceinline__ void store(T* p, const float (&x)[8]) { store8<T>(p, x); }
+};
+template <typename T> struct Eight<T, false> {
+    Any8<T> r;
+    template <bool CACHED> __device__ __forceinline__ void load(const T* p) { r = load8_any<T>(p); }
+    static __device__ __forceinline__ void store(T* p, const float (&x)[8]) { store8_any<T>(p, x); }
+};
+
 // ---- dropout's generator ----
 // Philox-4x32 with ten rounds (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy
 // as 1, 2, 3", SC 2011): counter {element / 8 (64 bits), offset (64 bits)}, key = seed.  The
