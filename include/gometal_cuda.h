@@ -374,7 +374,7 @@ int gm_embedding_forward_async(uintptr_t device_ptr, const gm_embedding_t* e, ui
  * in ascending t after a sort of the tokens, no float atomics: the same call gives the same
  * bits.  grad_dtype is GM_F32 or e->dtype.  accumulate 0 writes every row of the table's
  * gradient (zeros where no token points); accumulate 1 adds to the rows that tokens point at and
- * leaves the others untouched.  A row's sum may be taken in runs of 8 or 32 tokens whose sums are added. */
+ * leaves the others untouched.  A row's sum may be taken in runs of 8 to 32 tokens whose sums are added. */
 int64_t gm_embedding_workspace_bytes(const gm_embedding_t* e);   /* of the backward pass; -1: bad argument */
 int gm_embedding_backward_async(uintptr_t device_ptr, const gm_embedding_t* e, uintptr_t tokens, uintptr_t dout,
                                 const gm_dropout_t* dropout /* NULL: none */, uintptr_t dtable, int grad_dtype,
