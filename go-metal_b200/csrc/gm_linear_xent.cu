@@ -760,11 +760,13 @@ static int make_map(CUtensorMap* map, int dtype, uintptr_t base, int64_t rows, i
     return GM_OK;
 }
 
-// Launches one product with as many CTA pairs as fit at once, at most one per tile.
-template <int TN, bool MN_A, bool MN_B, typename Ops>
-static int launch_tiles(Device* d, const CUtensorMap& a, const CUtensorMap& b, const Ops& ops, int64_t max_tiles, int* launched = nullptr) {
-    auto kernel = tile_gemm_kernel<TN, MN_A, MN_B, Ops>;
-    constexpr int kGemmSmem = Ring<TN>::kSmem + (Ops::kStaging ? 8 * kStagingBytes : 0);
+// Launches one product or two with as many CTA pairs as fit at once, at most one per turn.
+template <int TN, typename First, typename Second = NoProduct>
+static int launch_tiles(Device* d, const First& first, int64_t max_turns, int* launched = nullptr, const Second& second = Second()) {
+    auto kernel = tile_gemm_kernel<TN, First, Second>;
+    bool staging = First::Ops::kStaging;
+    if constexpr (Second::kAny) staging = staging || Second::Ops::kStaging;
+    const int smem = Ring<TN>::kSmem + (staging ? 8 * kStagingBytes : 0);
     static std::mutex mu;
     static int pairs_of[64] = {0};                   // per device ordinal
     int pairs;
@@ -772,11 +774,11 @@ static int launch_tiles(Device* d, const CUtensorMap& a, const CUtensorMap& b, c
         std::lock_guard<std::mutex> lk(mu);
         int& known = pairs_of[d->ordinal & 63];
         if (known == 0) {
-            GM_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem));
+            GM_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
             cudaLaunchConfig_t cfg = {};
             cfg.gridDim = dim3((unsigned)(d->sm_count / 2 * 2));
             cfg.blockDim = dim3(kGemmThreads);
-            cfg.dynamicSmemBytes = kGemmSmem;
+            cfg.dynamicSmemBytes = smem;
             cudaLaunchAttribute attr = {};
             attr.id = cudaLaunchAttributeClusterDimension;
             attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
@@ -789,9 +791,9 @@ static int launch_tiles(Device* d, const CUtensorMap& a, const CUtensorMap& b, c
         }
         pairs = known;
     }
-    if (max_tiles < pairs) pairs = (int)max_tiles;
+    if (max_turns < pairs) pairs = (int)max_turns;
     if (launched) *launched = pairs;
-    GM_CUDA_CHECK(launch_chained(kernel, dim3((unsigned)pairs * 2), dim3(kGemmThreads), kGemmSmem, d->stream, a, b, ops,
+    GM_CUDA_CHECK(launch_chained(kernel, dim3((unsigned)pairs * 2), dim3(kGemmThreads), smem, d->stream, first, second,
                                  reinterpret_cast<int*>(d->scalars + kXentStatusWord), d->barrier_budget_cycles));
     d->launches++;
     return GM_OK;
@@ -945,7 +947,7 @@ static int forward_few(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
     }
     float2* stats = (float2*)(c.ws + s.stats);
     const FewStatsOps<T, TN> ops{c.sc(), (const int*)targets, stats, (int)h->tokens, (int)s.cap, (int)h->dim, (int)h->vocab, height, 0, 0};
-    GM_TRY((launch_tiles<TN, false, false>(c.d, map_w, map_x, ops, tiles)));
+    GM_TRY((launch_tiles<TN>(c.d, Product<FewStatsOps<T, TN>, false, false>{map_w, map_x, ops}, tiles)));
     GM_CUDA_CHECK(launch_chained(xent_few_join_kernel<T>, dim3((unsigned)h->tokens), dim3(256), 0, c.d->stream, c.sc(), (const T*)hidden, h->ld_hidden,
                                  (const T*)weight, h->ld_weight, (const int*)targets, (int)h->dim, (int)h->vocab, stats, (int)s.cap, (int)tiles * 8, losses, lse,
                                  (float*)(c.ws + s.partial), total, h->mean, reinterpret_cast<const int*>(c.d->scalars + kXentStatusWord)));
@@ -971,7 +973,7 @@ static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
     const int64_t n_tiles = (h->vocab + kTileN - 1) / kTileN;
     const int tiles = (int)((h->vocab + kTileN / 2 - 1) / (kTileN / 2));
     const StatsOps<T> ops{c.sc(), c.target(), stats, (int)s.cap, (int)h->dim, (int)h->vocab, logits_group(h), 0, 0};
-    GM_TRY((launch_tiles<kTileN, false, false>(c.d, map_x, map_w, ops, s.cap / kTileM * n_tiles)));
+    GM_TRY((launch_tiles<kTileN>(c.d, Product<StatsOps<T>, false, false>{map_x, map_w, ops}, s.cap / kTileM * n_tiles)));
     // a CTA per row up to a few rows per SM, 8 rows per CTA beyond
     auto join = h->tokens <= 1024 ? xent_join_kernel<1> : xent_join_kernel<8>;
     const int64_t ctas = h->tokens <= 1024 ? h->tokens : s.cap / 8;
@@ -998,28 +1000,36 @@ static int run_backward(const XentCall& c, uintptr_t hidden, uintptr_t weight, u
     const GradScale scale{scale_device, grad_scale, h->mean, 1.0f / Half16<T>::kUp};
     const int dim = (int)h->dim, vocab = (int)h->vocab;
     const int64_t m_tiles = s.cap / kTileM, d_tiles = (h->dim + kTileN - 1) / kTileN;
+    using Hidden = Product<HiddenGradOps<T>, false, true>;
+    using Weight = Product<WeightGradOps<T>, true, true>;
     for (int64_t v = 0; v < vocab; v += s.width) {
         const int v0 = (int)v, v1 = (int)(v + s.width < vocab ? v + s.width : vocab);
         const int64_t v_tiles = (v1 - v0 + kTileN - 1) / kTileN;
         const SoftmaxGradOps<T> grad{c.sc(), c.target(), c.rows(), lse, (T*)ds, s.width, dim, v0, v1, logits_group(h), 0, v0};
-        GM_TRY((launch_tiles<kTileN, false, false>(c.d, x_k, w_k, grad, m_tiles * v_tiles)));
+        GM_TRY((launch_tiles<kTileN>(c.d, Product<SoftmaxGradOps<T>, false, false>{x_k, w_k, grad}, m_tiles * v_tiles)));
+        const HiddenPlan shape{dim, v0, v1, (int)split_parts(h)};
+        const HiddenOut<T> out{(float*)(c.ws + s.carried), s.ld_carried, (T*)dhidden, h->ld_hidden, scale, v0 == 0, v1 == vocab,
+                               dhidden % 16 == 0 && h->ld_hidden % 8 == 0};
+        float* parts = (float*)(c.ws + s.parts);
+        const Hidden dx{ds_k, w_mn, HiddenGradOps<T>{c.sc(), c.rows(), parts, shape, out, 0, v0}};
+        const Weight dw{ds_mn, x_mn, WeightGradOps<T>{c.sc(), (T*)dweight, h->ld_weight, scale, dim, v0, v1, 0, 0, accumulate, dweight % 16 == 0}};
+        const int64_t x_turns = m_tiles * d_tiles * 16, w_turns = v_tiles * d_tiles;
+        int pairs = 0;
+        // One launch of both gradients saves a start and an end and fills dX's last round: 54 -> 47 us
+        // at 256 x 512 x 10,007, 156 -> 142 us at 6,525 x 1,808 x 1,314, 1,778 -> 1,737 us at 512 x 4,096 x
+        // 131,072.  In many rounds with dX in more than two, its longer turns on a fixed schedule lose
+        // more: 4.24 -> 4.32 ms at 8,862 x 1,384 x 55,838.
+        const int64_t per_round = c.d->sm_count / 2;
+        const bool both = dhidden && dweight && ((m_tiles + v_tiles) * d_tiles <= 16 * per_round || m_tiles * d_tiles <= 2 * per_round);
+        if (both) GM_TRY((launch_tiles<kTileN>(c.d, dx, x_turns + w_turns, &pairs, dw)));
+        else if (dhidden) GM_TRY((launch_tiles<kTileN>(c.d, dx, x_turns, &pairs)));
         if (dhidden) {
-            const bool vec = dhidden % 16 == 0 && h->ld_hidden % 8 == 0;
-            const HiddenPlan shape{dim, v0, v1, (int)split_parts(h)};
-            const HiddenOut<T> out{(float*)(c.ws + s.carried), s.ld_carried, (T*)dhidden, h->ld_hidden, scale, v0 == 0, v1 == vocab, vec};
-            float* parts = (float*)(c.ws + s.parts);
-            int pairs = 0;
-            GM_TRY((launch_tiles<kTileN, false, true>(c.d, ds_k, w_mn, HiddenGradOps<T>{c.sc(), c.rows(), parts, shape, out, 0, v0}, m_tiles * d_tiles * 16, &pairs)));
             // how many tiles are split follows from the rows with a target, which only the device knows
             GM_CUDA_CHECK(launch_chained(xent_hidden_join_kernel<T>, dim3((unsigned)c.d->sm_count * 4), dim3(256), 0, c.d->stream, c.sc(), c.rows(), parts, shape,
                                          out, pairs));
             c.d->launches++;
         }
-        if (dweight) {
-            const bool vec = dweight % 16 == 0;
-            const WeightGradOps<T> ops{c.sc(), (T*)dweight, h->ld_weight, scale, dim, v0, v1, 0, 0, accumulate, vec};
-            GM_TRY((launch_tiles<kTileN, true, true>(c.d, ds_mn, x_mn, ops, v_tiles * d_tiles)));
-        }
+        if (dweight && !both) GM_TRY((launch_tiles<kTileN>(c.d, dw, w_turns)));
     }
     return GM_OK;
 }

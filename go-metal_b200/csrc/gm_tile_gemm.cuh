@@ -30,6 +30,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "gm_lm.cuh"
 
 namespace gm {
@@ -278,7 +280,7 @@ __device__ __forceinline__ void split_tail(TilePlan* p, int pairs, int most_part
         }
 }
 
-// MN_A / MN_B: that operand is MN-major.  Ops provides
+// A product: the operands' maps, which of them are MN-major, and Ops, which provides
 //   kBf16             whether the inputs are bf16 (else fp16)
 //   kStaging          whether the epilogue wants shared memory
 //   begin()           run by one thread before anything else
@@ -291,12 +293,25 @@ __device__ __forceinline__ void split_tail(TilePlan* p, int pairs, int most_part
 //   epilogue(plan, at, row, v, half, stage, prepared)   the row inside the tile, half of its
 //                     columns (zeros with an empty share of K), which half, 4 KB of shared memory for
 //                     the warp (with kStaging); called by whole warps, also for rows behind the last one
-template <int TN, bool MN_A, bool MN_B, typename Ops>
+template <typename Ops_, bool MN_A, bool MN_B>
+struct Product {
+    using Ops = Ops_;
+    static constexpr bool kMnA = MN_A, kMnB = MN_B, kAny = true;
+    CUtensorMap a, b;
+    Ops ops;
+    __device__ __forceinline__ TilePlan plan(int pairs) const { return ops.plan(pairs); }
+};
+struct NoProduct {
+    static constexpr bool kAny = false;
+    __device__ __forceinline__ TilePlan plan(int) const { return {0, 0, 0, 0, 1, 0, 1}; }
+};
+
+// One product, or two whose inputs are ready at the same time: the second one's tiles then fill the
+// pairs that the first one's last round leaves idle.
+template <int TN, typename First, typename Second>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGemmThreads, 1)
-tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Ops ops,
-                 int* status, const long long budget) {
+tile_gemm_kernel(const __grid_constant__ First first, const __grid_constant__ Second second, int* status, const long long budget) {
     constexpr int kStages = Ring<TN>::kStages, kStageBytes = Ring<TN>::kStageBytes, kRowsB = Ring<TN>::kRowsB;
-    static_assert(!MN_B || TN == 256, "an MN-major B comes in two blocks of 64 columns per CTA");
     extern __shared__ unsigned char dyn[];
     __shared__ __align__(8) unsigned long long full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
     __shared__ unsigned tmem_base;
@@ -315,8 +330,12 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (tid == 64) {
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&first.a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&first.b) : "memory");
+        if constexpr (Second::kAny) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&second.a) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&second.b) : "memory");
+        }
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_base)) : "memory");
@@ -329,68 +348,80 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const unsigned tmem = tmem_base;
     // all of the above may run while the kernel before this one ends
     chain_begin();
-    if (blockIdx.x == 0 && tid == 0) ops.begin();
-    const TilePlan plan = ops.plan(pairs);
-    const int items = plan.items();
+    if (blockIdx.x == 0 && tid == 0) first.ops.begin();
+    const TilePlan plan = first.plan(pairs), plan2 = second.plan(pairs);
+    const int items = plan.items(), all = items + plan2.items();
 
     unsigned issued = 0;                                         // k-blocks this thread copied; stage and parity follow from it
     if (warp == 0 && lane == 0) {
         // ---- copies ----
-        bool ok = true;
-        const int rows_a = ops.rows_a();
-        const unsigned bytes = 2u * (unsigned)(rows_a + kRowsB) * (kTileK * 2);              // both CTAs' copies
-
-        for (int t = pair; t < items && ok; t += pairs) {
-            const TileAt at = plan.at(t);
+        auto copy = [&](const auto& product, const TileAt at) {
+            using P = std::decay_t<decltype(product)>;
+            static_assert(!P::kMnB || TN == 256, "an MN-major B comes in two blocks of 64 columns per CTA");
+            const int rows_a = product.ops.rows_a();
+            const unsigned bytes = 2u * (unsigned)(rows_a + kRowsB) * (kTileK * 2);          // both CTAs' copies
             const int row_a = (at.m * 2 + (int)rank) * rows_a, row_b = at.n * TN + (int)rank * kRowsB;
             for (int k = at.k0; k < at.k1; ++k, ++issued) {
                 const int s = issued % kStages;
                 const unsigned turn = issued / kStages;
-                if (!mbar_wait(smem_u32(&empty[s]), (turn & 1u) ^ 1u, &abort_flag, budget)) { ok = false; break; }
+                if (!mbar_wait(smem_u32(&empty[s]), (turn & 1u) ^ 1u, &abort_flag, budget)) return false;
                 const unsigned bar = pair_leader_addr(smem_u32(&full[s]));
                 if (rank == 0) mbar_expect(smem_u32(&full[s]), bytes);
                 const unsigned a = ring + s * kStageBytes, b = a + kOperandBytes;
-                if (MN_A) {
-                    tma_load(a, &map_a, row_a, ops.a0 + k * kTileK, bar);
-                    tma_load(a + 8192, &map_a, row_a + 64, ops.a0 + k * kTileK, bar);
+                if (P::kMnA) {
+                    tma_load(a, &product.a, row_a, product.ops.a0 + k * kTileK, bar);
+                    tma_load(a + 8192, &product.a, row_a + 64, product.ops.a0 + k * kTileK, bar);
                 } else {
-                    tma_load(a, &map_a, k * kTileK, ops.a0 + row_a, bar);
+                    tma_load(a, &product.a, k * kTileK, product.ops.a0 + row_a, bar);
                 }
-                if (MN_B) {
-                    tma_load(b, &map_b, row_b, ops.b0 + k * kTileK, bar);
-                    tma_load(b + 8192, &map_b, row_b + 64, ops.b0 + k * kTileK, bar);
+                if (P::kMnB) {
+                    tma_load(b, &product.b, row_b, product.ops.b0 + k * kTileK, bar);
+                    tma_load(b + 8192, &product.b, row_b + 64, product.ops.b0 + k * kTileK, bar);
                 } else {
-                    tma_load(b, &map_b, k * kTileK, ops.b0 + row_b, bar);
+                    tma_load(b, &product.b, k * kTileK, product.ops.b0 + row_b, bar);
                 }
             }
+            return true;
+        };
+        bool ok = true;
+        for (int t = pair; t < all && ok; t += pairs) {
+            if constexpr (Second::kAny)
+                if (t >= items) { ok = copy(second, plan2.at(t - items)); continue; }
+            ok = copy(first, plan.at(t));
         }
     } else if (warp == 1 && lane == 0 && rank == 0) {
         // ---- products ----
-        // accumulators binary32, inputs fp16 or bf16, N / 8 in bits 17-22, M / 16 in bits 24-28
-        const unsigned in = Ops::kBf16 ? 1u : 0u;
-        const unsigned idesc = (1u << 4) | (in << 7) | (in << 10) | ((MN_A ? 1u : 0u) << 15) | ((MN_B ? 1u : 0u) << 16) |
-                               ((unsigned)(TN / 8) << 17) | ((unsigned)(kTileM / 16) << 24);
         unsigned used = 0;                                       // k-blocks consumed
         int count = 0;
-        bool ok = true;
-        for (int t = pair; t < items && ok; t += pairs, ++count) {
-            const TileAt at = plan.at(t);
+        auto multiply = [&](const auto& product, const TileAt at) {
+            using P = std::decay_t<decltype(product)>;
+            // accumulators binary32, inputs fp16 or bf16, N / 8 in bits 17-22, M / 16 in bits 24-28
+            const unsigned in = P::Ops::kBf16 ? 1u : 0u;
+            const unsigned idesc = (1u << 4) | (in << 7) | (in << 10) | ((P::kMnA ? 1u : 0u) << 15) | ((P::kMnB ? 1u : 0u) << 16) |
+                                   ((unsigned)(TN / 8) << 17) | ((unsigned)(kTileM / 16) << 24);
             const int slot = count & 1;
-            if (!mbar_wait(smem_u32(&acc_empty[slot]), ((count >> 1) & 1) ^ 1, &abort_flag, budget)) { ok = false; break; }
+            if (!mbar_wait(smem_u32(&acc_empty[slot]), ((count >> 1) & 1) ^ 1, &abort_flag, budget)) return false;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const unsigned d = tmem + (unsigned)slot * 256u;
             for (int k = at.k0; k < at.k1; ++k, ++used) {
                 const int s = used % kStages;
-                if (!mbar_wait(smem_u32(&full[s]), (used / kStages) & 1u, &abort_flag, budget)) { ok = false; break; }
+                if (!mbar_wait(smem_u32(&full[s]), (used / kStages) & 1u, &abort_flag, budget)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const unsigned a = ring + s * kStageBytes;
-                const unsigned long long da = mat_desc(a, MN_A), db = mat_desc(a + kOperandBytes, MN_B);
+                const unsigned long long da = mat_desc(a, P::kMnA), db = mat_desc(a + kOperandBytes, P::kMnB);
 #pragma unroll
                 for (int i = 0; i < kTileK / 16; ++i)
-                    mma_pair(d, da + (MN_A ? 128 * i : 2 * i), db + (MN_B ? 128 * i : 2 * i), idesc, k > at.k0 || i > 0);
+                    mma_pair(d, da + (P::kMnA ? 128 * i : 2 * i), db + (P::kMnB ? 128 * i : 2 * i), idesc, k > at.k0 || i > 0);
                 mma_commit_pair(smem_u32(&empty[s]));
             }
-            if (ok) mma_commit_pair(smem_u32(&acc_full[slot]));
+            mma_commit_pair(smem_u32(&acc_full[slot]));
+            return true;
+        };
+        bool ok = true;
+        for (int t = pair; t < all && ok; t += pairs, ++count) {
+            if constexpr (Second::kAny)
+                if (t >= items) { ok = multiply(second, plan2.at(t - items)); continue; }
+            ok = multiply(first, plan.at(t));
         }
         if (!ok) {
             mma_commit_pair(smem_u32(&drain));
@@ -405,12 +436,11 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const unsigned staging = ring + kStages * kStageBytes + (warp - 2) * kStagingBytes;
         constexpr int kColumns = TN / 2 < 32 ? 32 : TN / 2;       // a narrow tile is all the first half's
         int count = 0;
-        for (int t = pair; t < items; t += pairs, ++count) {
-            const TileAt at = plan.at(t);
+        auto finish = [&](const auto& product, const TilePlan& tiles, const TileAt at) {
             const int slot = count & 1;
-            const auto prepared = ops.prepare(plan, at, row);
+            const auto prepared = product.ops.prepare(tiles, at, row);
             const bool ok = mbar_wait(smem_u32(&acc_full[slot]), (count >> 1) & 1, &abort_flag, budget);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            if (!__all_sync(0xffffffffu, ok)) return false;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float v[kColumns];
             tmem_read<kColumns>(tmem + (unsigned)(slot * 256 + half * kColumns) + ((unsigned)(quarter * 32) << 16), v);
@@ -421,7 +451,14 @@ tile_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
                 for (int j = 0; j < kColumns; ++j) v[j] = 0.0f;
             }
-            ops.epilogue(plan, at, row, v, half, staging, prepared);
+            product.ops.epilogue(tiles, at, row, v, half, staging, prepared);
+            return true;
+        };
+        bool ok = true;
+        for (int t = pair; t < all && ok; t += pairs, ++count) {
+            if constexpr (Second::kAny)
+                if (t >= items) { ok = finish(second, plan2, plan2.at(t - items)); continue; }
+            ok = finish(first, plan, plan.at(t));
         }
     }
     __syncwarp();
