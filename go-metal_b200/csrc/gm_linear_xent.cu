@@ -23,6 +23,7 @@
 // has to be.  In fp16 it is first multiplied by 2^15 (|S| <= 1), which keeps probabilities
 // down to 2^-29 normal, in bf16 by 2^32, so that the exponential's flush to zero at 2^-126 lies
 // below what bf16 holds; the factor is taken out in binary32 in the epilogue.
+#include <climits>
 #include <mutex>
 
 #include "gm_tile_gemm.cuh"
@@ -368,6 +369,7 @@ struct SoftmaxGradOps {
     T* ds;
     long long ld_ds;
     int dim, v0, v1, group, a0, b0;
+    static constexpr int kNoRow = INT_MIN;   // `at` of a row behind the last one
     struct Row { int at; float ref; };       // target in the tile; log2 of what the row's exponentials are divided by
     __device__ __forceinline__ TilePlan plan(int) const {
         const int count = sc->count;
@@ -375,18 +377,22 @@ struct SoftmaxGradOps {
     }
     __device__ __forceinline__ Row prepare(const TilePlan& plan, const TileAt& tile, int in_tile) const {
         const int row = tile.m * kTileM + in_tile;
-        if (row >= plan.count) return {-1, INFINITY};             // zeros: such a row's logits are 0, 2^(0 - inf) = 0
+        if (row >= plan.count) return {kNoRow, 0.0f};
         return {__ldg(target + row) - v0 - tile.n * kTileN, fmaf(__ldg(lse + __ldg(rows + row)), kLog2e, -Half16<T>::kUpLog2)};
     }
     __device__ __forceinline__ void epilogue(const TilePlan&, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned stage,
                                              const Row row) const {
 #pragma unroll
         for (int j = 0; j < 128; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -row.ref));
-        const int at = row.at - half * 128;
+        const int at = row.at == kNoRow ? -1 : row.at - half * 128;
         if ((unsigned)at < 128u) {
 #pragma unroll
             for (int j = 0; j < 128; ++j)
                 if (at == j) v[j] -= Half16<T>::kUp;
+        }
+        if (row.at == kNoRow) {                                           // whatever its logits: 0 times an infinity of the table is NaN
+#pragma unroll
+            for (int j = 0; j < 128; ++j) v[j] = 0.0f;
         }
         const int width = v1 - v0 - tile.n * kTileN - half * 128;        // columns that exist, the others are zeros
         if (width < 128) {
@@ -582,6 +588,20 @@ __device__ __forceinline__ MaxSum joined(const MaxSum a, const MaxSum b) {
     return {m, fmaf(a.s, exp2f(fmaf(a.m, kLog2e, -ref)), b.s * exp2f(fmaf(b.m, kLog2e, -ref)))};
 }
 
+// Loss and log-sum-exp of a row whose target's logit is z and whose other entries are `a`.  The loss is
+// taken as the logarithm of a sum, not as a difference, so a small loss keeps its bits.  A target with
+// logit -inf has an infinite loss, and a log-sum-exp that is its other entries'; with logit +inf both
+// the loss and its gradient are NaN, as inf - inf is.
+struct RowLoss { float loss, lse; };
+__device__ __forceinline__ RowLoss row_loss(const float z, const MaxSum a) {
+    if (z >= a.m) {
+        const float loss = log1pf(a.s * expf(a.m - z)) + (z - z);
+        return {loss, z + loss};
+    }
+    const float rest = logf(a.s + expf(z - a.m));
+    return {(a.m - z) + rest, z == -INFINITY ? a.m + rest : z + ((a.m - z) + rest)};
+}
+
 // A CTA takes ROWS rows with 256 / ROWS lanes over the vocabulary's pieces; the CTA that finishes
 // last adds up the loss.  ROWS is 8 (64 bytes of neighbouring rows; with 32 the walk over the pieces
 // is 4 times as long and took 17 us instead of 9 at 1,640 rows), or 1 in a small call.
@@ -614,10 +634,10 @@ xent_join_kernel(XentScalars* sc, const float2* __restrict__ stats, const int ro
         float loss = 0.0f;
         if (y == 0 && row < count) {
             a = part[0][x];
-            const float z = target_logit[row];
-            loss = z >= a.m ? log1pf(a.s * expf(a.m - z)) : (a.m - z) + logf(a.s + expf(z - a.m));
+            const RowLoss of = row_loss(target_logit[row], a);
+            loss = of.loss;
             losses[rows[row]] = loss;
-            lse[rows[row]] = z + loss;
+            lse[rows[row]] = of.lse;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
@@ -678,8 +698,9 @@ xent_few_join_kernel(XentScalars* sc, const T* __restrict__ hidden, const long l
         if (live) {
             z = dots[0];
             for (int k = 1; k < 8; ++k) { z += dots[k]; a = joined(a, part[k]); }
-            loss = z >= a.m ? log1pf(a.s * expf(a.m - z)) : (a.m - z) + logf(a.s + expf(z - a.m));
-            l = z + loss;
+            const RowLoss of = row_loss(z, a);
+            loss = of.loss;
+            l = of.lse;
         }
         losses[row] = loss;
         lse[row] = l;

@@ -266,6 +266,44 @@ def test_nan_reaches_its_row_and_an_infinite_gradient_is_infinite(gm, dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [20, 140])
+def test_infinite_logits(gm, dev, n):
+    """Entries masked by -inf: as targets they have an infinite loss, and their rows' log-sum-exp and gradient are
+    those of the other entries.  A target with logit +inf has no loss: NaN, in the total too."""
+    x, w, t = make(F16, n, 24, 300, 16)
+    x[:, -1], w[:, -1] = 1.0, 0.0
+    masked = np.arange(300) % 7 == 3
+    t[::5] = 3
+    left = np.flatnonzero(~masked)
+    fake = np.where(masked[t], 0, np.searchsorted(left, t)).astype(np.int32)       # the table without the masked entries
+    ref, err, _ = reference(x, w[left], fake, 1.0)
+    w[masked, -1] = -np.inf
+    call = Call(gm, dev, F16, x, w, t, mean=0)
+    losses, lse, total = call.forward()
+    hit = masked[t]
+    assert hit.any() and np.all(losses[hit] == np.inf) and total[0] == np.inf and total[1] == n
+    assert np.all(np.abs(losses[~hit] - ref["losses"][~hit]) <= err["losses"][~hit])
+    assert np.all(np.abs(lse - ref["lse"]) <= err["lse"])
+    dw = call.backward(dx=False)[1]
+    l = np.where(masked[None, :], -np.inf, x @ np.where(np.isinf(w), 0, w).T)
+    s = np.exp(l - np.logaddexp.reduce(l, 1)[:, None])
+    s[np.arange(n), t] -= 1
+    want = s.T @ x
+    err["dw_s"] = (np.abs(s).T @ np.abs(x))[left]
+    assert np.all(np.abs(dw - want)[left] <= grad_bound(err, "dw", want[left], F16, n))
+    whole = -np.stack([x[t == v].sum(0) for v in np.flatnonzero(masked)])           # softmax is 0 there
+    size = np.stack([np.abs(x[t == v]).sum(0) for v in np.flatnonzero(masked)])
+    assert np.all(np.abs(dw[masked] - whole) <= 1.01 * R.HALF_STEP[F16] * np.abs(whole) + (n + 2) * 2.0 ** -23 * size)
+    call.close()
+    w[masked, -1] = 0.0
+    w[3, -1] = np.inf
+    call = Call(gm, dev, F16, x, w, t)
+    losses, lse, total = call.forward()
+    assert np.isnan(losses[t == 3]).all() and not np.isfinite(losses).any() and np.isnan(total[0])
+    call.close()
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences(gm, dev):
     """The summed loss along a direction: a central difference of the library's own forward pass, whose
     step leaves at most h^2 of third derivatives (bounded by |d|^3) and 2 error(total) / h of rounding."""
