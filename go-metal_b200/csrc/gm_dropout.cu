@@ -7,12 +7,12 @@
 
 namespace gm {
 
-int make_drop(const gm_dropout_t* in, Drop* out) {
+int make_drop(const Device* d, const gm_dropout_t* in, Drop* out) {
     *out = Drop{};
     out->up = 1.0f;
     if (!in) return GM_OK;
     if (!(in->p >= 0.0f && in->p <= 1.0f)) { set_error("dropout probability %g is outside [0, 1]", (double)in->p); return GM_ERR_BAD_ARG; }
-    if (in->offset_device % 8) { set_error("the device offset of dropout is not 8-byte aligned"); return GM_ERR_BAD_ARG; }
+    if (in->offset_device) GM_TRY(check_buffer(d, in->offset_device, 8, 8, "device offset of dropout"));
     for (int r = 0; r < 10; ++r) {
         out->key[2 * r] = (unsigned)in->seed + (unsigned)r * 0x9E3779B9u;
         out->key[2 * r + 1] = (unsigned)(in->seed >> 32) + (unsigned)r * 0xBB67AE85u;
@@ -159,7 +159,7 @@ extern "C" int gm_dropout_async(uintptr_t device_ptr, int dtype, int64_t rows, i
         return GM_ERR_BAD_ARG;
     }
     Drop drop;
-    GM_TRY(make_drop(dropout, &drop));
+    GM_TRY(make_drop(d, dropout, &drop));
     DeviceGuard g(d);
     if (dtype == GM_F32) return residual ? launch_dropout<float, true>(d, rows, cols, x, ld_x, residual, ld_residual, y, ld_y, drop)
                                          : launch_dropout<float, false>(d, rows, cols, x, ld_x, 0, 0, y, ld_y, drop);

@@ -508,7 +508,7 @@ int gm_embedding_forward_async(uintptr_t device_ptr, const gm_embedding_t* e, ui
     GM_TRY(check_buffer(d, tokens, e->tokens * 4, 4, "tokens"));
     GM_TRY(check_buffer(d, out, matrix_bytes(e->tokens, e->dim, e->ld_out, eb), eb, "embedding output"));
     Drop drop;
-    GM_TRY(make_drop(dropout, &drop));
+    GM_TRY(make_drop(d, dropout, &drop));
     DeviceGuard g(d);
     if (e->dtype == GM_F32) return launch_embedding_forward<float>(d, e, table, tokens, out, drop);
     if (e->dtype == GM_F16) return launch_embedding_forward<__half>(d, e, table, tokens, out, drop);
@@ -534,7 +534,7 @@ int gm_embedding_backward_async(uintptr_t device_ptr, const gm_embedding_t* e, u
     if (workspace_bytes < need) { set_error("workspace of %lld bytes, the call needs %lld", (long long)workspace_bytes, (long long)need); return GM_ERR_BAD_SIZE; }
     GM_TRY(check_buffer(d, workspace, need, 256, "workspace"));
     Drop drop;
-    GM_TRY(make_drop(dropout, &drop));
+    GM_TRY(make_drop(d, dropout, &drop));
     DeviceGuard g(d);
     const bool acc = accumulate != 0;
     if (e->dtype == GM_F32) return launch_embedding_backward<float, float>(d, e, tokens, dout, drop, dtable, acc, workspace);

@@ -253,7 +253,7 @@ __device__ __forceinline__ void chain_begin() {
 inline int dtype_bytes(int dtype) { return dtype == GM_F32 ? 4 : dtype == GM_F16 || dtype == GM_BF16 ? 2 : 0; }
 
 // Fills the kernel's form of a dropout argument (null: none).  Returns GM_OK or a code.
-int make_drop(const gm_dropout_t* in, Drop* out);
+int make_drop(const Device* d, const gm_dropout_t* in, Drop* out);
 
 // A buffer of at least `need` bytes on this device, aligned to `align`; need 0 checks the rest.
 int check_buffer(const Device* d, uintptr_t p, int64_t need, int64_t align, const char* what);

@@ -169,3 +169,13 @@ def test_refusals(gm, dev):
     call(-10, rows=2, ld_x=24)                  # in place with another stride
     assert L.gm_device_launch_count(dev.h) == before
     dev.free(b)
+
+
+@pytest.mark.gpu
+def test_refuses_a_device_offset_shorter_than_a_word(gm, dev):
+    b, word = dev.alloc(4 * 64), dev.alloc(4)
+    before = gm.lib.gm_device_launch_count(dev.h)
+    assert gm.lib.gm_dropout_async(dev.h, 0, 4, 16, b, 16, 0, 16, b, 16, gm.dropout(0.1, 1, 0, word)) == -9
+    assert gm.last_error() and gm.lib.gm_device_launch_count(dev.h) == before
+    dev.free(b)
+    dev.free(word)
