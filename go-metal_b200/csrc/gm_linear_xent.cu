@@ -23,7 +23,6 @@
 // has to be.  In fp16 it is first multiplied by 2^15 (|S| <= 1), which keeps probabilities
 // down to 2^-29 normal, in bf16 by 2^32, so that the exponential's flush to zero at 2^-126 lies
 // below what bf16 holds; the factor is taken out in binary32 in the epilogue.
-#include <climits>
 #include <mutex>
 
 #include "gm_tile_gemm.cuh"
@@ -253,11 +252,12 @@ struct StatsOps {
         const int count = sc->count;
         return whole_tiles(count, (count + kTileM - 1) / kTileM, (vocab + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, group);
     }
+    __device__ __forceinline__ Nothing once(const TilePlan&) const { return {}; }
     __device__ __forceinline__ Goal prepare(const TilePlan& plan, const TileAt& tile, int in_tile) const {
         const int row = tile.m * kTileM + in_tile;
         return {row < plan.count ? __ldg(target + row) - tile.n * kTileN : -1};
     }
-    __device__ __forceinline__ void epilogue(const TilePlan& plan, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned,
+    __device__ __forceinline__ void epilogue(const TilePlan& plan, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned, Nothing,
                                              const Goal goal) const {
         const int row = tile.m * kTileM + in_tile;
         const int width = vocab - tile.n * kTileN - half * 128;           // columns that exist
@@ -321,8 +321,9 @@ struct FewStatsOps {
     __device__ __forceinline__ TilePlan plan(int) const {
         return whole_tiles(n, (vocab + 2 * height - 1) / (2 * height), 1, (dim + kTileK - 1) / kTileK, 1);
     }
+    __device__ __forceinline__ Nothing once(const TilePlan&) const { return {}; }
     __device__ __forceinline__ Goal prepare(const TilePlan&, const TileAt&, int) const { return {0}; }
-    __device__ __forceinline__ void epilogue(const TilePlan&, const TileAt& tile, int in_tile, float (&all)[kColumns], int half, unsigned, const Goal) const {
+    __device__ __forceinline__ void epilogue(const TilePlan&, const TileAt& tile, int in_tile, float (&all)[kColumns], int half, unsigned, Nothing, const Goal) const {
         const int cta = in_tile / kHalf, local = in_tile % kHalf, lane = threadIdx.x & 31;
         const int base = (tile.m * 2 + cta) * height + (local & ~31);      // entry of the warp's first lane
         const bool real = local < height && base + lane < vocab;
@@ -366,8 +367,7 @@ struct SoftmaxGradOps {
     const int* target;
     const int* rows;
     const float* lse;            // by row of the caller
-    T* ds;
-    long long ld_ds;
+    CUtensorMap ds;
     int dim, v0, v1, group, a0, b0;
     static constexpr int kNoRow = INT_MIN;   // `at` of a row behind the last one
     struct Row { int at; float ref; };       // target in the tile; log2 of what the row's exponentials are divided by
@@ -375,13 +375,16 @@ struct SoftmaxGradOps {
         const int count = sc->count;
         return whole_tiles(count, (count + kTileM - 1) / kTileM, (v1 - v0 + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, group);
     }
+    __device__ __forceinline__ Nothing once(const TilePlan&) const { return {}; }
     __device__ __forceinline__ Row prepare(const TilePlan& plan, const TileAt& tile, int in_tile) const {
         const int row = tile.m * kTileM + in_tile;
         if (row >= plan.count) return {kNoRow, 0.0f};
         return {__ldg(target + row) - v0 - tile.n * kTileN, fmaf(__ldg(lse + __ldg(rows + row)), kLog2e, -Half16<T>::kUpLog2)};
     }
-    __device__ __forceinline__ void epilogue(const TilePlan&, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned stage,
+    __device__ __forceinline__ void epilogue(const TilePlan& plan, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned stage, Nothing,
                                              const Row row) const {
+        const int first_row = tile.m * kTileM + (in_tile & ~31);
+        if (first_row >= up_to(plan.count, kTileK)) return;               // dW's sum ends there, and nothing takes what dX makes of such rows
 #pragma unroll
         for (int j = 0; j < 128; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -row.ref));
         const int at = row.at == kNoRow ? -1 : row.at - half * 128;
@@ -400,8 +403,7 @@ struct SoftmaxGradOps {
             for (int j = 0; j < 128; ++j)
                 if (j >= width) v[j] = 0.0f;
         }
-        T* first = ds + (long long)(tile.m * kTileM + (in_tile & ~31)) * ld_ds + tile.n * kTileN + half * 128;
-        rows_to_memory<T>(stage, v, 128, [&](int r) { return first + r * ld_ds; });
+        rows_to_memory<T>(stage, v, 128, &ds, tile.n * kTileN + half * 128, first_row);
     }
 };
 
@@ -491,24 +493,26 @@ struct HiddenGradOps {
     HiddenOut<T> out;
     int a0, b0;
     __device__ __forceinline__ TilePlan plan(int pairs) const { return shape.plan(sc->count, pairs); }
-    struct Row { int to; float c_all; };     // the caller's row, -1 behind the last one; the factor
-    __device__ __forceinline__ Row prepare(const TilePlan& plan, const TileAt& tile, int in_tile) const {
+    __device__ __forceinline__ float once(const TilePlan& plan) const { return out.scale.value(plan.count); }
+    // the caller's row, -1 behind the last one
+    __device__ __forceinline__ int prepare(const TilePlan& plan, const TileAt& tile, int in_tile) const {
         const int row = tile.m * kTileM + in_tile;
-        return {row < plan.count ? __ldg(rows + row) : -1, out.scale.value(plan.count)};
+        return row < plan.count ? __ldg(rows + row) : -1;
     }
     __device__ __forceinline__ void epilogue(const TilePlan& plan, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned stage,
-                                             const Row to) const {
+                                             const float c_all, const int to) const {
         const int col = tile.n * kTileN + half * 128, cols = shape.dim - col;
         const int first_row = tile.m * kTileM + (in_tile & ~31);
         if (tile.part >= 0) {
             float* part = parts + (long long)tile.part * (kTileM * kTileN) + (in_tile & ~31) * kTileN + half * 128;
-            rows_by_fours(stage, v, cols, 0, [](int, int, int) { return 0; },
-                          [&](int r, int, int c, float4 x, int) { *reinterpret_cast<float4*>(part + r * kTileN + c) = x; });
+            if (first_row < plan.count)
+                rows_by_fours(stage, v, cols, 0, [](int, int, int) { return 0; },
+                              [&](int r, int, int c, float4 x, int) { *reinterpret_cast<float4*>(part + r * kTileN + c) = x; });
         } else {
-            rows_by_fours(stage, v, cols, to.to,
+            rows_by_fours(stage, v, cols, to,
                           [&](int r, int to_row, int c) { return to_row >= 0 ? out.get(first_row + r, col + c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f); },
                           [&](int r, int to_row, int c, float4 x, const float4 old) {
-                              if (to_row >= 0) out.put(first_row + r, to_row, col + c, x, old, cols - c, to.c_all);
+                              if (to_row >= 0) out.put(first_row + r, to_row, col + c, x, old, cols - c, c_all);
                           });
         }
     }
@@ -531,6 +535,7 @@ xent_hidden_join_kernel(const XentScalars* __restrict__ sc, const int* __restric
         plan.place(plan.whole + tile, &m, &n);
         const int row = m * kTileM + r, col = n * kTileN + c;
         if (row >= count || col >= shape.dim) continue;
+        const int to_row = __ldg(rows + row);
         const float4* p = reinterpret_cast<const float4*>(parts + (long long)tile * plan.splits * (kTileM * kTileN) + r * kTileN + c);
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
@@ -538,36 +543,40 @@ xent_hidden_join_kernel(const XentScalars* __restrict__ sc, const int* __restric
             const float4 x = __ldcs(p + s * kPerTile);
             sum = make_float4(__fadd_rn(sum.x, x.x), __fadd_rn(sum.y, x.y), __fadd_rn(sum.z, x.z), __fadd_rn(sum.w, x.w));
         }
-        out.put(row, rows[row], col, sum, out.get(row, col), shape.dim - col, c_all);
+        out.put(row, to_row, col, sum, out.get(row, col), shape.dim - col, c_all);
     }
 }
 
-// dW of a piece: S^T [piece, rows] times X [rows, D].
-template <typename T>
+// dW of a piece: S^T [piece, rows] times X [rows, D].  MAP: not added to what is there, and stored by
+// TMA, which writes the last 16 bytes of a row whole: the columns have to be a multiple of eight.
+template <typename T, bool MAP>
 struct WeightGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
     static constexpr bool kStaging = true;
     __device__ __forceinline__ void begin() const {}
     __device__ __forceinline__ int rows_a() const { return kHalf; }
     const XentScalars* sc;
+    CUtensorMap to;              // of the caller's gradient, with MAP
     T* out;
     long long ld_out;
     GradScale scale;
     int dim, v0, v1, a0, b0;
-    bool add, vec;
+    bool add, vec;               // vec: rows begin on 16-byte boundaries
     __device__ __forceinline__ TilePlan plan(int) const {
         const int count = sc->count;
         return whole_tiles(count, (v1 - v0 + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (count + kTileK - 1) / kTileK, kGroupM);
     }
-    __device__ __forceinline__ float prepare(const TilePlan& plan, const TileAt&, int) const { return scale.value(plan.count); }
+    __device__ __forceinline__ float once(const TilePlan& plan) const { return scale.value(plan.count); }
+    __device__ __forceinline__ Nothing prepare(const TilePlan&, const TileAt&, int) const { return {}; }
     __device__ __forceinline__ void epilogue(const TilePlan&, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned stage,
-                                             const float c_all) const {
+                                             const float c_all, Nothing) const {
         const int col = tile.n * kTileN + half * 128, cols = dim - col;
         const int first_row = tile.m * kTileM + (in_tile & ~31), rows = v1 - v0 - first_row;
+        if (rows <= 0) return;
         T* first = out + (long long)(v0 + first_row) * ld_out + col;
 #pragma unroll
         for (int j = 0; j < 128; ++j) v[j] = __fmul_rn(v[j], c_all);
-        if (vec && !add) rows_to_memory<T>(stage, v, cols, [&](int r) { return r < rows ? first + r * ld_out : nullptr; });
+        if constexpr (MAP) rows_to_memory<T>(stage, v, cols, &to, col, v0 + first_row);      // a last piece's rows end with the map
         else
             rows_by_fours(stage, v, cols, 0,
                           [&](int r, int, int c) {
@@ -1004,42 +1013,44 @@ static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
     return GM_OK;
 }
 
-template <typename T>
-static int run_backward(const XentCall& c, uintptr_t hidden, uintptr_t weight, uintptr_t targets, const float* lse, const float* scale_device,
-                        float grad_scale, uintptr_t dhidden, uintptr_t dweight, bool accumulate) {
+template <typename T, bool MAP>
+static int backward_pieces(const XentCall& c, uintptr_t hidden, uintptr_t weight, uintptr_t targets, const float* lse, const float* scale_device,
+                           float grad_scale, uintptr_t dhidden, uintptr_t dweight, bool accumulate) {
     const gm_linear_xent_t* h = c.h;
     const XentSpace& s = c.s;
     const uintptr_t packed = c.ws + s.packed, ds = c.ws + s.ds;
     CUtensorMap x_k, x_mn, w_k, w_mn, ds_k, ds_mn;       // K-major for the logits and dX's S, MN-major for the rest
+    CUtensorMap ds_out, dw_out = {};                     // what the epilogues store to
     GM_TRY(make_map(&x_k, h->dtype, packed, s.cap, h->dim, s.ld_packed, kHalf));
     GM_TRY(make_map(&x_mn, h->dtype, packed, s.cap, h->dim, s.ld_packed, kTileK));
     GM_TRY(make_map(&w_k, h->dtype, weight, h->vocab, h->dim, h->ld_weight, kHalf));
     GM_TRY(make_map(&w_mn, h->dtype, weight, h->vocab, h->dim, h->ld_weight, kTileK));
     GM_TRY(make_map(&ds_k, h->dtype, ds, s.cap, s.width, s.width, kHalf));
     GM_TRY(make_map(&ds_mn, h->dtype, ds, s.cap, s.width, s.width, kTileK));
+    GM_TRY(make_map(&ds_out, h->dtype, ds, s.cap, s.width, s.width, 32));
+    if (MAP) GM_TRY(make_map(&dw_out, h->dtype, dweight, h->vocab, h->dim, h->ld_weight, 32));
     GM_TRY(index_and_gather<T>(c, hidden, targets, 0, nullptr, nullptr, nullptr, (T*)dhidden));
     const GradScale scale{scale_device, grad_scale, h->mean, 1.0f / Half16<T>::kUp};
     const int dim = (int)h->dim, vocab = (int)h->vocab;
     const int64_t m_tiles = s.cap / kTileM, d_tiles = (h->dim + kTileN - 1) / kTileN;
     using Hidden = Product<HiddenGradOps<T>, false, true>;
-    using Weight = Product<WeightGradOps<T>, true, true>;
+    using Weight = Product<WeightGradOps<T, MAP>, true, true>;
     for (int64_t v = 0; v < vocab; v += s.width) {
         const int v0 = (int)v, v1 = (int)(v + s.width < vocab ? v + s.width : vocab);
         const int64_t v_tiles = (v1 - v0 + kTileN - 1) / kTileN;
-        const SoftmaxGradOps<T> grad{c.sc(), c.target(), c.rows(), lse, (T*)ds, s.width, dim, v0, v1, logits_group(h), 0, v0};
+        const SoftmaxGradOps<T> grad{c.sc(), c.target(), c.rows(), lse, ds_out, dim, v0, v1, logits_group(h), 0, v0};
         GM_TRY((launch_tiles<kTileN>(c.d, Product<SoftmaxGradOps<T>, false, false>{x_k, w_k, grad}, m_tiles * v_tiles)));
         const HiddenPlan shape{dim, v0, v1, (int)split_parts(h)};
         const HiddenOut<T> out{(float*)(c.ws + s.carried), s.ld_carried, (T*)dhidden, h->ld_hidden, scale, v0 == 0, v1 == vocab,
                                dhidden % 16 == 0 && h->ld_hidden % 8 == 0};
         float* parts = (float*)(c.ws + s.parts);
         const Hidden dx{ds_k, w_mn, HiddenGradOps<T>{c.sc(), c.rows(), parts, shape, out, 0, v0}};
-        const Weight dw{ds_mn, x_mn, WeightGradOps<T>{c.sc(), (T*)dweight, h->ld_weight, scale, dim, v0, v1, 0, 0, accumulate, dweight % 16 == 0}};
+        const Weight dw{ds_mn, x_mn, WeightGradOps<T, MAP>{c.sc(), dw_out, (T*)dweight, h->ld_weight, scale, dim, v0, v1, 0, 0, accumulate, dweight % 16 == 0}};
         const int64_t x_turns = m_tiles * d_tiles * 16, w_turns = v_tiles * d_tiles;
         int pairs = 0;
-        // One launch of both gradients saves a start and an end and fills dX's last round: 54 -> 47 us
-        // at 256 x 512 x 10,007, 156 -> 142 us at 6,525 x 1,808 x 1,314, 1,778 -> 1,737 us at 512 x 4,096 x
-        // 131,072.  In many rounds with dX in more than two, its longer turns on a fixed schedule lose
-        // more: 4.24 -> 4.32 ms at 8,862 x 1,384 x 55,838.
+        // One launch of both gradients saves a start and an end and fills dX's last round: 46 -> 43 us
+        // at 256 x 512 x 10,007, 136 -> 131 us at 6,525 x 1,808 x 1,314.  In many rounds with dX in more than
+        // two, its longer turns on a fixed schedule lose more: 4.12 -> 4.23 ms at 8,862 x 1,384 x 55,838.
         const int64_t per_round = c.d->sm_count / 2;
         const bool both = dhidden && dweight && ((m_tiles + v_tiles) * d_tiles <= 16 * per_round || m_tiles * d_tiles <= 2 * per_round);
         if (both) GM_TRY((launch_tiles<kTileN>(c.d, dx, x_turns + w_turns, &pairs, dw)));
@@ -1053,6 +1064,13 @@ static int run_backward(const XentCall& c, uintptr_t hidden, uintptr_t weight, u
         if (dweight && !both) GM_TRY((launch_tiles<kTileN>(c.d, dw, w_turns)));
     }
     return GM_OK;
+}
+
+template <typename T>
+static int run_backward(const XentCall& c, uintptr_t hidden, uintptr_t weight, uintptr_t targets, const float* lse, const float* scale_device,
+                        float grad_scale, uintptr_t dhidden, uintptr_t dweight, bool accumulate) {
+    const bool map = dweight && dweight % 16 == 0 && c.h->dim % 8 == 0 && !accumulate;
+    return (map ? backward_pieces<T, true> : backward_pieces<T, false>)(c, hidden, weight, targets, lse, scale_device, grad_scale, dhidden, dweight, accumulate);
 }
 
 }  // namespace gm

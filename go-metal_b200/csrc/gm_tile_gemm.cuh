@@ -30,6 +30,7 @@
 
 #include <cuda.h>
 
+#include <climits>
 #include <type_traits>
 
 #include "gm_lm.cuh"
@@ -162,41 +163,38 @@ __device__ __forceinline__ uint4 stage_get(unsigned stage, int row, int unit) {
     return x;
 }
 
-// 128 columns of 32 rows in a 16-bit type: to(row in the warp) is where its first column goes, null
-// for a row that is not written; `cols` columns exist; rows begin on 16-byte boundaries.
-template <typename T, typename To>
-__device__ __forceinline__ void rows_to_memory(unsigned stage, const float (&v)[128], int cols, To to) {
+// The staging is this warp's again: the stores that read it have done so.
+__device__ __forceinline__ void stage_free() {
+    if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+}
+
+// 128 columns of 32 rows in a 16-bit type to a map's rows from y on and columns from x on (a multiple of
+// 64), by TMA stores that run on while the warp takes its next tile; rows and 16-byte words outside the map
+// are not written, `cols` columns exist.  The staging is what the map's 128-byte swizzle says.  Read
+// back and stored by the warp itself, a tile's epilogue took 6,000 cycles, more than the product of
+// a short K: dW at 64 x 2,048 x 50,257 168 -> 120 us, a backward pass of 1,002 x 1,184 x 10,878 157 -> 103 us.
+template <typename T>
+__device__ __forceinline__ void rows_to_memory(unsigned stage, const float (&v)[128], int cols, const CUtensorMap* map, int x, int y) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int c = 0; c < 128; c += 64) {
         if (c >= cols) break;
-        __syncwarp();
+        stage_free();
 #pragma unroll
         for (int u = 0; u < 8; ++u)
             stage_put(stage, lane, u, make_uint4(pack2<T>(v[c + 8 * u], v[c + 8 * u + 1]), pack2<T>(v[c + 8 * u + 2], v[c + 8 * u + 3]),
                                                  pack2<T>(v[c + 8 * u + 4], v[c + 8 * u + 5]), pack2<T>(v[c + 8 * u + 6], v[c + 8 * u + 7])));
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        const int unit = lane & 7, at = c + unit * 8;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int row = i * 4 + (lane >> 3);
-            const uint4 x = stage_get(stage, row, unit);
-            T* p = to(row);
-            if (p == nullptr) continue;
-            if (at + 8 <= cols) {
-                *reinterpret_cast<uint4*>(p + at) = x;
-            } else {
-                const unsigned w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (at + k < cols) reinterpret_cast<unsigned short*>(p)[at + k] = (unsigned short)(w[k >> 1] >> (16 * (k & 1)));
-            }
-        }
+        if (lane == 0)
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\t"
+                         "cp.async.bulk.commit_group;" ::"l"(map), "r"(x + c), "r"(y), "r"(stage) : "memory");
     }
 }
 
 // 128 columns of 32 rows as they are (binary32), four at a time, neighbouring lanes with neighbouring
-// columns: first old = get(row in the warp, that row's lane's tag, column) for eight of them, so that
+// columns: first old = get(row in the warp, that row's lane's tag, column) for four of them, so that
 // what is read is in flight together, then put(row, tag, column, four values, old).
 template <typename Get, typename Put>
 __device__ __forceinline__ void rows_by_fours(unsigned stage, const float (&v)[128], int cols, int tag, Get get, Put put) {
@@ -204,25 +202,27 @@ __device__ __forceinline__ void rows_by_fours(unsigned stage, const float (&v)[1
 #pragma unroll
     for (int c = 0; c < 128; c += 32) {
         if (c >= cols) break;
-        __syncwarp();
+        stage_free();
 #pragma unroll
         for (int u = 0; u < 8; ++u)
             stage_put(stage, lane, u, make_uint4(__float_as_uint(v[c + 4 * u]), __float_as_uint(v[c + 4 * u + 1]), __float_as_uint(v[c + 4 * u + 2]),
                                                  __float_as_uint(v[c + 4 * u + 3])));
         __syncwarp();
         const int unit = lane & 7, at = c + unit * 4;
-        decltype(get(0, 0, 0)) old[8];
-        int tags[8];
+#pragma unroll 1
+        for (int r = lane >> 3; r < 32; r += 16) {
+            decltype(get(0, 0, 0)) old[4];
+            int tags[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            tags[i] = __shfl_sync(0xffffffffu, tag, i * 4 + (lane >> 3));
-            if (at < cols) old[i] = get(i * 4 + (lane >> 3), tags[i], at);
-        }
+            for (int i = 0; i < 4; ++i) {
+                tags[i] = __shfl_sync(0xffffffffu, tag, r + i * 4);
+                if (at < cols) old[i] = get(r + i * 4, tags[i], at);
+            }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int row = i * 4 + (lane >> 3);
-            const uint4 x = stage_get(stage, row, unit);
-            if (at < cols) put(row, tags[i], at, make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w)), old[i]);
+            for (int i = 0; i < 4; ++i) {
+                const uint4 x = stage_get(stage, r + i * 4, unit);
+                if (at < cols) put(r + i * 4, tags[i], at, make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w)), old[i]);
+            }
         }
     }
 }
@@ -267,17 +267,20 @@ __device__ __forceinline__ TilePlan whole_tiles(int count, int m_tiles, int n_ti
 
 // Splits the tiles behind the last full round of `pairs` (or of the round before, too), into at
 // most 16 shares each and `most_parts` in all, for the shortest run: rounds of turns, each as long as
-// its k-blocks plus a start and an epilogue (about eight).
+// its k-blocks plus a start and an epilogue (about eight).  Called by whole warps: each lane weighs one
+// of the 30 choices (weighed one after the other they took 3 us at the start of two kernels).
 __device__ __forceinline__ void split_tail(TilePlan* p, int pairs, int most_parts) {
-    const int tiles = p->tiles(), k = p->k_blocks;
-    p->whole = tiles;
-    p->splits = 1;
-    int best = (tiles + pairs - 1) / pairs * (k + 8);
-    for (int tail = tiles % pairs; tail <= tiles && tail <= tiles % pairs + pairs; tail += pairs)
-        for (int s = 2; s <= 16 && s <= k && tail * s <= most_parts; ++s) {
-            const int cost = (tiles - tail) / pairs * (k + 8) + (tail * s + pairs - 1) / pairs * ((k + s - 1) / s + 8) + 8;
-            if (tail > 0 && cost < best) { best = cost; p->whole = tiles - tail; p->splits = s; }
-        }
+    const int tiles = p->tiles(), k = p->k_blocks, lane = threadIdx.x & 31;
+    const int tail = tiles % pairs + (lane >= 15 ? pairs : 0), s = 2 + (lane >= 15 ? lane - 15 : lane);
+    const bool possible = lane < 30 && tail > 0 && tail <= tiles && s <= k && tail * s <= most_parts;
+    const int cost = (tiles - tail) / pairs * (k + 8) + (tail * s + pairs - 1) / pairs * ((k + s - 1) / s + 8) + 8;
+    const int best = __reduce_min_sync(0xffffffffu, possible ? cost : INT_MAX);
+    const unsigned at = __ballot_sync(0xffffffffu, possible && cost == best);
+    const bool split = at != 0u && best < (tiles + pairs - 1) / pairs * (k + 8);
+    const int from = at != 0u ? __ffs((int)at) - 1 : 0;
+    const int best_tail = __shfl_sync(0xffffffffu, tail, from), best_s = __shfl_sync(0xffffffffu, s, from);
+    p->whole = split ? tiles - best_tail : tiles;
+    p->splits = split ? best_s : 1;
 }
 
 // A product: the operands' maps, which of them are MN-major, and Ops, which provides
@@ -286,11 +289,12 @@ __device__ __forceinline__ void split_tail(TilePlan* p, int pairs, int most_part
 //   begin()           run by one thread before anything else
 //   rows_a()          rows of A per CTA, 128 or a smaller multiple of 8 (K-major A only); the box of
 //                     its map has as many, the accumulators' other rows hold anything
-//   plan(pairs)       the tiles, read on the device
+//   plan(pairs)       the tiles, read on the device by whole warps
 //   a0, b0            first row of A and of B (first K-row of an MN-major operand) in their maps
+//   once(plan)        what the epilogues of all turns need
 //   prepare(plan, at, row)   what the epilogue of this turn needs for the row inside the tile, read
 //                     while the product runs
-//   epilogue(plan, at, row, v, half, stage, prepared)   the row inside the tile, half of its
+//   epilogue(plan, at, row, v, half, stage, once, prepared)   the row inside the tile, half of its
 //                     columns (zeros with an empty share of K), which half, 4 KB of shared memory for
 //                     the warp (with kStaging); called by whole warps, also for rows behind the last one
 template <typename Ops_, bool MN_A, bool MN_B>
@@ -301,6 +305,7 @@ struct Product {
     Ops ops;
     __device__ __forceinline__ TilePlan plan(int pairs) const { return ops.plan(pairs); }
 };
+struct Nothing {};
 struct NoProduct {
     static constexpr bool kAny = false;
     __device__ __forceinline__ TilePlan plan(int) const { return {0, 0, 0, 0, 1, 0, 1}; }
@@ -436,7 +441,7 @@ tile_gemm_kernel(const __grid_constant__ First first, const __grid_constant__ Se
         const unsigned staging = ring + kStages * kStageBytes + (warp - 2) * kStagingBytes;
         constexpr int kColumns = TN / 2 < 32 ? 32 : TN / 2;       // a narrow tile is all the first half's
         int count = 0;
-        auto finish = [&](const auto& product, const TilePlan& tiles, const TileAt at) {
+        auto finish = [&](const auto& product, const TilePlan& tiles, const auto& once, const TileAt at) {
             const int slot = count & 1;
             const auto prepared = product.ops.prepare(tiles, at, row);
             const bool ok = mbar_wait(smem_u32(&acc_full[slot]), (count >> 1) & 1, &abort_flag, budget);
@@ -451,15 +456,21 @@ tile_gemm_kernel(const __grid_constant__ First first, const __grid_constant__ Se
 #pragma unroll
                 for (int j = 0; j < kColumns; ++j) v[j] = 0.0f;
             }
-            product.ops.epilogue(tiles, at, row, v, half, staging, prepared);
+            product.ops.epilogue(tiles, at, row, v, half, staging, once, prepared);
             return true;
         };
+        const auto once = first.ops.once(plan);
+        const auto once2 = [&] {
+            if constexpr (Second::kAny) return second.ops.once(plan2);
+            else return Nothing{};
+        }();
         bool ok = true;
         for (int t = pair; t < all && ok; t += pairs, ++count) {
             if constexpr (Second::kAny)
-                if (t >= items) { ok = finish(second, plan2, plan2.at(t - items)); continue; }
-            ok = finish(first, plan, plan.at(t));
+                if (t >= items) { ok = finish(second, plan2, once2, plan2.at(t - items)); continue; }
+            ok = finish(first, plan, once, plan.at(t));
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncwarp();
     __syncthreads();
