@@ -9,7 +9,7 @@
 // the target's, then a small kernel joins them with the target's logit, which comes from a dot
 // product of its own.  loss = log(1 + sum of the others / the target's) then loses nothing when the
 // model is sure of the target, and the target's logit is as good as binary32 makes it (the
-// tensor cores cut where they add).  Backward: for one piece of the vocabulary after the other the logits
+// tensor cores cut where they add; the other logits' long sums are taken in parts for that).  Backward: for one piece of the vocabulary after the other the logits
 // are formed again, S goes to the workspace in 16 bits, and two products take it from there;
 // dX is carried from piece to piece in binary32.  8 N D V operations for a training step: 2
 // forward, 2 again for the logits, 4 for the gradients.  Bound by the tensor cores, for a few
@@ -238,10 +238,12 @@ constexpr int kGroupM = 8;      // m-tiles walked together in the gradient produ
 
 // Row maximum and sum of exponentials of half a tile's logits (128), the target's left out.
 struct Goal { int at; };        // a row's target
-template <typename T>
+// LONG: for more than kOneSum columns.
+template <typename T, bool LONG>
 struct StatsOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
     static constexpr bool kStaging = false;
+    static constexpr bool kLong = LONG;
     __device__ __forceinline__ void begin() const {}
     __device__ __forceinline__ int rows_a() const { return kHalf; }
     const XentScalars* sc;
@@ -307,10 +309,11 @@ template <bool MAX> __device__ __forceinline__ float lanes_to_columns(float (&v)
     return v[0];
 }
 
-template <typename T, int TN>
+template <typename T, int TN, bool LONG>
 struct FewStatsOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
     static constexpr bool kStaging = false;
+    static constexpr bool kLong = LONG;
     static constexpr int kColumns = TN / 2 < 32 ? 32 : TN / 2;
     XentScalars* sc;
     const int* target;           // by row of the caller
@@ -361,6 +364,7 @@ template <typename T>
 struct SoftmaxGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
     static constexpr bool kStaging = true;
+    static constexpr bool kLong = false;
     __device__ __forceinline__ void begin() const {}
     __device__ __forceinline__ int rows_a() const { return kHalf; }
     const XentScalars* sc;
@@ -484,6 +488,7 @@ template <typename T>
 struct HiddenGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
     static constexpr bool kStaging = true;
+    static constexpr bool kLong = false;
     __device__ __forceinline__ void begin() const {}
     __device__ __forceinline__ int rows_a() const { return kHalf; }
     const XentScalars* sc;
@@ -553,6 +558,7 @@ template <typename T, bool MAP>
 struct WeightGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
     static constexpr bool kStaging = true;
+    static constexpr bool kLong = false;
     __device__ __forceinline__ void begin() const {}
     __device__ __forceinline__ int rows_a() const { return kHalf; }
     const XentScalars* sc;
@@ -976,8 +982,10 @@ static int forward_few(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
         c.d->launches++;
     }
     float2* stats = (float2*)(c.ws + s.stats);
-    const FewStatsOps<T, TN> ops{c.sc(), (const int*)targets, stats, (int)h->tokens, (int)s.cap, (int)h->dim, (int)h->vocab, height, 0, 0};
-    GM_TRY((launch_tiles<TN>(c.d, Product<FewStatsOps<T, TN>, false, false>{map_w, map_x, ops}, tiles)));
+    auto product = [&](auto ops) { return launch_tiles<TN>(c.d, Product<decltype(ops), false, false>{map_w, map_x, ops}, tiles); };
+    const int n = (int)h->tokens, cap = (int)s.cap, dim = (int)h->dim, vocab = (int)h->vocab;
+    if (dim > kOneSum) GM_TRY(product(FewStatsOps<T, TN, true>{c.sc(), (const int*)targets, stats, n, cap, dim, vocab, height, 0, 0}));
+    else GM_TRY(product(FewStatsOps<T, TN, false>{c.sc(), (const int*)targets, stats, n, cap, dim, vocab, height, 0, 0}));
     GM_CUDA_CHECK(launch_chained(xent_few_join_kernel<T>, dim3((unsigned)h->tokens), dim3(256), 0, c.d->stream, c.sc(), (const T*)hidden, h->ld_hidden,
                                  (const T*)weight, h->ld_weight, (const int*)targets, (int)h->dim, (int)h->vocab, stats, (int)s.cap, (int)tiles * 8, losses, lse,
                                  (float*)(c.ws + s.partial), total, h->mean, reinterpret_cast<const int*>(c.d->scalars + kXentStatusWord)));
@@ -1002,8 +1010,10 @@ static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
     float2* stats = (float2*)(c.ws + s.stats);
     const int64_t n_tiles = (h->vocab + kTileN - 1) / kTileN;
     const int tiles = (int)((h->vocab + kTileN / 2 - 1) / (kTileN / 2));
-    const StatsOps<T> ops{c.sc(), c.target(), stats, (int)s.cap, (int)h->dim, (int)h->vocab, logits_group(h), 0, 0};
-    GM_TRY((launch_tiles<kTileN>(c.d, Product<StatsOps<T>, false, false>{map_x, map_w, ops}, s.cap / kTileM * n_tiles)));
+    auto product = [&](auto ops) { return launch_tiles<kTileN>(c.d, Product<decltype(ops), false, false>{map_x, map_w, ops}, s.cap / kTileM * n_tiles); };
+    const int cap = (int)s.cap, dim = (int)h->dim, vocab = (int)h->vocab;
+    if (dim > kOneSum) GM_TRY(product(StatsOps<T, true>{c.sc(), c.target(), stats, cap, dim, vocab, logits_group(h), 0, 0}));
+    else GM_TRY(product(StatsOps<T, false>{c.sc(), c.target(), stats, cap, dim, vocab, logits_group(h), 0, 0}));
     // a CTA per row up to a few rows per SM, 8 rows per CTA beyond
     auto join = h->tokens <= 1024 ? xent_join_kernel<1> : xent_join_kernel<8>;
     const int64_t ctas = h->tokens <= 1024 ? h->tokens : s.cap / 8;

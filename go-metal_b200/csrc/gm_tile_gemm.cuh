@@ -146,6 +146,22 @@ __device__ __forceinline__ void tmem_read(unsigned addr, float (&v)[COUNT]) {
     for (int i = 0; i < COUNT; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// The same, added to what v holds; eight columns at a time, which leaves v its registers.
+template <int COUNT>
+__device__ __forceinline__ void tmem_add(unsigned addr, float (&v)[COUNT]) {
+#pragma unroll
+    for (int c = 0; c < COUNT; c += 8) {
+        unsigned r[8];
+        __syncwarp();
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+                     "tcgen05.wait::ld.sync.aligned;"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                     : "r"(addr + c) : "memory");
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[c + k] = __fadd_rn(v[c + k], __uint_as_float(r[k]));
+    }
+}
+
 // ---- rows to memory ----
 // A warp holds 32 rows, one per lane.  Stored as they are, each lane's 16 bytes would be a line of
 // their own, and a line is a cycle of the memory that feeds the tensor core; so they go through 4 KB of
@@ -230,6 +246,19 @@ __device__ __forceinline__ void rows_by_fours(unsigned stage, const float (&v)[1
 // The work of one turn: a tile, its share of K, and the part it leaves (-1: the whole tile).
 struct TileAt { int m, n, part, k0, k1; };
 
+// How many sums a turn's K is cut into where it is to be cut.  The tensor cores cut where
+// they add, which shifts a sum of n blocks of 64 towards zero by up to n 2^-23 of it, and a mean loss
+// with it: with one sum, by 4.7e-6 of itself at 8,192 columns, 1.3e-6 at 4,096 and 3.4e-7 at 2,048.
+// Every sum more costs a read of the accumulators, 570 cycles: 2,048 columns in two sums 3.5 % (1.7e-7),
+// 4,096 in two 2 % (6.9e-7).  So: one up to kOneSum columns, two up to 4,096, 1,536 each beyond (the
+// logits grow with the columns, and the shift is in proportion to both).
+constexpr int kOneSum = 2048;
+template <bool LONG>
+__device__ __forceinline__ int chunks_of(const TileAt& at) {
+    const int n = at.k1 - at.k0;
+    return !LONG ? 1 : n <= 64 ? 2 : (n + 23) / 24;
+}
+
 // One product: m_tiles x n_tiles tiles, walked m first inside groups of `group` m-tiles, so that
 // the operands of the tiles in flight are shared in L2.  The first `whole` tiles are a turn each, the
 // others `splits` turns, each with a share of K.
@@ -286,6 +315,7 @@ __device__ __forceinline__ void split_tail(TilePlan* p, int pairs, int most_part
 // A product: the operands' maps, which of them are MN-major, and Ops, which provides
 //   kBf16             whether the inputs are bf16 (else fp16)
 //   kStaging          whether the epilogue wants shared memory
+//   kLong             whether K is cut into several sums, which the epilogue's warps add up
 //   begin()           run by one thread before anything else
 //   rows_a()          rows of A per CTA, 128 or a smaller multiple of 8 (K-major A only); the box of
 //                     its map has as many, the accumulators' other rows hold anything
@@ -404,26 +434,31 @@ tile_gemm_kernel(const __grid_constant__ First first, const __grid_constant__ Se
             const unsigned in = P::Ops::kBf16 ? 1u : 0u;
             const unsigned idesc = (1u << 4) | (in << 7) | (in << 10) | ((P::kMnA ? 1u : 0u) << 15) | ((P::kMnB ? 1u : 0u) << 16) |
                                    ((unsigned)(TN / 8) << 17) | ((unsigned)(kTileM / 16) << 24);
-            const int slot = count & 1;
-            if (!mbar_wait(smem_u32(&acc_empty[slot]), ((count >> 1) & 1) ^ 1, &abort_flag, budget)) return false;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const unsigned d = tmem + (unsigned)slot * 256u;
-            for (int k = at.k0; k < at.k1; ++k, ++used) {
-                const int s = used % kStages;
-                if (!mbar_wait(smem_u32(&full[s]), (used / kStages) & 1u, &abort_flag, budget)) return false;
+            const int chunks = chunks_of<P::Ops::kLong>(at);
+            for (int c = 0; c < chunks; ++c, ++count) {
+                const int slot = count & 1;
+                if (!mbar_wait(smem_u32(&acc_empty[slot]), ((count >> 1) & 1) ^ 1, &abort_flag, budget)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const unsigned a = ring + s * kStageBytes;
-                const unsigned long long da = mat_desc(a, P::kMnA), db = mat_desc(a + kOperandBytes, P::kMnB);
+                const unsigned d = tmem + (unsigned)slot * 256u;
+                const long long n = at.k1 - at.k0;
+                const int k0 = at.k0 + (int)(n * c / chunks), k1 = at.k0 + (int)(n * (c + 1) / chunks);
+                for (int k = k0; k < k1; ++k, ++used) {
+                    const int s = used % kStages;
+                    if (!mbar_wait(smem_u32(&full[s]), (used / kStages) & 1u, &abort_flag, budget)) return false;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned a = ring + s * kStageBytes;
+                    const unsigned long long da = mat_desc(a, P::kMnA), db = mat_desc(a + kOperandBytes, P::kMnB);
 #pragma unroll
-                for (int i = 0; i < kTileK / 16; ++i)
-                    mma_pair(d, da + (P::kMnA ? 128 * i : 2 * i), db + (P::kMnB ? 128 * i : 2 * i), idesc, k > at.k0 || i > 0);
-                mma_commit_pair(smem_u32(&empty[s]));
+                    for (int i = 0; i < kTileK / 16; ++i)
+                        mma_pair(d, da + (P::kMnA ? 128 * i : 2 * i), db + (P::kMnB ? 128 * i : 2 * i), idesc, k > k0 || i > 0);
+                    mma_commit_pair(smem_u32(&empty[s]));
+                }
+                mma_commit_pair(smem_u32(&acc_full[slot]));
             }
-            mma_commit_pair(smem_u32(&acc_full[slot]));
             return true;
         };
         bool ok = true;
-        for (int t = pair; t < all && ok; t += pairs, ++count) {
+        for (int t = pair; t < all && ok; t += pairs) {
             if constexpr (Second::kAny)
                 if (t >= items) { ok = multiply(second, plan2.at(t - items)); continue; }
             ok = multiply(first, plan.at(t));
@@ -442,16 +477,27 @@ tile_gemm_kernel(const __grid_constant__ First first, const __grid_constant__ Se
         constexpr int kColumns = TN / 2 < 32 ? 32 : TN / 2;       // a narrow tile is all the first half's
         int count = 0;
         auto finish = [&](const auto& product, const TilePlan& tiles, const auto& once, const TileAt at) {
-            const int slot = count & 1;
             const auto prepared = product.ops.prepare(tiles, at, row);
-            const bool ok = mbar_wait(smem_u32(&acc_full[slot]), (count >> 1) & 1, &abort_flag, budget);
-            if (!__all_sync(0xffffffffu, ok)) return false;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float v[kColumns];
-            tmem_read<kColumns>(tmem + (unsigned)(slot * 256 + half * kColumns) + ((unsigned)(quarter * 32) << 16), v);
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(pair_leader_addr(smem_u32(&acc_empty[slot])));
+            auto take = [&](const bool first_sum) {
+                const int slot = count & 1;
+                const bool ok = mbar_wait(smem_u32(&acc_full[slot]), (count >> 1) & 1, &abort_flag, budget);
+                if (!__all_sync(0xffffffffu, ok)) return false;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const unsigned from = tmem + (unsigned)(slot * 256 + half * kColumns) + ((unsigned)(quarter * 32) << 16);
+                if (first_sum) tmem_read<kColumns>(from, v);
+                else tmem_add<kColumns>(from, v);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(pair_leader_addr(smem_u32(&acc_empty[slot])));
+                ++count;
+                return true;
+            };
+            if (!take(true)) return false;
+            using Ops = typename std::decay_t<decltype(product)>::Ops;
+            if constexpr (Ops::kLong)
+                for (int c = chunks_of<true>(at); c > 1; --c)
+                    if (!take(false)) return false;
             if (at.k0 == at.k1) {
 #pragma unroll
                 for (int j = 0; j < kColumns; ++j) v[j] = 0.0f;
@@ -465,7 +511,7 @@ tile_gemm_kernel(const __grid_constant__ First first, const __grid_constant__ Se
             else return Nothing{};
         }();
         bool ok = true;
-        for (int t = pair; t < all && ok; t += pairs, ++count) {
+        for (int t = pair; t < all && ok; t += pairs) {
             if constexpr (Second::kAny)
                 if (t >= items) { ok = finish(second, plan2, once2, plan2.at(t - items)); continue; }
             ok = finish(first, plan, once, plan.at(t));

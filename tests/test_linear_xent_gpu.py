@@ -304,6 +304,29 @@ def test_infinite_logits(gm, dev, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [64, 192])
+def test_long_sums_do_not_shift_the_loss(gm, dev, n):
+    """The tensor cores cut where they add, 16 products at a time: half a unit in the last place on average, at most 2^-24 of
+    the sum so far, always towards zero.  The forward pass takes 8,192 columns in six sums, so a mean loss is off by at most
+    2^-24 of the sums so far of those, weighted with the probabilities (rounding errors average out over rows and entries); in
+    one sum it would be off by about twice that bound."""
+    x, w, t = make(BF16, n, 8192, 640, 33)
+    w = R.rounded(w * (0.02 * np.sqrt(8192)), BF16)
+    call = Call(gm, dev, BF16, x, w, t)
+    total = call.forward()[2][0]
+    call.close()
+    X, W = torch.from_numpy(x).cuda().view(n, 512, 16), torch.from_numpy(w).cuda().view(640, 512, 16)
+    steps = torch.einsum("nsk,vsk->snv", X, W)
+    l = steps.sum(0)
+    ends = [4 * (128 * c // 6) for c in range(7)]                     # a block of 64 columns is four steps
+    so_far = sum(steps[a:b].cumsum(0).abs().sum(0) for a, b in zip(ends, ends[1:]))
+    p = torch.softmax(l, 1)
+    want = float(torch.nn.functional.cross_entropy(l, torch.from_numpy(t.astype(np.int64)).cuda()))
+    bound = float((p * so_far).sum(1).mean()) * 2.0 ** -24
+    assert abs(total - want) <= bound + 2.0 ** -22 * want
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences(gm, dev):
     """The summed loss along a direction: a central difference of the library's own forward pass, whose
     step leaves at most h^2 of third derivatives (bounded by |d|^3) and 2 error(total) / h of rounding."""
