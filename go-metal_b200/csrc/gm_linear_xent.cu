@@ -1058,9 +1058,9 @@ static int backward_pieces(const XentCall& c, uintptr_t hidden, uintptr_t weight
         const Weight dw{ds_mn, x_mn, WeightGradOps<T, MAP>{c.sc(), dw_out, (T*)dweight, h->ld_weight, scale, dim, v0, v1, 0, 0, accumulate, dweight % 16 == 0}};
         const int64_t x_turns = m_tiles * d_tiles * 16, w_turns = v_tiles * d_tiles;
         int pairs = 0;
-        // One launch of both gradients saves a start and an end and fills dX's last round: 46 -> 43 us
-        // at 256 x 512 x 10,007, 136 -> 131 us at 6,525 x 1,808 x 1,314.  In many rounds with dX in more than
-        // two, its longer turns on a fixed schedule lose more: 4.12 -> 4.23 ms at 8,862 x 1,384 x 55,838.
+        // One launch of both gradients saves a start and an end and fills dX's last round: 39 -> 35 us
+        // at 256 x 512 x 10,007, 132 -> 127 us at 6,525 x 1,808 x 1,314.  In many rounds with dX in more than
+        // two, its longer turns on a fixed schedule lose more: 4.07 -> 4.15 ms at 8,862 x 1,384 x 55,838.
         const int64_t per_round = c.d->sm_count / 2;
         const bool both = dhidden && dweight && ((m_tiles + v_tiles) * d_tiles <= 16 * per_round || m_tiles * d_tiles <= 2 * per_round);
         if (both) GM_TRY((launch_tiles<kTileN>(c.d, dx, x_turns + w_turns, &pairs, dw)));

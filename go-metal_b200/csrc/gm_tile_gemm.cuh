@@ -62,9 +62,8 @@ __device__ __forceinline__ unsigned pair_leader_addr(unsigned addr) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
     return r;
 }
-// Relaxed: it says that TMEM has been read (tcgen05.wait::ld and the fence in front of it), nothing else.  A
-// release would first wait for the lane's stores to memory, which cost a tile's
-// epilogue 1,100 to 1,700 cycles (16,000 x 256 x 16,000 backward 530 -> 504 us, 64 x 2,048 x 50,257 174 -> 159 us).
+// Relaxed: it says that TMEM has been read (tcgen05.wait::ld and the fence in front of it), nothing else.
+// A release would first wait for the lane's stores to memory, which cost a tile's epilogue 1,100 to 1,700 cycles (16,000 x 256 x 16,000 backward 530 -> 504 us, 64 x 2,048 x 50,257 174 -> 159 us).
 __device__ __forceinline__ void mbar_arrive_cluster(unsigned cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
@@ -192,7 +191,7 @@ __device__ __forceinline__ void stage_free() {
 // 64), by TMA stores that run on while the warp takes its next tile; rows and 16-byte words outside the map
 // are not written, `cols` columns exist.  The staging is what the map's 128-byte swizzle says.  Read
 // back and stored by the warp itself, a tile's epilogue took 6,000 cycles, more than the product of
-// a short K: dW at 64 x 2,048 x 50,257 168 -> 120 us, a backward pass of 1,002 x 1,184 x 10,878 157 -> 103 us.
+// a short K: logits and dW at 64 x 2,048 x 50,257 168 -> 120 us, a backward pass of 1,002 x 1,184 x 10,878 157 -> 103 us.
 template <typename T>
 __device__ __forceinline__ void rows_to_memory(unsigned stage, const float (&v)[128], int cols, const CUtensorMap* map, int x, int y) {
     const int lane = threadIdx.x & 31;

@@ -336,7 +336,8 @@ int gm_dot_canonical_static(uintptr_t a, uintptr_t b, int64_t n, uintptr_t out_d
  * and hold nothing between calls; two calls or captured graphs that can run at the same
  * time need workspaces of their own.  Matrices are row-major with a row stride (ld, in
  * elements) of at least their columns, below 2^31 rows and at most 2^30 columns.  Buffers are read and written only inside the
- * rows and columns named. */
+ * rows and columns named.  What a call writes overlaps nothing else it reads or writes, except where
+ * it says so. */
 
 /* Element types: the codes of memory/tensor.go:12-17, and one more for bfloat16. */
 enum { GM_F32 = 0, GM_F16 = 2, GM_BF16 = 4 };
