@@ -62,8 +62,9 @@ __device__ __forceinline__ unsigned pair_leader_addr(unsigned addr) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
     return r;
 }
-// Relaxed: it says that TMEM has been read (tcgen05.wait::ld and the fence in front of it), nothing else.
-// A release would first wait for the lane's stores to memory, which cost a tile's epilogue 1,100 to 1,700 cycles (16,000 x 256 x 16,000 backward 530 -> 504 us, 64 x 2,048 x 50,257 174 -> 159 us).
+// Relaxed: it says that TMEM has been read (tcgen05.wait::ld and the fence in front of it), nothing
+// else.  A release would first wait for the lane's stores to memory, which cost a tile's epilogue 1,100
+// to 1,700 cycles (16,000 x 256 x 16,000 backward 530 -> 504 us, 64 x 2,048 x 50,257 174 -> 159 us).
 __device__ __forceinline__ void mbar_arrive_cluster(unsigned cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
