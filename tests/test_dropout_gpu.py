@@ -179,3 +179,25 @@ def test_refuses_a_device_offset_shorter_than_a_word(gm, dev):
     assert gm.last_error() and gm.lib.gm_device_launch_count(dev.h) == before
     dev.free(b)
     dev.free(word)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [0, 2, 4])
+@pytest.mark.parametrize("rows,cols,ld", [(200, 13, 15), (64, 4091, 4091), (64, 4091, 4093), (40, 1000, 1001)])
+def test_in_place_at_odd_addresses(gm, dev, dtype, rows, cols, ld):
+    """Groups of eight share 16-byte words with their neighbours there, which other threads write meanwhile."""
+    rng = np.random.default_rng(cols)
+    x, res = R.rounded(rng.standard_normal((rows, cols)), dtype), R.rounded(rng.standard_normal((rows, cols)), dtype)
+    want = expected(x, res, 0.25, 1, 2, dtype)
+    eb = R.eb(dtype)
+    for target in ("x", "res"):
+        dx, dr = (dev.to_device(np.concatenate([np.zeros(eb, np.uint8), R.bytes_of(R.strided(a, ld, dtype), dtype), np.zeros(64, np.uint8)])) for a in (x, res))
+        y = dx if target == "x" else dr
+        gm.check(gm.lib.gm_dropout_async(dev.h, dtype, rows, cols, dx + eb, ld, dr + eb, ld, y + eb, ld, gm.dropout(0.25, 1, 2)), "dropout")
+        got = dev.to_host(y, eb + rows * ld * eb + 64, np.uint8)
+        assert not got[:eb].any() and not got[eb + rows * ld * eb:].any(), "bytes around the matrix were written"
+        body = got[eb:eb + rows * ld * eb].reshape(rows, ld * eb)
+        assert np.array_equal(body[:, :cols * eb].reshape(-1), want)
+        assert np.all(R.values_of(body[:, cols * eb:].copy().reshape(-1), dtype) == -7.0), "columns behind the row were written"
+        dev.free(dx)
+        dev.free(dr)
