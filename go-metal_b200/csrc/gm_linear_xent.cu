@@ -234,6 +234,12 @@ xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n
 }
 
 // ---------------------------------------------------------------- epilogues
+// The exponentials of a piece are 2^(l log2e - ref) with ref = m log2e rounded, one operation each; their
+// sum is then relative to 2^ref, not to e^m, and those are apart by the rounding of ref (up to 11 units in the last
+// place at m = 20, a hundred at 200).  This takes it out, once per piece; 1 where the piece holds nothing but -inf.
+__device__ __forceinline__ float reference_of(const float m) { return m == -INFINITY ? 0.0f : m * kLog2e; }
+__device__ __forceinline__ float off_reference(const float m, const float ref) { return m == -INFINITY ? 1.0f : exp2f(-fmaf(m, kLog2e, -ref)); }
+
 constexpr int kGroupM = 8;      // m-tiles walked together in the gradient products
 
 // Row maximum and sum of exponentials of half a tile's logits (128), the target's left out.
@@ -281,11 +287,11 @@ struct StatsOps {
 #pragma unroll
         for (int j = 8; j < 128; ++j) top[j & 7] = fmaxf(top[j & 7], v[j]);
         const float m = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
-        const float ref = m == -INFINITY ? 0.0f : m * kLog2e;              // nothing but -inf: exponentials are zero
+        const float ref = reference_of(m);
 #pragma unroll
         for (int j = 0; j < 128; ++j) sum[j & 7] += exp2_fast(fmaf(v[j], kLog2e, -ref));
         const float s = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
-        if (row < plan.count) stats[(long long)(2 * tile.n + half) * rows_cap + row] = make_float2(m, s);
+        if (row < plan.count) stats[(long long)(2 * tile.n + half) * rows_cap + row] = make_float2(m, s * off_reference(m, ref));
     }
 };
 
@@ -350,11 +356,11 @@ struct FewStatsOps {
 #pragma unroll
             for (int j = 0; j < 32; ++j) w[j] = v[j];
             const float top = lanes_to_columns<true>(w, lane);
-            const float ref = top == -INFINITY ? 0.0f : top * kLog2e;
+            const float ref = reference_of(top);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -__shfl_sync(0xffffffffu, ref, j)));
             const float sum = lanes_to_columns<false>(v, lane);
-            if (c + lane < n) to[c + lane] = make_float2(top, sum);
+            if (c + lane < n) to[c + lane] = make_float2(top, sum * off_reference(top, ref));
         }
     }
 };
@@ -596,11 +602,13 @@ struct WeightGradOps {
 };
 
 // ---------------------------------------------------------------- joining the row statistics
+// By differences of the maxima, so that the side that holds the larger one keeps its sum as it is: a row is
+// joined some tens of times, and any factor but 1 there would be an error that many times over.
 struct MaxSum { float m, s; };                       // sum of exponentials relative to the maximum
 __device__ __forceinline__ MaxSum joined(const MaxSum a, const MaxSum b) {
     const float m = fmaxf(a.m, b.m);
-    const float ref = m == -INFINITY ? 0.0f : m * kLog2e;
-    return {m, fmaf(a.s, exp2f(fmaf(a.m, kLog2e, -ref)), b.s * exp2f(fmaf(b.m, kLog2e, -ref)))};
+    const float fa = a.m == m ? 1.0f : exp2f((a.m - m) * kLog2e), fb = b.m == m ? 1.0f : exp2f((b.m - m) * kLog2e);
+    return {m, fmaf(a.s, fa, b.s * fb)};
 }
 
 // Loss and log-sum-exp of a row whose target's logit is z and whose other entries are `a`.  The loss is
