@@ -10,7 +10,7 @@
 // product of its own.  loss = log(1 + sum of the others / the target's) then loses nothing when the
 // model is sure of the target, and the target's logit is as good as binary32 makes it (the
 // tensor cores cut where they add; the other logits' long sums are taken in parts for that).  Backward: for one piece of the vocabulary after the other the logits
-// are formed again, S goes to the workspace in 16 bits, and two products take it from there;
+// are formed again (the target's as in the forward pass), S goes to the workspace in 16 bits, and two products take it from there;
 // dX is carried from piece to piece in binary32.  8 N D V operations for a training step: 2
 // forward, 2 again for the logits, 4 for the gradients.  Bound by the tensor cores, for a few
 // rows by the read of W.
@@ -155,15 +155,38 @@ __device__ __forceinline__ void find_row(const int* __restrict__ targets, const 
     *target = r < total ? found[1] : 0;
 }
 
+// A target's logit, the dot product of its hidden state and its row of W in binary32.  Both passes take it
+// in the same order, 128 threads with eight columns each at a time (VEC: the hidden state begins on a
+// 16-byte boundary, as the table's rows do), so that the backward pass has the forward pass's bits.
+constexpr int kDotThreads = kGatherThreads;
+template <typename T>
+__device__ __forceinline__ void dot_eight(const Raw8<T>& x, const T* w, float* dot) {
+    float a[8], b[8];
+    widen8<T>(x, a);
+    widen8<T>(load8<T, true>(w), b);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) *dot = fmaf(a[k], b[k], *dot);
+}
+template <typename T>
+__device__ __forceinline__ float dot_share(const T* x, const T* w, const int dim, const bool vec, const int tid) {
+    float dot = 0.0f;
+    const int groups = vec ? dim >> 3 : 0;
+    for (int g = tid; g < groups; g += kDotThreads) dot_eight<T>(load8<T, false>(x + g * 8), w + g * 8, &dot);
+    for (int c = groups * 8 + tid; c < dim; c += kDotThreads) dot = fmaf(to_f32<T>(x[c]), to_f32<T>(w[c]), dot);
+    return dot;
+}
+
 // Gathers the hidden states of the rows with a target, zeroes the rows behind them up to a
-// whole tile, and clears the outputs of rows without a target.  One CTA per row.  With
-// target_logit (forward) it also takes the dot product of the row with its target's row of W.
+// whole tile, and clears the outputs of rows without a target.  One CTA per row.  It also takes the logit z of
+// the row's target, and leaves that (forward), or, given the rows' log-sum-exp (backward), the target's entry
+// of softmax - onehot, exp(z - lse) - 1.
 template <typename T>
 __global__ void __launch_bounds__(kGatherThreads)
 xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n, const int dim, const int vocab, const int* __restrict__ targets,
                    int* rows, int* target, XentScalars* sc, const bool few, T* __restrict__ packed,
-                   const long long ld_packed, const T* __restrict__ weight, const long long ld_weight, float* __restrict__ target_logit,
-                   float* __restrict__ losses, float* __restrict__ lse, T* __restrict__ dhidden, const bool vec, const bool vec_out) {
+                   const long long ld_packed, const T* __restrict__ weight, const long long ld_weight, float* __restrict__ of_target,
+                   const float* __restrict__ lse_given, float* __restrict__ losses, float* __restrict__ lse, T* __restrict__ dhidden, const bool vec,
+                   const bool vec_out) {
     __shared__ float warp_sum[kGatherThreads / 32];
     const int r = blockIdx.x, tid = threadIdx.x;
     chain_begin();
@@ -201,35 +224,29 @@ xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n
         return;
     }
     const T* from = hidden + (long long)row * ld;
-    const T* w = target_logit ? weight + (long long)goal * ld_weight : nullptr;
-    float dot = 0.0f;
+    const T* w = weight + (long long)goal * ld_weight;
+    const float norm = lse_given ? __ldg(lse_given + row) : 0.0f;
+    float dot = 0.0f;                                                  // as dot_share takes it
     int c0 = 0;
     if (vec) {
         c0 = groups * 8;
         for (int g = tid; g < groups; g += kGatherThreads) {
             const Raw8<T> x = load8<T, false>(from + g * 8);
             *reinterpret_cast<uint4*>(to + g * 8) = x.a;
-            if (w) {
-                float a[8], b[8];
-                widen8<T>(x, a);
-                widen8<T>(load8<T, true>(w + g * 8), b);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) dot = fmaf(a[k], b[k], dot);
-            }
+            dot_eight<T>(x, w + g * 8, &dot);
         }
     }
     for (int c = c0 + tid; c < dim; c += kGatherThreads) {
         to[c] = from[c];
-        if (w) dot = fmaf(to_f32<T>(from[c]), to_f32<T>(w[c]), dot);
+        dot = fmaf(to_f32<T>(from[c]), to_f32<T>(w[c]), dot);
     }
-    if (!w) return;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
     if ((tid & 31) == 0) warp_sum[tid >> 5] = dot;
     __syncthreads();
     if (tid == 0) {
         for (int k = 1; k < kGatherThreads / 32; ++k) dot += warp_sum[k];
-        target_logit[r] = dot;
+        of_target[r] = lse_given ? expm1f(dot - norm) : dot;
     }
 }
 
@@ -365,7 +382,10 @@ struct FewStatsOps {
     }
 };
 
-// S of one tile, rounded to 16 bits, into the workspace; zeros behind the last row and column.
+// S of one tile, rounded to 16 bits, into the workspace; zeros behind the last row and column.  The target's
+// entry comes from its binary32 logit (xent_gather_kernel).  From the product's it would be a difference of nearly
+// equal numbers for a model that is sure: the tensor cores cut where they add, the log-sum-exp does not go along,
+// and where p is 0.999 it was off by 15 % at 4,096 columns and by 30 % at 8,192, always to the same side.
 template <typename T>
 struct SoftmaxGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
@@ -377,6 +397,7 @@ struct SoftmaxGradOps {
     const int* target;
     const int* rows;
     const float* lse;            // by row of the caller
+    const float* own;            // the targets' entries, by row
     CUtensorMap ds;
     int dim, v0, v1, group, a0, b0;
     static constexpr int kNoRow = INT_MIN;   // `at` of a row behind the last one
@@ -399,9 +420,10 @@ struct SoftmaxGradOps {
         for (int j = 0; j < 128; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -row.ref));
         const int at = row.at == kNoRow ? -1 : row.at - half * 128;
         if ((unsigned)at < 128u) {
+            const float x = __ldg(own + tile.m * kTileM + in_tile) * Half16<T>::kUp;
 #pragma unroll
             for (int j = 0; j < 128; ++j)
-                if (at == j) v[j] -= Half16<T>::kUp;
+                if (at == j) v[j] = x;
         }
         if (row.at == kNoRow) {                                           // whatever its logits: 0 times an infinity of the table is NaN
 #pragma unroll
@@ -630,7 +652,7 @@ __device__ __forceinline__ RowLoss row_loss(const float z, const MaxSum a) {
 // is 4 times as long and took 17 us instead of 9 at 1,640 rows), or 1 in a small call.
 template <int ROWS>
 __global__ void __launch_bounds__(256)
-xent_join_kernel(XentScalars* sc, const float2* __restrict__ stats, const int rows_cap, const int tiles, const float* __restrict__ target_logit,
+xent_join_kernel(XentScalars* sc, const float2* __restrict__ stats, const int rows_cap, const int tiles, const float* __restrict__ of_target,
                  const int* __restrict__ rows, float* __restrict__ losses, float* __restrict__ lse, float* partial, float* __restrict__ total,
                  const int mean, const int* status) {
     constexpr int WAYS = 256 / ROWS;
@@ -657,7 +679,7 @@ xent_join_kernel(XentScalars* sc, const float2* __restrict__ stats, const int ro
         float loss = 0.0f;
         if (y == 0 && row < count) {
             a = part[0][x];
-            const RowLoss of = row_loss(target_logit[row], a);
+            const RowLoss of = row_loss(of_target[row], a);
             loss = of.loss;
             losses[rows[row]] = loss;
             lse[rows[row]] = of.lse;
@@ -689,22 +711,19 @@ xent_join_kernel(XentScalars* sc, const float2* __restrict__ stats, const int ro
 template <typename T>
 __global__ void __launch_bounds__(256)
 xent_few_join_kernel(XentScalars* sc, const T* __restrict__ hidden, const long long ld, const T* __restrict__ weight, const long long ld_weight,
-                     const int* __restrict__ targets, const int dim, const int vocab, const float2* __restrict__ stats, const int rows_cap, const int pieces,
+                     const int* __restrict__ targets, const int dim, const int vocab, const bool vec, const float2* __restrict__ stats, const int rows_cap, const int pieces,
                      float* __restrict__ losses, float* __restrict__ lse, float* partial, float* __restrict__ total, const int mean, const int* status) {
     __shared__ MaxSum part[256];
-    __shared__ float dots[8];
+    __shared__ float dots[kDotThreads / 32];
     __shared__ int is_last;
     const int row = blockIdx.x, n = gridDim.x, tid = threadIdx.x;
     const int goal = __ldg(targets + row);
     const bool live = goal >= 0 && goal < vocab;
     float z = 0.0f;
-    if (live) {
-        const T *x = hidden + row * ld, *w = weight + goal * ld_weight;
-        for (int c = tid; c < dim; c += 256) z = fmaf(to_f32<T>(x[c]), to_f32<T>(w[c]), z);
-    }
+    if (live && tid < kDotThreads) z = dot_share<T>(hidden + row * ld, weight + goal * ld_weight, dim, vec, tid);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    if ((tid & 31) == 0) dots[tid >> 5] = z;
+    if ((tid & 31) == 0 && tid < kDotThreads) dots[tid >> 5] = z;
     chain_begin();
     MaxSum a = {-INFINITY, 0.0f};
     if (live)
@@ -720,7 +739,8 @@ xent_few_join_kernel(XentScalars* sc, const T* __restrict__ hidden, const long l
         float loss = 0.0f, l = 0.0f;
         if (live) {
             z = dots[0];
-            for (int k = 1; k < 8; ++k) { z += dots[k]; a = joined(a, part[k]); }
+            for (int k = 1; k < kDotThreads / 32; ++k) z += dots[k];
+            for (int k = 1; k < 8; ++k) a = joined(a, part[k]);
             const RowLoss of = row_loss(z, a);
             loss = of.loss;
             l = of.lse;
@@ -861,8 +881,8 @@ static int logits_group(const gm_linear_xent_t* h) {
 
 struct XentSpace {
     int64_t cap, ld_packed;                          // rows up to a whole tile, stride of the gathered hidden states
-    int64_t scalars, rows, target, packed;           // both passes
-    int64_t stats, target_logit, partial;            // forward
+    int64_t scalars, rows, target, of_target, packed;  // both passes
+    int64_t stats, partial;                          // forward
     int64_t parts, carried, ld_carried, ds, width;   // backward
     int64_t total;
 };
@@ -873,7 +893,8 @@ static XentSpace common_space(const gm_linear_xent_t* h) {
     s.ld_packed = (h->dim + 7) / 8 * 8;
     s.rows = 256;
     s.target = s.rows + up256(s.cap * 4);
-    s.packed = s.target + up256(s.cap * 4);
+    s.of_target = s.target + up256(s.cap * 4);
+    s.packed = s.of_target + up256(s.cap * 4);
     s.total = s.packed + up256(s.cap * s.ld_packed * 2);
     return s;
 }
@@ -884,8 +905,7 @@ static XentSpace forward_space(const gm_linear_xent_t* h) {
     // a few rows: eight pieces per tile of at least 16 entries, and no more tiles than rounds of half the SMs
     const int64_t few_tiles = (h->vocab + 15) / 16 < 1024 ? (h->vocab + 15) / 16 : 1024 + (h->vocab + 127) / 128;
     const int64_t stat_tiles = h->tokens <= kFewRows ? few_tiles * 8 : (h->vocab + kTileN / 2 - 1) / (kTileN / 2);
-    s.target_logit = s.stats + up256(stat_tiles * s.cap * 8);
-    s.partial = s.target_logit + up256(s.cap * 4);
+    s.partial = s.stats + up256(stat_tiles * s.cap * 8);
     s.total = s.partial + up256(s.cap * 4);
     return s;
 }
@@ -949,10 +969,11 @@ struct XentCall {
     XentScalars* sc() const { return (XentScalars*)(ws + s.scalars); }
     int* rows() const { return (int*)(ws + s.rows); }
     int* target() const { return (int*)(ws + s.target); }
+    float* of_target() const { return (float*)(ws + s.of_target); }      // the targets' logits, or their entries of softmax - onehot
 };
 
 template <typename T>
-static int index_and_gather(const XentCall& c, uintptr_t hidden, uintptr_t targets, uintptr_t weight, float* target_logit, float* losses, float* lse,
+static int index_and_gather(const XentCall& c, uintptr_t hidden, uintptr_t targets, uintptr_t weight, const float* lse_given, float* losses, float* lse,
                             T* dhidden) {
     const gm_linear_xent_t* h = c.h;
     const bool few = h->tokens <= kFewIndex;
@@ -965,7 +986,8 @@ static int index_and_gather(const XentCall& c, uintptr_t hidden, uintptr_t targe
     const bool vec_out = (uintptr_t)dhidden % 16 == 0 && h->ld_hidden % 8 == 0;
     GM_CUDA_CHECK(launch_chained(xent_gather_kernel<T>, dim3((unsigned)c.s.cap), dim3(kGatherThreads), 0, c.d->stream, (const T*)hidden, h->ld_hidden,
                                  (int)h->tokens, (int)h->dim, (int)h->vocab, (const int*)targets, c.rows(), c.target(), c.sc(), few,
-                                 (T*)(c.ws + c.s.packed), c.s.ld_packed, (const T*)weight, h->ld_weight, target_logit, losses, lse, dhidden, vec, vec_out));
+                                 (T*)(c.ws + c.s.packed), c.s.ld_packed, (const T*)weight, h->ld_weight, c.of_target(), lse_given, losses, lse, dhidden, vec,
+                                 vec_out));
     c.d->launches++;
     return GM_OK;
 }
@@ -995,7 +1017,7 @@ static int forward_few(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
     if (dim > kOneSum) GM_TRY(product(FewStatsOps<T, TN, true>{c.sc(), (const int*)targets, stats, n, cap, dim, vocab, height, 0, 0}));
     else GM_TRY(product(FewStatsOps<T, TN, false>{c.sc(), (const int*)targets, stats, n, cap, dim, vocab, height, 0, 0}));
     GM_CUDA_CHECK(launch_chained(xent_few_join_kernel<T>, dim3((unsigned)h->tokens), dim3(256), 0, c.d->stream, c.sc(), (const T*)hidden, h->ld_hidden,
-                                 (const T*)weight, h->ld_weight, (const int*)targets, (int)h->dim, (int)h->vocab, stats, (int)s.cap, (int)tiles * 8, losses, lse,
+                                 (const T*)weight, h->ld_weight, (const int*)targets, (int)h->dim, (int)h->vocab, in_place, stats, (int)s.cap, (int)tiles * 8, losses, lse,
                                  (float*)(c.ws + s.partial), total, h->mean, reinterpret_cast<const int*>(c.d->scalars + kXentStatusWord)));
     c.d->launches++;
     return GM_OK;
@@ -1013,8 +1035,7 @@ static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
     CUtensorMap map_w, map_x;
     GM_TRY(make_map(&map_w, h->dtype, weight, h->vocab, h->dim, h->ld_weight, kHalf));
     GM_TRY(make_map(&map_x, h->dtype, c.ws + s.packed, s.cap, h->dim, s.ld_packed, kHalf));
-    float* target_logit = (float*)(c.ws + s.target_logit);
-    GM_TRY(index_and_gather<T>(c, hidden, targets, weight, target_logit, losses, lse, (T*)nullptr));
+    GM_TRY(index_and_gather<T>(c, hidden, targets, weight, nullptr, losses, lse, (T*)nullptr));
     float2* stats = (float2*)(c.ws + s.stats);
     const int64_t n_tiles = (h->vocab + kTileN - 1) / kTileN;
     const int tiles = (int)((h->vocab + kTileN / 2 - 1) / (kTileN / 2));
@@ -1025,7 +1046,7 @@ static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, ui
     // a CTA per row up to a few rows per SM, 8 rows per CTA beyond
     auto join = h->tokens <= 1024 ? xent_join_kernel<1> : xent_join_kernel<8>;
     const int64_t ctas = h->tokens <= 1024 ? h->tokens : s.cap / 8;
-    GM_CUDA_CHECK(launch_chained(join, dim3((unsigned)ctas), dim3(256), 0, c.d->stream, c.sc(), stats, (int)s.cap, tiles, target_logit, c.rows(), losses, lse,
+    GM_CUDA_CHECK(launch_chained(join, dim3((unsigned)ctas), dim3(256), 0, c.d->stream, c.sc(), stats, (int)s.cap, tiles, c.of_target(), c.rows(), losses, lse,
                                  (float*)(c.ws + s.partial), total, h->mean, reinterpret_cast<const int*>(c.d->scalars + kXentStatusWord)));
     c.d->launches++;
     return GM_OK;
@@ -1047,7 +1068,7 @@ static int backward_pieces(const XentCall& c, uintptr_t hidden, uintptr_t weight
     GM_TRY(make_map(&ds_mn, h->dtype, ds, s.cap, s.width, s.width, kTileK));
     GM_TRY(make_map(&ds_out, h->dtype, ds, s.cap, s.width, s.width, 32));
     if (MAP) GM_TRY(make_map(&dw_out, h->dtype, dweight, h->vocab, h->dim, h->ld_weight, 32));
-    GM_TRY(index_and_gather<T>(c, hidden, targets, 0, nullptr, nullptr, nullptr, (T*)dhidden));
+    GM_TRY(index_and_gather<T>(c, hidden, targets, weight, lse, nullptr, nullptr, (T*)dhidden));
     const GradScale scale{scale_device, grad_scale, h->mean, 1.0f / Half16<T>::kUp};
     const int dim = (int)h->dim, vocab = (int)h->vocab;
     const int64_t m_tiles = s.cap / kTileM, d_tiles = (h->dim + kTileN - 1) / kTileN;
@@ -1056,7 +1077,7 @@ static int backward_pieces(const XentCall& c, uintptr_t hidden, uintptr_t weight
     for (int64_t v = 0; v < vocab; v += s.width) {
         const int v0 = (int)v, v1 = (int)(v + s.width < vocab ? v + s.width : vocab);
         const int64_t v_tiles = (v1 - v0 + kTileN - 1) / kTileN;
-        const SoftmaxGradOps<T> grad{c.sc(), c.target(), c.rows(), lse, ds_out, dim, v0, v1, logits_group(h), 0, v0};
+        const SoftmaxGradOps<T> grad{c.sc(), c.target(), c.rows(), lse, c.of_target(), ds_out, dim, v0, v1, logits_group(h), 0, v0};
         GM_TRY((launch_tiles<kTileN>(c.d, Product<SoftmaxGradOps<T>, false, false>{x_k, w_k, grad}, m_tiles * v_tiles)));
         const HiddenPlan shape{dim, v0, v1, (int)split_parts(h)};
         const HiddenOut<T> out{(float*)(c.ws + s.carried), s.ld_carried, (T*)dhidden, h->ld_hidden, scale, v0 == 0, v1 == vocab,
