@@ -278,6 +278,7 @@ struct StatsOps {
         return whole_tiles(count, (count + kTileM - 1) / kTileM, (vocab + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, group);
     }
     __device__ __forceinline__ Nothing once(const TilePlan&) const { return {}; }
+    __device__ __forceinline__ void gave_up(const TilePlan&, const TileAt&, int, int) const {}     // the status is read behind it
     __device__ __forceinline__ Goal prepare(const TilePlan& plan, const TileAt& tile, int in_tile) const {
         const int row = tile.m * kTileM + in_tile;
         return {row < plan.count ? __ldg(target + row) - tile.n * kTileN : -1};
@@ -348,6 +349,7 @@ struct FewStatsOps {
         return whole_tiles(n, (vocab + 2 * height - 1) / (2 * height), 1, (dim + kTileK - 1) / kTileK, 1);
     }
     __device__ __forceinline__ Nothing once(const TilePlan&) const { return {}; }
+    __device__ __forceinline__ void gave_up(const TilePlan&, const TileAt&, int, int) const {}     // the status is read behind it
     __device__ __forceinline__ Goal prepare(const TilePlan&, const TileAt&, int) const { return {0}; }
     __device__ __forceinline__ void epilogue(const TilePlan&, const TileAt& tile, int in_tile, float (&all)[kColumns], int half, unsigned, Nothing, const Goal) const {
         const int cta = in_tile / kHalf, local = in_tile % kHalf, lane = threadIdx.x & 31;
@@ -407,6 +409,7 @@ struct SoftmaxGradOps {
         return whole_tiles(count, (count + kTileM - 1) / kTileM, (v1 - v0 + kTileN - 1) / kTileN, (dim + kTileK - 1) / kTileK, group);
     }
     __device__ __forceinline__ Nothing once(const TilePlan&) const { return {}; }
+    __device__ __forceinline__ void gave_up(const TilePlan&, const TileAt&, int, int) const {}     // the status is read behind it
     __device__ __forceinline__ Row prepare(const TilePlan& plan, const TileAt& tile, int in_tile) const {
         const int row = tile.m * kTileM + in_tile;
         if (row >= plan.count) return {kNoRow, 0.0f};
@@ -439,8 +442,10 @@ struct SoftmaxGradOps {
     }
 };
 
-// What both gradient products multiply by.
+// What both gradient products multiply by.  NaN once a wait has run out, in this call or before: an optimizer
+// step that follows without a look at the status then finds a gradient that it must not take.
 struct GradScale {
+    const int* status;
     const float* scale;          // device scalar (the loss scale), or null
     float grad_scale;
     int mean;
@@ -448,6 +453,7 @@ struct GradScale {
     __device__ __forceinline__ float value(int count) const {
         float c = scale ? __fmul_rn(grad_scale, *scale) : grad_scale;
         if (mean) c = __fdiv_rn(c, (float)(count > 0 ? count : 1));
+        if (*(const volatile int*)status) c = NAN;
         return c * down;
     }
 };
@@ -527,6 +533,13 @@ struct HiddenGradOps {
     int a0, b0;
     __device__ __forceinline__ TilePlan plan(int pairs) const { return shape.plan(sc->count, pairs); }
     __device__ __forceinline__ float once(const TilePlan& plan) const { return out.scale.value(plan.count); }
+    __device__ __forceinline__ void gave_up(const TilePlan& plan, const TileAt& tile, int in_tile, int half) const {
+        const int row = tile.m * kTileM + in_tile, col = tile.n * kTileN + half * 128;
+        if (row >= plan.count || col >= shape.dim) return;
+        if (tile.part >= 0) parts[(long long)tile.part * (kTileM * kTileN) + in_tile * kTileN + half * 128] = NAN;
+        else if (out.last) out.out[(long long)rows[row] * out.ld_out + col] = from_f32<T>(NAN);
+        else out.carried[(long long)row * out.ld_carried + col] = NAN;
+    }
     // the caller's row, -1 behind the last one
     __device__ __forceinline__ int prepare(const TilePlan& plan, const TileAt& tile, int in_tile) const {
         const int row = tile.m * kTileM + in_tile;
@@ -601,6 +614,10 @@ struct WeightGradOps {
         return whole_tiles(count, (v1 - v0 + kTileM - 1) / kTileM, (dim + kTileN - 1) / kTileN, (count + kTileK - 1) / kTileK, kGroupM);
     }
     __device__ __forceinline__ float once(const TilePlan& plan) const { return scale.value(plan.count); }
+    __device__ __forceinline__ void gave_up(const TilePlan&, const TileAt& tile, int in_tile, int half) const {
+        const int row = tile.m * kTileM + in_tile, col = tile.n * kTileN + half * 128;
+        if (row < v1 - v0 && col < dim) out[(long long)(v0 + row) * ld_out + col] = from_f32<T>(NAN);
+    }
     __device__ __forceinline__ Nothing prepare(const TilePlan&, const TileAt&, int) const { return {}; }
     __device__ __forceinline__ void epilogue(const TilePlan&, const TileAt& tile, int in_tile, float (&v)[128], int half, unsigned stage,
                                              const float c_all, Nothing) const {
@@ -1069,7 +1086,7 @@ static int backward_pieces(const XentCall& c, uintptr_t hidden, uintptr_t weight
     GM_TRY(make_map(&ds_out, h->dtype, ds, s.cap, s.width, s.width, 32));
     if (MAP) GM_TRY(make_map(&dw_out, h->dtype, dweight, h->vocab, h->dim, h->ld_weight, 32));
     GM_TRY(index_and_gather<T>(c, hidden, targets, weight, lse, nullptr, nullptr, (T*)dhidden));
-    const GradScale scale{scale_device, grad_scale, h->mean, 1.0f / Half16<T>::kUp};
+    const GradScale scale{reinterpret_cast<const int*>(c.d->scalars + kXentStatusWord), scale_device, grad_scale, h->mean, 1.0f / Half16<T>::kUp};
     const int dim = (int)h->dim, vocab = (int)h->vocab;
     const int64_t m_tiles = s.cap / kTileM, d_tiles = (h->dim + kTileN - 1) / kTileN;
     using Hidden = Product<HiddenGradOps<T>, false, true>;

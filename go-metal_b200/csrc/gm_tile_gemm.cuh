@@ -25,7 +25,8 @@
 // pattern; an MN-major tile is blocks of 64 columns by 64 K-rows (8 KB each).
 //
 // Every wait is bounded: one that runs out raises the CTA's abort flag and *status, all
-// roles leave their loops, copies in flight are waited for (bounded again) and TMEM is freed.
+// roles leave their loops, copies in flight are waited for (bounded again) and TMEM is freed.  An epilogue
+// whose accumulators did not come marks its tile with NaN, so that the outputs show it.
 #pragma once
 
 #include <cuda.h>
@@ -330,6 +331,7 @@ __device__ __forceinline__ void split_tail(TilePlan* p, int pairs, int most_part
 //   epilogue(plan, at, row, v, half, stage, once, prepared)   the row inside the tile, half of its
 //                     columns (zeros with an empty share of K), which half, 4 KB of shared memory for
 //                     the warp (with kStaging); called by whole warps, also for rows behind the last one
+//   gave_up(plan, at, row, half)   a NaN into what this thread would have written
 template <typename Ops_, bool MN_A, bool MN_B>
 struct Product {
     using Ops = Ops_;
@@ -514,10 +516,19 @@ tile_gemm_kernel(const __grid_constant__ First first, const __grid_constant__ Se
             else return Nothing{};
         }();
         bool ok = true;
-        for (int t = pair; t < all && ok; t += pairs) {
+        int t = pair;
+        for (; t < all && ok; t += pairs) {
             if constexpr (Second::kAny)
                 if (t >= items) { ok = finish(second, plan2, once2, plan2.at(t - items)); continue; }
             ok = finish(first, plan, once, plan.at(t));
+        }
+        if (!ok) {
+            t -= pairs;                                          // the turn that did not end; its tile is this warp's alone
+            bool of_second = false;
+            if constexpr (Second::kAny) of_second = t >= items;
+            if (!of_second) first.ops.gave_up(plan, plan.at(t), row, half);
+            if constexpr (Second::kAny)
+                if (of_second) second.ops.gave_up(plan2, plan2.at(t - items), row, half);
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }

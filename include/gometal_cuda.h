@@ -413,8 +413,10 @@ int gm_linear_xent_backward_async(uintptr_t device_ptr, const gm_linear_xent_t* 
                                   float grad_scale, uintptr_t dhidden, uintptr_t dweight, int accumulate_dweight,
                                   uintptr_t workspace, int64_t workspace_bytes);
 /* Waits for the device's stream; GM_ERR_TIMEOUT when a bounded wait inside one of these
- * products ran out since the last query (that call's outputs are not complete; a forward
- * pass reports NaN as its total until the query). */
+ * products ran out since the last query.  That call's outputs are not complete, and until the query
+ * it and every later one show it: a forward pass reports NaN as its total, a backward pass NaN in its
+ * gradients (in all of dW and of the rows of dX with a target where it began after the wait ran out), which
+ * the overflow check of a mixed-precision step finds and skips. */
 int gm_linear_xent_status(uintptr_t device_ptr);
 
 /* ---- ZeRO-1: sharded state + all-gather of updated parameters ---- */
@@ -498,8 +500,8 @@ int gm_selftest_const_div(uintptr_t device_ptr, float c, uint64_t* mismatches, u
 int gm_selftest_barrier_timeout(uintptr_t device_ptr, long long budget_cycles, int* gave_up);
 
 /* The same for the products of the vocabulary loss: runs their bounded wait on a barrier that
- * nothing arrives at.  *gave_up must be 1; afterwards a forward pass reports NaN as its total and
- * gm_linear_xent_status returns GM_ERR_TIMEOUT once, as after a product whose wait ran out. */
+ * nothing arrives at.  *gave_up must be 1; afterwards a forward pass reports NaN as its total, a backward
+ * pass NaN in its gradients, and gm_linear_xent_status returns GM_ERR_TIMEOUT once, as after a product whose wait ran out. */
 int gm_selftest_xent_timeout(uintptr_t device_ptr, long long budget_cycles, int* gave_up);
 
 /* ---- timing on the device's stream (CUDA events) ---- */
