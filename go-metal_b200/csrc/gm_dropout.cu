@@ -40,6 +40,7 @@ int check_matrix(int64_t rows, int64_t cols, int64_t ld, const char* what) {
     }
     if (ld > 0x7fffffffLL) { set_error("%s: row stride %lld is outside [1, 2^31)", what, (long long)ld); return GM_ERR_BAD_SIZE; }
     if (ld < cols) { set_error("%s: row stride %lld is smaller than its %lld columns", what, (long long)ld, (long long)cols); return GM_ERR_BAD_ARG; }
+    if (rows * ld > (1LL << 60)) { set_error("%s: %lld rows of stride %lld hold more than 2^60 elements", what, (long long)rows, (long long)ld); return GM_ERR_BAD_SIZE; }
     return GM_OK;
 }
 

@@ -258,8 +258,9 @@ int make_drop(const Device* d, const gm_dropout_t* in, Drop* out);
 // A buffer of at least `need` bytes on this device, aligned to `align`; need 0 checks the rest.
 int check_buffer(const Device* d, uintptr_t p, int64_t need, int64_t align, const char* what);
 
-// Rows and row stride below 2^31, at most 2^30 columns (column arithmetic is in 32 bits), and a stride
-// that covers the columns.
+// Rows and row stride below 2^31, at most 2^30 columns (column arithmetic is in 32 bits), a stride
+// that covers the columns, and at most 2^60 elements, so that no count of bytes passes 64 bits (a wrapped
+// one would let a small buffer pass for large enough).
 int check_matrix(int64_t rows, int64_t cols, int64_t ld, const char* what);
 
 // Bytes from a matrix's first element to behind its last one.

@@ -335,8 +335,8 @@ int gm_dot_canonical_static(uintptr_t a, uintptr_t b, int64_t n, uintptr_t out_d
  * captured into a graph (on gm_device_stream).  Workspaces are the caller's, 256-byte aligned,
  * and hold nothing between calls; two calls or captured graphs that can run at the same
  * time need workspaces of their own.  Matrices are row-major with a row stride (ld, in
- * elements) of at least their columns, below 2^31 rows and at most 2^30 columns.  Buffers are read and written only inside the
- * rows and columns named.  What a call writes overlaps nothing else it reads or writes, except where
+ * elements) of at least their columns, below 2^31 rows, at most 2^30 columns and 2^60 elements.  Buffers are read and
+ * written only inside the rows and columns named.  What a call writes overlaps nothing else it reads or writes, except where
  * it says so. */
 
 /* Element types: the codes of memory/tensor.go:12-17, and one more for bfloat16. */
