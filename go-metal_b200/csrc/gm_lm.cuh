@@ -75,8 +75,9 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float (
 }
 
 // Eight elements at any address, read as the 16-byte words that hold them (each word holds at least
-// one of the eight, so nothing outside their 16-byte words is touched) and shifted into place when
-// they are used.  Matrices whose rows do not begin on 16-byte boundaries come this way: element
+// one of the eight, so nothing outside their 16-byte words is touched, and no page that holds none of
+// them) and shifted into place when they are used; what else those words hold, which a neighbour may be writing,
+// falls out there.  Matrices whose rows do not begin on 16-byte boundaries come this way: element
 // by element the same traffic took 4 times as long.
 template <typename T> struct Any8 {
     uint4 a, b, c;               // c: fp32 only

@@ -335,9 +335,11 @@ int gm_dot_canonical_static(uintptr_t a, uintptr_t b, int64_t n, uintptr_t out_d
  * captured into a graph (on gm_device_stream).  Workspaces are the caller's, 256-byte aligned,
  * and hold nothing between calls; two calls or captured graphs that can run at the same
  * time need workspaces of their own.  Matrices are row-major with a row stride (ld, in
- * elements) of at least their columns, below 2^31 rows, at most 2^30 columns and 2^60 elements.  Buffers are read and
- * written only inside the rows and columns named.  What a call writes overlaps nothing else it reads or writes, except where
- * it says so. */
+ * elements) of at least their columns, below 2^31 rows, at most 2^30 columns and 2^60 elements.  Buffers are
+ * written only inside the rows and columns named.  They are read inside the aligned 16-byte words that hold
+ * those: up to 14 bytes in front of or behind a row whose begin or end lies inside such a word may be read too (never
+ * past the end of a page, and no result depends on them).  What a call writes overlaps nothing else it reads or
+ * writes, except where it says so. */
 
 /* Element types: the codes of memory/tensor.go:12-17, and one more for bfloat16. */
 enum { GM_F32 = 0, GM_F16 = 2, GM_BF16 = 4 };
