@@ -972,7 +972,9 @@ static int check_xent(const gm_linear_xent_t* h) {
     if (h->dtype != GM_F16 && h->dtype != GM_BF16) { set_error("element type %d is not Float16 or BFloat16", h->dtype); return GM_ERR_BAD_ARG; }
     GM_TRY(check_matrix(h->tokens, h->dim, h->ld_hidden, "hidden states"));
     GM_TRY(check_matrix(h->vocab, h->dim, h->ld_weight, "vocabulary table"));
-    if (h->tokens > (1LL << 28) || h->vocab > (1LL << 28) || h->dim > (1LL << 24)) { set_error("%lld tokens, %lld columns or %lld vocabulary entries are too many", (long long)h->tokens, (long long)h->dim, (long long)h->vocab); return GM_ERR_BAD_SIZE; }
+    // One tile of dW is a sum over all rows with a target: 2^26 of them are 2^20 blocks of 64 and 0.3 to 0.4 s, which
+    // the waits' default bound of 2^31 cycles (about 1.1 s) covers and 2^28 would not.
+    if (h->tokens > (1LL << 26) || h->vocab > (1LL << 28) || h->dim > (1LL << 24)) { set_error("%lld tokens, %lld columns or %lld vocabulary entries are too many", (long long)h->tokens, (long long)h->dim, (long long)h->vocab); return GM_ERR_BAD_SIZE; }
     if (up256(h->tokens) / 256 * (up256(h->vocab) / 256) > 0x3fffffffLL) { set_error("%lld tokens by %lld vocabulary entries are too many", (long long)h->tokens, (long long)h->vocab); return GM_ERR_BAD_SIZE; }
     if (h->ld_weight % 8) { set_error("the table's row stride %lld is not a multiple of 8 elements", (long long)h->ld_weight); return GM_ERR_BAD_ARG; }
     return GM_OK;

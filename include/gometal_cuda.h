@@ -335,7 +335,7 @@ int gm_dot_canonical_static(uintptr_t a, uintptr_t b, int64_t n, uintptr_t out_d
  * captured into a graph (on gm_device_stream).  Workspaces are the caller's, 256-byte aligned,
  * and hold nothing between calls; two calls or captured graphs that can run at the same
  * time need workspaces of their own.  Matrices are row-major with a row stride (ld, in
- * elements) of at least their columns, below 2^31 rows, at most 2^30 columns and 2^60 elements.  Buffers are
+ * elements) of at least their columns, 1 to below 2^31 rows, 1 to 2^30 columns, at most 2^60 elements.  Buffers are
  * written only inside the rows and columns named.  They are read inside the aligned 16-byte words that hold
  * those: up to 14 bytes in front of or behind a row whose begin or end lies inside such a word may be read too (never
  * past the end of a page, and no result depends on them).  What a call writes overlaps nothing else it reads or
@@ -395,7 +395,8 @@ int gm_embedding_backward_async(uintptr_t device_ptr, const gm_embedding_t* e, u
  * of the losses, rows with a target} (a mean over no rows is 0).  dX or dW may be 0.
  * The logits and both gradients are tensor-core products with binary32 sums; softmax - onehot is
  * rounded to the inputs' type in between.  The same call gives the same bits.
- * The table's rows begin on 16-byte boundaries (its address, and ld_weight a multiple of 8). */
+ * The table's rows begin on 16-byte boundaries (its address, and ld_weight a multiple of 8).
+ * At most 2^26 tokens, 2^28 vocabulary entries and 2^24 columns. */
 typedef struct {
     int dtype;                                   /* GM_F16 or GM_BF16: X, W, dX, dW */
     int64_t tokens, dim, vocab;
