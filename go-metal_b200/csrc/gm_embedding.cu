@@ -366,7 +366,8 @@ embedding_join_kernel(const unsigned long long* __restrict__ words, const float*
 // Sorted words per chunk: 32 in a large call, 16 or 8 where that would leave an SM fewer than 512
 // threads: the walk over a chunk is serial, and a small call is as long as one walk (4,095 x 1,000: 46
 // us with 8, 50 us with 16; 65,536 x 4,096: 0.32 ms with 32, 0.55 ms with 16, whose partial sums are
-// twice as many).
+// twice as many).  148 is the B200's number of SMs, written in because the workspace's size, which follows
+// from the chunks, is told without a device.
 static int piece_of(const gm_embedding_t* e) {
     const int64_t walks = e->tokens * ((e->dim + 7) / 8);              // one word each
     return walks >= 32LL * 148 * 512 ? 32 : walks >= 16LL * 148 * 512 ? 16 : 8;

@@ -7,11 +7,12 @@
 // Forward: one matrix product whose epilogue leaves, per row and 128 vocabulary entries, the
 // maximum and the sum of exponentials (8 bytes for 128 logits) of all entries but
 // the target's, then a small kernel joins them with the target's logit, which comes from a dot
-// product of its own.  loss = log(1 + sum of the others / the target's) then loses nothing when the
-// model is sure of the target, and the target's logit is as good as binary32 makes it (the
-// tensor cores cut where they add; the other logits' long sums are taken in parts for that).  Backward: for one piece of the vocabulary after the other the logits
-// are formed again (the target's as in the forward pass), S goes to the workspace in 16 bits, and two products take it from there;
-// dX is carried from piece to piece in binary32.  8 N D V operations for a training step: 2
+// product of its own.  loss = log(1 + sum of the others / the target's) then keeps its relative
+// accuracy when the model is sure of the target, and the target's logit is as good as binary32 makes it (the
+// tensor cores cut where they add; the other logits' long sums are taken in parts for that).  Backward: for one
+// piece of the vocabulary after the other the logits are formed again, the target's entry of S comes from its
+// binary32 logit as in the forward pass, S goes to the workspace in 16 bits, and two products take it from
+// there; dX is carried from piece to piece in binary32.  8 N D V operations for a training step: 2
 // forward, 2 again for the logits, 4 for the gradients.  Bound by the tensor cores, for a few
 // rows by the read of W.
 //
@@ -387,7 +388,8 @@ struct FewStatsOps {
 // S of one tile, rounded to 16 bits, into the workspace; zeros behind the last row and column.  The target's
 // entry comes from its binary32 logit (xent_gather_kernel).  From the product's it would be a difference of nearly
 // equal numbers for a model that is sure: the tensor cores cut where they add, the log-sum-exp does not go along,
-// and where p is 0.999 it was off by 15 % at 4,096 columns and by 30 % at 8,192, always to the same side.
+// and where p is 0.999 with a logit of 13 it was off by 35 % at 4,096 columns and by 70 % at 8,192, always to the same
+// side.  What is left is the rounding of the log-sum-exp: at most half a unit in its last place, and no wrong sign.
 template <typename T>
 struct SoftmaxGradOps {
     static constexpr bool kBf16 = Half16<T>::kBf16;
@@ -651,7 +653,8 @@ __device__ __forceinline__ MaxSum joined(const MaxSum a, const MaxSum b) {
 }
 
 // Loss and log-sum-exp of a row whose target's logit is z and whose other entries are `a`.  The loss is
-// taken as the logarithm of a sum, not as a difference, so a small loss keeps its bits.  A target with
+// taken as the logarithm of a sum, not as a difference, so a small loss is as good, relatively, as that sum
+// (3.5e-7 with 131,072 entries around 200).  A target with
 // logit -inf has an infinite loss, and a log-sum-exp that is its other entries'; with logit +inf both
 // the loss and its gradient are NaN, as inf - inf is.
 struct RowLoss { float loss, lse; };
@@ -1046,8 +1049,9 @@ template <typename T>
 static int run_forward(const XentCall& c, uintptr_t hidden, uintptr_t weight, uintptr_t targets, float* losses, float* lse, float* total) {
     const gm_linear_xent_t* h = c.h;
     const XentSpace& s = c.s;
-    // 16 x 1,024 x 32,000 takes 21, 23 and 27 us with tiles for 32, 64 and 128 rows, 64 rows 22 and 26 us,
-    // 128 rows 27 us, and 129 rows by the way below 38 us
+    // 16 x 1,024 x 32,000 takes 20.3, 20.3 and 24.1 us with tiles for 32, 64 and 128 rows and 26.2 us by the way below, 64 rows
+    // 20.8 and 25.1 us with tiles for 64 and 128 and 27.5 below, 128 rows 26.0 us and 27.1 below; larger tables: 16 x 4,096 x
+    // 131,072 with tiles for 32 and 64 rows 175.6 and 179.6 us
     if (h->tokens <= 32) return forward_few<T, 32>(c, hidden, weight, targets, losses, lse, total);
     if (h->tokens <= 64) return forward_few<T, 64>(c, hidden, weight, targets, losses, lse, total);
     if (h->tokens <= kFewRows) return forward_few<T, kFewRows>(c, hidden, weight, targets, losses, lse, total);
