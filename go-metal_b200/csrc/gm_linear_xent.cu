@@ -252,11 +252,18 @@ xent_gather_kernel(const T* __restrict__ hidden, const long long ld, const int n
 }
 
 // ---------------------------------------------------------------- epilogues
-// The exponentials of a piece are 2^(l log2e - ref) with ref = m log2e rounded, one operation each; their
-// sum is then relative to 2^ref, not to e^m, and those are apart by the rounding of ref (up to 11 units in the last
-// place at m = 20, a hundred at 200).  This takes it out, once per piece; 1 where the piece holds nothing but -inf.
-__device__ __forceinline__ float reference_of(const float m) { return m == -INFINITY ? 0.0f : m * kLog2e; }
-__device__ __forceinline__ float off_reference(const float m, const float ref) { return m == -INFINITY ? 1.0f : exp2f(-fmaf(m, kLog2e, -ref)); }
+// The exponentials of a piece are 2^(scale l - ref) with scale = log2e and ref = m log2e rounded, one operation
+// each; their sum is then relative to 2^ref, not to e^m, and those are apart by the rounding of ref (up to 11 units
+// in the last place at m = 20, a hundred at 200).  off() takes it out, once per piece.
+// Where m log2e would pass binary32 (a piece of nothing but bf16's lowest number, as masks have it) scale is 1 and ref is m:
+// logits of that size are equal to m or 1e31 and more below it, so any base gives 1 and 0.  A piece of nothing
+// but -inf has zeros.
+struct Reference {
+    float m, scale, ref;
+    __device__ __forceinline__ explicit Reference(const float top)
+        : m(top), scale(fabsf(top) > 2e38f ? 1.0f : kLog2e), ref(top == -INFINITY ? 0.0f : top * scale) {}
+    __device__ __forceinline__ float off() const { return m == -INFINITY ? 1.0f : exp2f(-fmaf(m, scale, -ref)); }
+};
 
 constexpr int kGroupM = 8;      // m-tiles walked together in the gradient products
 
@@ -306,11 +313,11 @@ struct StatsOps {
 #pragma unroll
         for (int j = 8; j < 128; ++j) top[j & 7] = fmaxf(top[j & 7], v[j]);
         const float m = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
-        const float ref = reference_of(m);
+        const Reference r(m);
 #pragma unroll
-        for (int j = 0; j < 128; ++j) sum[j & 7] += exp2_fast(fmaf(v[j], kLog2e, -ref));
+        for (int j = 0; j < 128; ++j) sum[j & 7] += exp2_fast(fmaf(v[j], r.scale, -r.ref));
         const float s = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
-        if (row < plan.count) stats[(long long)(2 * tile.n + half) * rows_cap + row] = make_float2(m, s * off_reference(m, ref));
+        if (row < plan.count) stats[(long long)(2 * tile.n + half) * rows_cap + row] = make_float2(m, s * r.off());
     }
 };
 
@@ -376,11 +383,12 @@ struct FewStatsOps {
 #pragma unroll
             for (int j = 0; j < 32; ++j) w[j] = v[j];
             const float top = lanes_to_columns<true>(w, lane);
-            const float ref = reference_of(top);
+            const Reference r(top);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -__shfl_sync(0xffffffffu, ref, j)));
+            for (int j = 0; j < 32; ++j)
+                v[j] = exp2_fast(fmaf(v[j], __shfl_sync(0xffffffffu, r.scale, j), -__shfl_sync(0xffffffffu, r.ref, j)));
             const float sum = lanes_to_columns<false>(v, lane);
-            if (c + lane < n) to[c + lane] = make_float2(top, sum * off_reference(top, ref));
+            if (c + lane < n) to[c + lane] = make_float2(top, sum * r.off());
         }
     }
 };

@@ -394,7 +394,8 @@ int gm_embedding_backward_async(uintptr_t device_ptr, const gm_embedding_t* e, u
  * gradient are 0 and it may hold anything.  losses, lse: one float per row; total: {sum or mean
  * of the losses, rows with a target} (a mean over no rows is 0).  dX or dW may be 0.
  * The logits and both gradients are tensor-core products with binary32 sums; softmax - onehot is
- * rounded to the inputs' type in between.  The same call gives the same bits.
+ * rounded to the inputs' type in between.  The backward pass has the probabilities from lse, so to |lse| 2^-24
+ * of themselves besides their logits' errors.  The same call gives the same bits.
  * The table's rows begin on 16-byte boundaries (its address, and ld_weight a multiple of 8).
  * At most 2^26 tokens, 2^28 vocabulary entries and 2^24 columns. */
 typedef struct {
